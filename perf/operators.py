@@ -25,30 +25,30 @@ _TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 def listed():
     return [
         # one token of a chat or of a preview, top 2 of 4 experts of the HiDream layer: weights are read once, latency counts
-        dict(name="experts, one token", op="experts", dtype="bf16", experts=4, tokens=1, top_k=2, k=2560, n=6912),
+        dict(name="experts one token", op="experts", dtype="bf16", experts=4, tokens=1, top_k=2, k=2560, n=6912),
         # a short prompt through 8 wider experts
-        dict(name="experts, 75 tokens", op="experts", dtype="bf16", experts=8, tokens=75, top_k=2, k=2048, n=8192),
+        dict(name="experts 75 tokens", op="experts", dtype="bf16", experts=8, tokens=75, top_k=2, k=2048, n=8192),
         # an image pair: 2 x 4096 tokens
-        dict(name="experts, 8192 tokens", op="experts", dtype="bf16", experts=4, tokens=8192, top_k=2, k=2560, n=6912),
+        dict(name="experts 8192 tokens", op="experts", dtype="bf16", experts=4, tokens=8192, top_k=2, k=2560, n=6912),
         # a small fine-tuning step in half precision, top 1, sizes that are no multiple of a tile
-        dict(name="experts train, odd", op="experts train", dtype="fp16", experts=8, tokens=1003, top_k=1, k=1000, n=2056),
+        dict(name="experts train odd", op="experts train", dtype="fp16", experts=8, tokens=1003, top_k=1, k=1000, n=2056),
         # a training step of a block with 8 experts
-        dict(name="experts train, 8192 tokens", op="experts train", dtype="bf16", experts=8, tokens=8192, top_k=2, k=2048,
+        dict(name="experts train 8192 tokens", op="experts train", dtype="bf16", experts=8, tokens=8192, top_k=2, k=2048,
              n=8192),
         # one row through a projection: the adaptive norm's input, a single token
-        dict(name="block, one row", op="block", dtype="bf16", rows=1, k=2560, n=6912, bias=False, grad=False),
+        dict(name="block one row", op="block", dtype="bf16", rows=1, k=2560, n=6912, bias=False, grad=False),
         # the text rows of an image pair through the second product of a feed-forward
-        dict(name="block, 768 rows", op="block", dtype="bf16", rows=768, k=6912, n=2560, bias=True, grad=False),
+        dict(name="block 768 rows", op="block", dtype="bf16", rows=768, k=6912, n=2560, bias=True, grad=False),
         # the image rows through the first product
-        dict(name="block, 8192 rows", op="block", dtype="bf16", rows=8192, k=2560, n=6912, bias=False, grad=False),
+        dict(name="block 8192 rows", op="block", dtype="bf16", rows=8192, k=2560, n=6912, bias=False, grad=False),
         # an adapter's training step through a frozen projection
-        dict(name="block train, 1999 rows", op="block", dtype="fp16", rows=1999, k=2560, n=2560, bias=True, grad=True),
-        dict(name="block experts, one token", op="block experts", dtype="bf16", experts=4, tokens=1, top_k=2, k=2560, n=6912,
+        dict(name="block train 1999 rows", op="block", dtype="fp16", rows=1999, k=2560, n=2560, bias=True, grad=True),
+        dict(name="block experts one token", op="block experts", dtype="bf16", experts=4, tokens=1, top_k=2, k=2560, n=6912,
              grad=False),
-        dict(name="block experts, 8192 tokens", op="block experts", dtype="bf16", experts=4, tokens=8192, top_k=2, k=2560,
+        dict(name="block experts 8192 tokens", op="block experts", dtype="bf16", experts=4, tokens=8192, top_k=2, k=2560,
              n=6912, grad=False),
         # an adapter's training step through frozen experts, odd rows
-        dict(name="block experts train, odd", op="block experts", dtype="bf16", experts=8, tokens=2051, top_k=1, k=2048,
+        dict(name="block experts train odd", op="block experts", dtype="bf16", experts=8, tokens=2051, top_k=1, k=2048,
              n=2064, grad=True),
     ]
 
