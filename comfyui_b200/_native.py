@@ -11,7 +11,7 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int6
 
 from . import build as _build
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 OK, EINVAL, EUNSUPPORTED, ECUDA, ETIMEOUT, EDEVICE, ETOOLARGE = range(7)
 BF16, FP32, FP8_E4M3, FP16 = 0, 1, 2, 3
@@ -20,6 +20,7 @@ TOKENS_PER_BLOCK = 32
 MAX_EXPERTS = 8
 STATIC_MAX_TOKENS = 131072
 STATUS_WORDS = 4         # [0] sticky device status, [1] near-ties of the last gate call, [2] e4m3 overflows, [3] reserved
+RAGGED_MAX_GROUPS = 1024     # COMFY_MOE_RAGGED_MAX_GROUPS: groups of one call over ragged rows
 LINEAR_MAX_MAPS = 22     # COMFY_MOE_LINEAR_MAX_MAPS: distinct operands of one comfy_moe_grouped_linear call
 MAX_RANKS = 8
 EP_ARRIVED, EP_DONE = 0, 1
@@ -55,6 +56,9 @@ EXPORTS = (
     "comfy_attn_rmsnorm_rope",
     "comfy_attn_forward",
     "comfy_moe_grouped_linear",
+    "comfy_moe_grouped_matmul",
+    "comfy_moe_grouped_matmul_dgrad",
+    "comfy_moe_grouped_matmul_wgrad",
     "comfy_moe_ep_dispatch",
     "comfy_moe_ep_signal",
     "comfy_moe_ep_wait",
@@ -299,6 +303,15 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
     lib.comfy_attn_forward.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
                                        c_void_p, c_void_p]
     lib.comfy_moe_grouped_linear.argtypes = [c_int, POINTER(LinearGroup), c_void_p, c_void_p]
+    lib.comfy_moe_grouped_matmul.argtypes = [
+        c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
+        c_void_p, c_int64, c_void_p, c_void_p,
+    ]
+    lib.comfy_moe_grouped_matmul_dgrad.argtypes = lib.comfy_moe_grouped_matmul.argtypes
+    lib.comfy_moe_grouped_matmul_wgrad.argtypes = [
+        c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+        c_int64, c_int64, c_void_p, c_void_p,
+    ]
     lib.comfy_moe_stochastic_round_e4m3.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p]
     lib.comfy_moe_quantize_weight_e4m3.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]
     lib.comfy_moe_ep_signal.argtypes = [POINTER(PeerPlan), c_int, c_uint32, c_void_p]

@@ -24,10 +24,11 @@ SOURCES = [
     "moe_peer.cu",
     "attn_glue.cu",
     "attn_fwd_sm100.cu",
+    "grouped_matmul_sm100.cu",
     "weight_ingest.cu",
     "moe_c_api.cu",
 ]
-HEADERS = ["moe_common.cuh", "ptx_sm100.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
+HEADERS = ["moe_common.cuh", "moe_gate.cuh", "ptx_sm100.cuh", "ragged.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
 
 
 def _nvcc() -> str:

@@ -84,28 +84,6 @@ struct AttnParams {
   float scale_log2;                            // softmax scale * log2(e)
 };
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      :
-      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-
-// Shared-memory descriptor of a B operand whose N dimension is the contiguous one (V: rows = keys = K of the MMA,
-// 64 head-dimension elements per 128-byte row, the other 64 in a second box `box_stride` bytes further), 128-byte
-// swizzle: leading byte offset = distance between the two 64-element column blocks, stride byte offset = distance
-// between groups of eight keys.
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t box_stride) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
-  d |= static_cast<uint64_t>((box_stride >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
 // D[tmem] (+)= A[tmem] * B[smem]: the A operand (P) is read from tensor memory.
 __device__ __forceinline__ void umma_ts_bf16(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
                                              uint32_t accumulate) {

@@ -1,0 +1,435 @@
+// Matrix products grouped by expert with ragged sizes, and their gradients, on tcgen05 tensor cores:
+//   forward   y[r, :]  = x[r, :] W[g]^T                 for the rows r of group g,   x [R, K], W [G, N, K], y [R, N]
+//   d x       dx[r, :] = dy[r, :] W[g]
+//   d W       dw[g]    = sum over the rows r of g of dy[r, :]^T x[r, :]              (zeros for a group without rows)
+// The groups' rows are read from the device (offsets, optional counts), so no call waits for the host.  All three run
+// on one kernel; what differs is which dimension of an operand is contiguous in memory.  tcgen05 reads both kinds from
+// shared memory (a K-major tile: rows of 64 elements of the contraction; an MN-major tile: 64 output elements per row,
+// one row per step of the contraction), so nothing is transposed in memory:
+//   forward: A = x (K-major), B = W[g] (K-major);   d x: A = dy (K-major), B = W[g] (MN-major);
+//   d W: A = dy, B = x, both MN-major, contraction over the group's rows.
+// A row of a tile depends on its own row of A only, so tiles of the first two may hang over the end of their group: the
+// loads take what follows, the stores leave it out.  In d W the rows behind the group are part of the sum: the MMA warp
+// overwrites them with zeros in shared memory (both operands: what stands there may be NaN) before it multiplies.
+#include "ragged.cuh"
+
+namespace comfy_b200 {
+
+enum RaggedForm { kForward = 0, kGradX = 1, kGradW = 2 };
+
+constexpr int kTileM = 128;
+constexpr int kStepK = 64;                     // contraction elements per stage: one 128-byte swizzled row
+constexpr int kABytes = kTileM * 128;
+constexpr int kMnBoxBytes = kStepK * 128;      // one box of an MN-major operand: 64 steps x 64 elements
+
+template <int kBN> struct GmmShape {
+  static constexpr int kStageBytes = kABytes + kBN * 128;
+  static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
+  static constexpr int kTmemCols = 2 * kBN;    // two accumulators: the epilogue of one tile overlaps the next one's MMAs
+  static constexpr int kTables = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
+};
+
+struct alignas(64) GmmParams {
+  CUtensorMap map_a, map_b, map_out;
+  const int32_t* offsets;
+  const int32_t* counts;
+  uint8_t* out;
+  int32_t* status;
+  long long ld_out;                            // bytes
+  int groups, rows;                            // rows of the buffers
+  int m_total;                                 // d W: rows of dw[g] (N); otherwise unused
+  int n_total;                                 // output columns
+  int k_total;                                 // contraction length (d W: the group's rows, unused)
+  int band;                                    // row tiles per band of the tile order
+  int zero_unused;
+  int fp16, out_fp32;
+  uint32_t idesc;
+};
+
+template <int kForm, int kBN>
+__global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
+  using Shape = GmmShape<kBN>;
+  constexpr int kStages = Shape::kStages;
+  constexpr int kStageBytes = Shape::kStageBytes;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
+  __shared__ __align__(8) uint64_t tmem_full_bar[2], tmem_empty_bar[2], drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
+  int* s_count = s_begin + p.groups;
+  int* s_first = s_count + p.groups;
+
+  const int n_tiles = (p.n_total + kBN - 1) / kBN;
+  const int m_tiles_w = (p.m_total + kTileM - 1) / kTileM;
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+      for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps); }
+      mbar_init(&drain_bar, 1);
+      fence_mbar_init();
+      abort_flag = 0;
+    }
+    __syncwarp();
+    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTileM,
+                  kForm == kGradW ? m_tiles_w * n_tiles : n_tiles, s_begin, s_count, s_first);
+  } else if (warp == 1) {
+    tmem_alloc(&tmem_slot, Shape::kTmemCols);
+    tmem_relinquish();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+  volatile int* abort_ptr = &abort_flag;
+  const int total = s_first[p.groups];
+  auto give_up = [&](int code) {
+    if (lane == 0) { atomicCAS(p.status, 0, code); abort_flag = 1; }
+  };
+
+  // Tiles t = blockIdx.x, + gridDim.x, ... in the order of the groups; g only ever moves forward.
+  struct Tile { int m0, n0, begin, count, steps; };
+  auto tile_at = [&](int t, int& g) {
+    while (t >= s_first[g + 1]) ++g;
+    Tile c;
+    c.begin = s_begin[g];
+    c.count = s_count[g];
+    int m, n;
+    ragged_tile(t - s_first[g], kForm == kGradW ? m_tiles_w : (c.count + kTileM - 1) / kTileM, n_tiles, p.band, m, n);
+    c.m0 = m * kTileM;
+    c.n0 = n * kBN;
+    c.steps = ((kForm == kGradW ? c.count : p.k_total) + kStepK - 1) / kStepK;
+    return c;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
+      const Tile c = tile_at(t, g);
+      for (int kb = 0; kb < c.steps; ++kb, ++it) {
+        const int s = it % kStages;
+        ok = mbar_wait_warp(&empty_bar[s], ((it / kStages) & 1u) ^ 1u, abort_ptr);
+        if (!ok) { give_up(kStatusRaggedProducer); break; }
+        uint8_t* a = smem + s * kStageBytes;
+        uint8_t* b = a + kABytes;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full_bar[s], kStageBytes);
+          if constexpr (kForm == kGradW) {
+#pragma unroll
+            for (int i = 0; i < kTileM / 64; ++i)
+              tma_load_2d(a + i * kMnBoxBytes, &p.map_a, &full_bar[s], c.m0 + i * 64, c.begin + kb * kStepK);
+#pragma unroll
+            for (int i = 0; i < kBN / 64; ++i)
+              tma_load_2d(b + i * kMnBoxBytes, &p.map_b, &full_bar[s], c.n0 + i * 64, c.begin + kb * kStepK);
+          } else {
+            tma_load_2d(a, &p.map_a, &full_bar[s], kb * kStepK, c.begin + c.m0);
+            if constexpr (kForm == kForward) {
+              tma_load_3d(b, &p.map_b, &full_bar[s], kb * kStepK, c.n0, g);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kBN / 64; ++i)
+                tma_load_3d(b + i * kMnBoxBytes, &p.map_b, &full_bar[s], c.n0 + i * 64, kb * kStepK, g);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    uint32_t it = 0, acc = 0;
+    bool ok = true;
+    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
+      const Tile c = tile_at(t, g);
+      if (c.steps == 0) continue;
+      const uint32_t as = acc & 1u;
+      ok = mbar_wait_warp(&tmem_empty_bar[as], ((acc >> 1) & 1u) ^ 1u, abort_ptr);
+      if (!ok) { give_up(kStatusRaggedMma); break; }
+      ++acc;
+      tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + as * kBN;
+      for (int kb = 0; kb < c.steps; ++kb, ++it) {
+        const int s = it % kStages;
+        ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u, abort_ptr);
+        if (!ok) { give_up(kStatusRaggedMma); break; }
+        uint8_t* a = smem + s * kStageBytes;
+        if constexpr (kForm == kGradW) {
+          // the last step of a group whose rows are no multiple of 64: rows of the next group, or of nobody, to zero
+          const int valid = c.count - kb * kStepK;
+          if (valid < kStepK) {
+            for (int box = 0; box < (kTileM + kBN) / 64; ++box)
+              for (int o = valid * 128 + lane * 16; o < kMnBoxBytes; o += 512)
+                *reinterpret_cast<uint4*>(a + box * kMnBoxBytes + o) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t a_addr = smem_u32(a);
+          const uint64_t a_desc = kForm == kGradW ? umma_desc_mn_sw128(a_addr, kMnBoxBytes) : umma_desc_k_sw128(a_addr);
+          const uint64_t b_desc = kForm == kForward ? umma_desc_k_sw128(a_addr + kABytes)
+                                                    : umma_desc_mn_sw128(a_addr + kABytes, kMnBoxBytes);
+          // 16 steps of the contraction per MMA: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
+          constexpr uint32_t kAdvA = kForm == kGradW ? 128 : 2, kAdvB = kForm == kForward ? 2 : 128;
+#pragma unroll
+          for (int k = 0; k < kStepK / 16; ++k)
+            umma_ss<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
+          umma_commit(&empty_bar[s]);
+        }
+        __syncwarp();
+      }
+      if (ok && elect_one()) umma_commit(&tmem_full_bar[as]);
+      __syncwarp();
+    }
+    if (elect_one()) umma_commit(&drain_bar);       // nothing of this warp is still running when TMEM is released
+    __syncwarp();
+    mbar_wait(&drain_bar, 0, abort_ptr);
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint8_t* store = smem + kStages * kStageBytes + (warp - 2) * kStoreTileBytes;
+    constexpr int kChunks = kBN / 64;               // chunks of 32 columns of this warp's half
+    uint32_t acc = 0;
+    for (int t = blockIdx.x, g = 0; t < total; t += gridDim.x) {
+      const Tile c = tile_at(t, g);
+      uint32_t r[kChunks][32];
+      if (c.steps == 0) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[i][j] = 0;
+      } else {
+        const uint32_t as = acc & 1u;
+        if (!mbar_wait_warp(&tmem_full_bar[as], (acc >> 1) & 1u, abort_ptr)) { give_up(kStatusRaggedEpilogue); break; }
+        ++acc;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+          tmem_ld_32x32b_x32(lane_base + as * kBN + half * (kBN / 2) + i * 32, r[i]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tmem_empty_bar[as]);   // the next tile's MMAs need not wait for the stores
+      }
+      const int row0 = c.m0 + quarter * 32;         // inside the group (d W: inside dw[g])
+      const int rows_here = (kForm == kGradW ? p.m_total : c.count) - row0;
+      const bool whole = rows_here >= 32;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = c.n0 + half * (kBN / 2) + i * 32;
+        if (rows_here <= 0 || col >= p.n_total) continue;
+        const int parts = kForm == kGradW && p.out_fp32 ? 2 : 1;      // 32 columns of fp32 are two store tiles
+        for (int part = 0; part < parts; ++part) {
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 v;
+            if (parts == 2) {
+              // (selected by a loop-invariant condition: r stays in registers)
+              v = part == 0 ? make_uint4(r[i][4 * q], r[i][4 * q + 1], r[i][4 * q + 2], r[i][4 * q + 3])
+                            : make_uint4(r[i][16 + 4 * q], r[i][17 + 4 * q], r[i][18 + 4 * q], r[i][19 + 4 * q]);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float lo = __uint_as_float(r[i][8 * q + 2 * j]), hi = __uint_as_float(r[i][8 * q + 2 * j + 1]);
+                w[j] = p.fp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+              }
+              v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            *reinterpret_cast<uint4*>(store + store_piece(lane, q)) = v;
+          }
+          const int x = col + part * 16;
+          if (whole || kForm == kGradW) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kForm == kGradW) tma_store_3d(&p.map_out, store, x, row0, g);
+              else tma_store_2d(&p.map_out, store, x, c.begin + row0);
+              bulk_commit_group();
+            }
+          } else {
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = k * 8 + (lane >> 2), piece = lane & 3;
+              if (row < rows_here && x + piece * 8 < p.n_total)
+                *reinterpret_cast<uint4*>(p.out + static_cast<long long>(c.begin + row0 + row) * p.ld_out +
+                                          2 * (x + piece * 8)) =
+                    *reinterpret_cast<const uint4*>(store + store_piece(row, piece));
+            }
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    if (kForm != kGradW && p.zero_unused)
+      zero_rows_between(s_begin, s_count, p.groups, p.rows, p.out, p.ld_out, 2 * p.n_total,
+                        blockIdx.x * kRaggedEpilogueWarps + warp - 2, gridDim.x * kRaggedEpilogueWarps);
+  }
+
+  // ------------------------------------------------------------------ teardown
+  __syncwarp();
+  if (*abort_ptr) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) __nanosleep(1000);     // copies in flight may still land in shared memory
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, Shape::kTmemCols);
+  }
+}
+
+template <int kForm, int kBN>
+static int launch_gmm(const GmmParams& p, int sms, cudaStream_t stream) {
+  const size_t smem = GmmShape<kBN>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
+  if (cudaFuncSetAttribute(grouped_matmul_kernel<kForm, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return COMFY_MOE_ECUDA;
+  grouped_matmul_kernel<kForm, kBN><<<sms, kRaggedThreads, smem, stream>>>(p);
+  return check_launch();
+}
+
+template <int kForm>
+static int launch_gmm_n(int bn, const GmmParams& p, int sms, cudaStream_t stream) {
+  return bn == 256 ? launch_gmm<kForm, 256>(p, sms, stream)
+                   : (bn == 128 ? launch_gmm<kForm, 128>(p, sms, stream) : launch_gmm<kForm, 64>(p, sms, stream));
+}
+
+// The widest column tile that still gives every SM one: wide tiles read less per product, but a call of few tiles is over
+// when its last SM is.
+static int pick_bn(int64_t row_tiles, int64_t cols, int sms) {
+  for (int bn = 256; bn > 64; bn >>= 1)
+    if (row_tiles * ((cols + bn - 1) / bn) >= sms) return bn;
+  return 64;
+}
+
+struct Ragged2D { const void* ptr; int64_t ld, group_stride; };
+
+static bool rows_ok(const void* p, int64_t ld, int64_t cols, int elem_bytes) {
+  return p && aligned16(p) && ld >= cols && ld * elem_bytes % 16 == 0 && cols * elem_bytes % 16 == 0;
+}
+
+static int check_gmm(int dtype, int rows, int groups, int n, int k, const int32_t* offsets, const int32_t* status) {
+  if (rows < 0 || groups < 0 || n <= 0 || k <= 0 || !status) return COMFY_MOE_EINVAL;
+  if (dtype != COMFY_MOE_BF16 && dtype != COMFY_MOE_FP16) return COMFY_MOE_EUNSUPPORTED;
+  if (groups > kRaggedMaxGroups || n % 8 || k % 8) return COMFY_MOE_EUNSUPPORTED;
+  if (groups > 0 && !offsets) return COMFY_MOE_EINVAL;
+  return COMFY_MOE_OK;
+}
+
+static uint32_t gmm_idesc(int dtype, int form, int bn) {
+  uint32_t d = umma_idesc<false>(kTileM, bn);
+  if (dtype == COMFY_MOE_FP16) d &= ~((7u << 7) | (7u << 10));       // format 0: both operands fp16
+  if (form == kGradW) d |= 1u << 15;                                 // A with its output dimension contiguous
+  if (form != kForward) d |= 1u << 16;                               // B with its output dimension contiguous
+  return d;
+}
+
+}  // namespace comfy_b200
+
+using namespace comfy_b200;
+
+static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, int64_t ld_w, int64_t w_group_stride,
+                         int dtype, int rows, int groups, int n, int k, const int32_t* offsets, const int32_t* counts,
+                         int zero_unused, void* out, int64_t ld_out, int32_t* status, void* stream) {
+  int rc = check_gmm(dtype, rows, groups, n, k, offsets, status);
+  if (rc != COMFY_MOE_OK || rows == 0) return rc;
+  const int in = form == kForward ? k : n, cols = form == kForward ? n : k;
+  if (!rows_ok(a, ld_a, in, 2) || !rows_ok(out, ld_out, cols, 2)) return COMFY_MOE_EINVAL;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (groups == 0) {
+    if (zero_unused && cudaMemset2DAsync(out, ld_out * 2, 0, static_cast<size_t>(cols) * 2, rows, s) != cudaSuccess)
+      return COMFY_MOE_ECUDA;
+    return COMFY_MOE_OK;
+  }
+  if (!rows_ok(w, ld_w, k, 2) || (groups > 1 && (w_group_stride % 8 || w_group_stride < 0))) return COMFY_MOE_EINVAL;
+  const int sms = sm100_count();
+  if (sms < 0) return -sms;
+  GmmParams p;
+  memset(&p, 0, sizeof(p));
+  const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // every group may end in a partial tile, but no more groups than rows have any
+  const int bn = pick_bn((rows + kTileM - 1) / kTileM, cols, sms);
+  if ((rc = ragged_map(&p.map_a, t, 2, a, in, rows, 0, ld_a, 0, 64, kTileM)) != COMFY_MOE_OK) return rc;
+  if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? bn : kStepK)) != COMFY_MOE_OK)
+    return rc;
+  if ((rc = ragged_map(&p.map_out, t, 2, out, cols, rows, 0, ld_out, 0, 32, 32)) != COMFY_MOE_OK) return rc;
+  p.offsets = offsets; p.counts = counts;
+  p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out * 2;
+  p.status = status;
+  p.groups = groups; p.rows = rows;
+  p.n_total = cols; p.k_total = in;
+  // a band's rows of A stay in L2 (126 MB) beside the panels of W that pass: 32 MB of them
+  const int64_t band = (32ll << 20) / (static_cast<int64_t>(kTileM) * in * 2);
+  p.band = static_cast<int>(band < 8 ? 8 : (band > 64 ? 64 : band));
+  p.zero_unused = zero_unused;
+  p.fp16 = dtype == COMFY_MOE_FP16;
+  p.idesc = gmm_idesc(dtype, form, bn);
+  return form == kForward ? launch_gmm_n<kForward>(bn, p, sms, s) : launch_gmm_n<kGradX>(bn, p, sms, s);
+}
+
+extern "C" int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride,
+                                        int dtype, int rows, int n_groups, int out_features, int in_features,
+                                        const int32_t* offsets, const int32_t* counts, int zero_unused, void* out,
+                                        int64_t ld_out, int32_t* status, void* stream) {
+  return rows_by_group(kForward, x, ld_x, w, ld_w, w_group_stride, dtype, rows, n_groups, out_features, in_features, offsets,
+                       counts, zero_unused, out, ld_out, status, stream);
+}
+
+extern "C" int comfy_moe_grouped_matmul_dgrad(const void* dy, int64_t ld_dy, const void* w, int64_t ld_w,
+                                              int64_t w_group_stride, int dtype, int rows, int n_groups, int out_features,
+                                              int in_features, const int32_t* offsets, const int32_t* counts,
+                                              int zero_unused, void* dx, int64_t ld_dx, int32_t* status, void* stream) {
+  return rows_by_group(kGradX, dy, ld_dy, w, ld_w, w_group_stride, dtype, rows, n_groups, out_features, in_features, offsets,
+                       counts, zero_unused, dx, ld_dx, status, stream);
+}
+
+extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int dtype, int rows,
+                                              int n_groups, int out_features, int in_features, const int32_t* offsets,
+                                              const int32_t* counts, int out_dtype, void* dw, int64_t ld_dw,
+                                              int64_t dw_group_stride, int32_t* status, void* stream) {
+  const int n = out_features, k = in_features;
+  int rc = check_gmm(dtype, rows, n_groups, n, k, offsets, status);
+  if (rc != COMFY_MOE_OK || n_groups == 0) return rc;
+  const bool fp32 = out_dtype == COMFY_MOE_FP32;
+  if (!fp32 && out_dtype != dtype) return COMFY_MOE_EUNSUPPORTED;
+  const int out_bytes = fp32 ? 4 : 2;
+  if (!rows_ok(dw, ld_dw, k, out_bytes) || (n_groups > 1 && (dw_group_stride * out_bytes % 16 || dw_group_stride < n * ld_dw)))
+    return COMFY_MOE_EINVAL;
+  if (rows > 0 && (!rows_ok(dy, ld_dy, n, 2) || !rows_ok(x, ld_x, k, 2))) return COMFY_MOE_EINVAL;
+  const int sms = sm100_count();
+  if (sms < 0) return -sms;
+  GmmParams p;
+  memset(&p, 0, sizeof(p));
+  const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int bn = pick_bn(static_cast<int64_t>(n_groups) * ((n + kTileM - 1) / kTileM), k, sms);
+  if (rows > 0) {
+    if ((rc = ragged_map(&p.map_a, t, 2, dy, n, rows, 0, ld_dy, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
+    if ((rc = ragged_map(&p.map_b, t, 2, x, k, rows, 0, ld_x, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
+  }
+  if ((rc = ragged_map(&p.map_out, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : t, out_bytes, dw, k, n, n_groups, ld_dw,
+                       dw_group_stride, fp32 ? 16 : 32, 32)) != COMFY_MOE_OK)
+    return rc;
+  p.offsets = offsets; p.counts = counts;
+  p.out = static_cast<uint8_t*>(dw); p.ld_out = ld_dw * out_bytes;
+  p.status = status;
+  p.groups = n_groups; p.rows = rows;
+  p.m_total = n; p.n_total = k;
+  p.band = 16;
+  p.fp16 = dtype == COMFY_MOE_FP16;
+  p.out_fp32 = fp32;
+  p.idesc = gmm_idesc(dtype, kGradW, bn);
+  return launch_gmm_n<kGradW>(bn, p, sms, static_cast<cudaStream_t>(stream));
+}

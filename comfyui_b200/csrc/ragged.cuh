@@ -1,0 +1,146 @@
+// What the products over ragged groups of rows share: the rows of each group, the order of the tiles, tensor maps.
+#pragma once
+#include <cstring>
+#include <cuda.h>
+
+#include "moe_common.cuh"
+#include "ptx_sm100.cuh"
+
+namespace comfy_b200 {
+
+constexpr int kRaggedMaxGroups = COMFY_MOE_RAGGED_MAX_GROUPS;
+constexpr int kRaggedThreads = 320;            // warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-9 = epilogue
+constexpr int kRaggedEpilogueWarps = 8;        // two per TMEM lane quarter, each takes half of a tile's columns
+constexpr int kStoreRowBytes = 64;             // one warp's store tile: 32 rows of 64 bytes, 64-byte swizzle
+constexpr int kStoreTileBytes = 32 * kStoreRowBytes;
+
+// Device-side status codes of a bounded wait that gave up.
+constexpr int kStatusRaggedProducer = 10;
+constexpr int kStatusRaggedMma = 11;
+constexpr int kStatusRaggedEpilogue = 12;
+
+// The groups' rows, made by one warp of every block from what the caller left on the device:
+//   begin[g] = max(offsets[0 .. g]) clipped to [0, rows],  end = the same up to g + 1,  count[g] = at most counts[g].
+// Offsets that do not rise therefore give empty groups, never rows outside the buffers or rows that two groups share.
+// first_tile[g] = tiles of the groups before g, for tiles of `tile_rows` rows (of one fixed number where tile_rows is 0).
+__device__ __forceinline__ void ragged_ranges(const int32_t* offsets, const int32_t* counts, int groups, int rows,
+                                              int tile_rows, int tiles_per_row_tile, int* begin, int* count,
+                                              int* first_tile) {
+  const int lane = threadIdx.x & 31;
+  int reach = 0, tiles = 0;                    // carried from one chunk of 32 groups to the next
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int lo = 0, hi = 0, most = 0;
+    if (g < groups) {
+      if (offsets) {
+        lo = min(max(offsets[g], 0), rows);
+        hi = min(max(offsets[g + 1], 0), rows);
+      } else {
+        hi = rows;                             // one group: all rows
+      }
+      most = counts ? max(counts[g], 0) : rows;
+    }
+    lo = max(lo, reach);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, max(lo, hi), d);
+      if (lane >= d) lo = max(lo, v);
+    }
+    hi = max(lo, hi);
+    const int n = min(hi - lo, most);
+    const int mine = g < groups ? (tile_rows ? (n + tile_rows - 1) / tile_rows : 1) * tiles_per_row_tile : 0;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (g < groups) {
+      begin[g] = lo;
+      count[g] = n;
+      first_tile[g] = tiles + upto - mine;
+    }
+    reach = __shfl_sync(0xffffffffu, hi, 31);
+    tiles += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) first_tile[groups] = tiles;
+}
+
+// Tile `local` of a group with m_tiles x n_tiles of them: row tiles fastest inside a band of `band` row tiles, so that
+// the tiles in flight share few column panels and the band's rows stay in L2 while the panels pass.
+__device__ __forceinline__ void ragged_tile(int local, int m_tiles, int n_tiles, int band, int& m, int& n) {
+  const int per_band = band * n_tiles;
+  const int b = local / per_band;
+  const int rem = local - b * per_band;
+  const int m0 = b * band;
+  const int in_band = min(band, m_tiles - m0);
+  n = rem / in_band;
+  m = m0 + rem - n * in_band;
+}
+
+// One warp's tile of 32 rows x 64 bytes: lane l has written row l as four 16-byte pieces at `store_piece` places.
+__device__ __forceinline__ uint32_t store_piece(int row, int piece) {
+  return row * kStoreRowBytes + ((piece ^ ((row >> 1) & 3)) << 4);
+}
+
+// Zeros in the rows that belong to no group, dealt to all epilogue warps of the grid.
+__device__ __forceinline__ void zero_rows_between(const int* begin, const int* count, int groups, int rows, uint8_t* out,
+                                                  long long ld_bytes, int row_bytes, int worker, int workers) {
+  const int lane = threadIdx.x & 31;
+  int from = 0;
+  for (int g = 0; g <= groups; ++g) {
+    const int to = g < groups ? begin[g] : rows;
+    for (int r = from + worker; r < to; r += workers)
+      for (int b = lane * 16; b < row_bytes; b += 512)
+        *reinterpret_cast<uint4*>(out + static_cast<long long>(r) * ld_bytes + b) = make_uint4(0, 0, 0, 0);
+    if (g < groups) from = begin[g] + count[g];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = []() -> EncodeTiled {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) != cudaSuccess ||
+        res != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<EncodeTiled>(ptr);
+  }();
+  return fn;
+}
+
+// [groups][rows][cols] with the last dimension contiguous; box of box_rows rows x 128 (swizzle 128) or 64 bytes.  What
+// lies past an extent reads as zero and is not written.  groups = 0: a map of two dimensions.
+inline int ragged_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int64_t cols,
+                      int64_t rows, int64_t groups, int64_t ld, int64_t group_stride, int box_cols, int box_rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return COMFY_MOE_EDEVICE;
+  if (groups <= 1) group_stride = rows * ld;   // the only one: a stride that is never taken
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * elem_bytes, static_cast<cuuint64_t>(group_stride) * elem_bytes};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1u};
+  const cuuint32_t one[3] = {1u, 1u, 1u};
+  const CUtensorMapSwizzle swizzle = box_cols * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const CUresult r = encode(map, type, groups ? 3 : 2, const_cast<void*>(base), dims, strides, box, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? COMFY_MOE_OK : COMFY_MOE_ECUDA;
+}
+
+// Number of SMs of the current device, or a negative value where it is no sm_100.  A thread that has not launched anything
+// yet (autograd's, in a backward pass) has no context that the tensor-map encoder could use: cudaSetDevice makes it one.
+inline int sm100_count() {
+  int dev = 0, major = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return -COMFY_MOE_ECUDA;
+  return major == 10 ? sms : -COMFY_MOE_EDEVICE;
+}
+
+}  // namespace comfy_b200

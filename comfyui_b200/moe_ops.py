@@ -775,3 +775,156 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
                                      float(scale if scale is not None else d ** -0.5), _ptr(out), _ptr(status), _stream())
     N.check("comfy_attn_forward", rc)
     return out
+
+
+# --------------------------------------------------------------------------------------- products over ragged rows
+_HALF_CODES = {torch.bfloat16: N.BF16, torch.float16: N.FP16}
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One C entry point on the current stream of the tensors' device, which need not be the current device."""
+    fn = getattr(N.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream())
+    if rc != N.OK:
+        N.check(name, rc)
+
+
+def _same_device(dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("the sm_100a kernels need CUDA tensors; there is no CPU path")
+        if t.device != dev:
+            raise ValueError(f"all tensors of a call live on one device, got {dev} and {t.device}")
+
+
+def _row_stride(what: str, t: torch.Tensor) -> int:
+    """Elements from one row of t [.., rows, cols] to the next, where the kernels can read and write it as it is."""
+    ld = t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+    unit = 16 // t.element_size()
+    if (t.shape[-1] > 1 and t.stride(-1) != 1) or t.shape[-1] % unit or ld % unit or ld < t.shape[-1] or t.data_ptr() % 16:
+        raise ValueError(f"{what}: rows must be contiguous, of a multiple of {unit} elements, and start on 16 bytes; "
+                         f"got shape {tuple(t.shape)}, strides {t.stride()}")
+    return ld
+
+
+def _group_stride(what: str, t: torch.Tensor) -> int:
+    """Elements from one group of t [G, rows, cols] to the next."""
+    if t.shape[0] <= 1:
+        return 0
+    if t.stride(0) <= 0 or t.stride(0) * t.element_size() % 16:
+        raise ValueError(f"{what}: groups must start on 16 bytes; got strides {t.stride()}")
+    return t.stride(0)
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it over (possibly expanded or transposed), as rows that the kernels can read."""
+    unit = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0)) and \
+        t.data_ptr() % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups: int) -> None:
+    if groups > N.RAGGED_MAX_GROUPS:
+        raise ValueError(f"at most {N.RAGGED_MAX_GROUPS} groups, got {groups}")
+    if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be a contiguous int32 vector of {groups + 1} elements")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (groups,) or not counts.is_contiguous()):
+        raise ValueError(f"counts must be a contiguous int32 vector of {groups} elements")
+
+
+def _check_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
+                   width: int) -> None:
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[width]:
+        raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+    _same_device(x.device, x, w, offsets, counts)
+    if x.dtype not in _HALF_CODES or w.dtype != x.dtype:
+        raise ValueError(f"rows and weights must both be bf16 or both fp16, got {x.dtype} and {w.dtype}")
+    _check_ragged(offsets, counts, w.shape[0])
+
+
+def _result(out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if out.shape != shape or out.dtype != dtype or out.device != dev:
+        raise ValueError(f"out must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
+    return out
+
+
+def _rows_by_group(name: str, a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
+                   out: Optional[torch.Tensor], cols: int) -> torch.Tensor:
+    g, n, k = w.shape
+    res = _result(out, (a.shape[0], cols), a.dtype, a.device)
+    _call(name, a.device, _ptr(a), _row_stride("rows", a), _ptr(w), _row_stride("weights", w), _group_stride("weights", w),
+          _HALF_CODES[a.dtype], a.shape[0], g, n, k, _ptr(offsets), _ptr(counts), int(out is None), _ptr(res),
+          _row_stride("out", res), _ptr(device_status(a.device)))
+    return res
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[r] = x[r] @ w[g].T`` for the rows r of group g = rows offsets[g] .. offsets[g + 1], of which the first counts[g]
+    where ``counts`` is given (the routing plan's expert_offsets and expert_counts).  x [R, K], w [G, N, K], both bf16 or
+    both fp16, y [R, N]; offsets int32 [G + 1], counts int32 [G], on the device and never read by the host.  Rows of no
+    group are zero in a result that this function makes, and stay as they were in ``out``.  Differentiable in x and w
+    (once); a group without rows has the gradient 0."""
+    _check_grouped(x, w, offsets, counts, 2)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        if out is not None:
+            raise ValueError("grouped_matmul: out cannot be given where a gradient is asked for")
+        return _GroupedMatmul.apply(x, w, offsets, counts)
+    return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, out, w.shape[1])
+
+
+def grouped_matmul_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dx[r] = dy[r] @ w[g]``: the gradient of grouped_matmul for x.  dy [R, N] -> [R, K]; rows of no group as there."""
+    _check_grouped(dy, w, offsets, counts, 1)
+    return _rows_by_group("comfy_moe_grouped_matmul_dgrad", dy, w, offsets, counts, out, w.shape[2])
+
+
+def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``dw[g] = sum over the rows r of group g of dy[r].T x[r]``: the gradient of grouped_matmul for w.  dy [R, N],
+    x [R, K] -> [G, N, K] in ``out_dtype`` (x's dtype, or fp32), summed in fp32."""
+    if dy.dim() != 2 or x.dim() != 2 or dy.shape[0] != x.shape[0]:
+        raise ValueError(f"need dy [R, N] and x [R, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
+    groups = offsets.numel() - 1
+    _same_device(x.device, x, dy, offsets, counts)
+    if x.dtype not in _HALF_CODES or dy.dtype != x.dtype:
+        raise ValueError(f"dy and x must both be bf16 or both fp16, got {dy.dtype} and {x.dtype}")
+    _check_ragged(offsets, counts, groups)
+    dt = out_dtype or (x.dtype if out is None else out.dtype)
+    if dt not in (x.dtype, torch.float32):
+        raise ValueError(f"the gradient of the weights comes in {x.dtype} or fp32, not {dt}")
+    res = _result(out, (groups, dy.shape[1], x.shape[1]), dt, x.device)
+    if groups:
+        ld, gs = _row_stride("out", res), _group_stride("out", res)
+        if groups > 1 and gs < res.shape[1] * ld:
+            raise ValueError("out: groups must not overlap")
+        _call("comfy_moe_grouped_matmul_wgrad", x.device, _ptr(dy), _row_stride("dy", dy), _ptr(x), _row_stride("x", x),
+              _HALF_CODES[x.dtype], x.shape[0], groups, dy.shape[1], x.shape[1], _ptr(offsets), _ptr(counts),
+              N.FP32 if dt == torch.float32 else _HALF_CODES[dt], _ptr(res), ld, gs, _ptr(device_status(x.device)))
+    return res
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets, counts):
+        ctx.save_for_backward(x, w, offsets, counts)
+        return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, None, w.shape[1])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets, counts = ctx.saved_tensors
+        dy = _readable(dy)
+        dx = grouped_matmul_dgrad(dy, w, offsets, counts) if ctx.needs_input_grad[0] else None
+        dw = grouped_matmul_wgrad(dy, x, offsets, counts) if ctx.needs_input_grad[1] else None
+        return dx, dw, None, None

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define COMFY_MOE_ABI_VERSION 9
+#define COMFY_MOE_ABI_VERSION 10
 
 /* Return codes. */
 #define COMFY_MOE_OK 0
@@ -357,6 +357,32 @@ typedef struct ComfyMoeLinearGroup {
 } ComfyMoeLinearGroup;
 
 int comfy_moe_grouped_linear(int n_groups, const ComfyMoeLinearGroup* h_groups, int32_t* status, void* stream);
+
+/* ---- products over ragged groups of rows, with any number of experts ----------------------------------------------
+ * Group g holds the rows [begin, begin + n) with begin = offsets[g] and n = offsets[g + 1] - offsets[g], at most counts[g]
+ * where `counts` is given (int32 [n_groups + 1] and [n_groups], on the device, read by the kernel: the routing plan's
+ * expert_offsets and expert_counts, or any others).  What the offsets say is clipped to the buffers, and a group whose
+ * offsets fall below an earlier one begins behind it, so no two groups share a row.
+ *   comfy_moe_grouped_matmul        out[r, :] = x[r, :] . w[g]^T                     x [rows, in], w [n_groups, out, in]
+ *   comfy_moe_grouped_matmul_dgrad  dx[r, :]  = dy[r, :] . w[g]                      its gradient for x
+ *   comfy_moe_grouped_matmul_wgrad  dw[g]     = sum over r in g of dy[r, :]^T x[r, :]  its gradient for w (0 for no rows)
+ * dtype COMFY_MOE_BF16 or COMFY_MOE_FP16 for all operands (wgrad: out_dtype the same or COMFY_MOE_FP32); products are summed
+ * in fp32 and rounded once.  Rows of `out` / `dx` that belong to no group are zeroed if zero_unused is set, else not
+ * touched.  Leading dimensions and group strides in elements; every row and group starts on 16 bytes; in_features and
+ * out_features are multiples of 8; n_groups <= COMFY_MOE_RAGGED_MAX_GROUPS.  status: a status block. */
+#define COMFY_MOE_RAGGED_MAX_GROUPS 1024
+int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride, int dtype,
+                             int rows, int n_groups, int out_features, int in_features, const int32_t* offsets,
+                             const int32_t* counts, int zero_unused, void* out, int64_t ld_out, int32_t* status,
+                             void* stream);
+int comfy_moe_grouped_matmul_dgrad(const void* dy, int64_t ld_dy, const void* w, int64_t ld_w, int64_t w_group_stride,
+                                   int dtype, int rows, int n_groups, int out_features, int in_features,
+                                   const int32_t* offsets, const int32_t* counts, int zero_unused, void* dx, int64_t ld_dx,
+                                   int32_t* status, void* stream);
+int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int dtype, int rows,
+                                   int n_groups, int out_features, int in_features, const int32_t* offsets,
+                                   const int32_t* counts, int out_dtype, void* dw, int64_t ld_dw, int64_t dw_group_stride,
+                                   int32_t* status, void* stream);
 
 /* ---- q / k / v glue of the HiDream attention processor (model.py:97-137) ------------------------------------------
  * One pass per projected tensor x [n_tokens, heads * head_dim] (bf16, row stride ld_x):
