@@ -20,6 +20,7 @@ TOKENS_PER_BLOCK = 32
 MAX_EXPERTS = 8
 STATIC_MAX_TOKENS = 131072
 STATUS_WORDS = 4         # [0] sticky device status, [1] near-ties of the last gate call, [2] e4m3 overflows, [3] reserved
+SCALE_BLOCK = 128            # COMFY_MOE_SCALE_BLOCK: elements along a row that share a scale
 RAGGED_MAX_GROUPS = 1024     # COMFY_MOE_RAGGED_MAX_GROUPS: groups of one call over ragged rows
 LINEAR_MAX_MAPS = 22     # COMFY_MOE_LINEAR_MAX_MAPS: distinct operands of one comfy_moe_grouped_linear call
 MAX_RANKS = 8
@@ -59,6 +60,10 @@ EXPORTS = (
     "comfy_moe_grouped_matmul",
     "comfy_moe_grouped_matmul_dgrad",
     "comfy_moe_grouped_matmul_wgrad",
+    "comfy_moe_block_quantize",
+    "comfy_moe_block_quantize_weight",
+    "comfy_moe_block_workspace",
+    "comfy_moe_block_matmul",
     "comfy_moe_ep_dispatch",
     "comfy_moe_ep_signal",
     "comfy_moe_ep_wait",
@@ -312,6 +317,15 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
         c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
         c_int64, c_int64, c_void_p, c_void_p,
     ]
+    lib.comfy_moe_block_quantize.argtypes = [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                             c_void_p]
+    lib.comfy_moe_block_quantize_weight.argtypes = [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+                                                    c_void_p, c_void_p]
+    lib.comfy_moe_block_workspace.argtypes = [c_int, c_int]
+    lib.comfy_moe_block_matmul.argtypes = [
+        c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
+        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+    ]
     lib.comfy_moe_stochastic_round_e4m3.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p]
     lib.comfy_moe_quantize_weight_e4m3.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]
     lib.comfy_moe_ep_signal.argtypes = [POINTER(PeerPlan), c_int, c_uint32, c_void_p]
@@ -322,6 +336,7 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
     for name in EXPORTS:
         if name not in ("comfy_moe_error_string",):
             getattr(lib, name).restype = c_int
+    lib.comfy_moe_block_workspace.restype = c_int64
     if lib.comfy_moe_abi_version() != ABI_VERSION:
         raise ImportError(f"{path}: ABI version {lib.comfy_moe_abi_version()} != expected {ABI_VERSION}; rebuild it")
     _lib = lib

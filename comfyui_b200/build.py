@@ -25,6 +25,8 @@ SOURCES = [
     "attn_glue.cu",
     "attn_fwd_sm100.cu",
     "grouped_matmul_sm100.cu",
+    "block_quantize.cu",
+    "block_matmul_sm100.cu",
     "weight_ingest.cu",
     "moe_c_api.cu",
 ]

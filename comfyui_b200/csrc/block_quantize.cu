@@ -1,0 +1,177 @@
+// e4m3 with a scale for each block of 128: the activation quantiser (blocks of 1 x 128 along a row) and the weight
+// quantiser (blocks of 128 x 128).  For a block with the largest magnitude m = max(max|x|, 2^-100):
+//   scale = m / 448 (fp32),   q = e4m3(x * 448 / m), round to nearest even.
+// x * 448 / m is formed as ((x * 0.4375) / m) * 1024: the product with 7/16 and the last one are exact (bf16, fp16), so there
+// is one rounding, of the quotient, and it never moves a value onto or over a border between two e4m3 values: a quotient
+// of numbers of at most 11 bits that is no border itself is further from it than half a step of fp32.  (x * (1 / scale)
+// would round ties such as x = 0.75 m either way.)  The floor 2^-100 keeps the scales and their products out of the
+// subnormal range; a block of zeros has zeros.  The maximum is taken on the bit patterns, so a NaN or an infinity wins it
+// and reaches every result the block takes part in: its scale is then NaN or infinite, and so is a product with it.
+// Both are bound by HBM: 3 bytes per element (read 2, written 1).
+#include "moe_common.cuh"
+
+namespace comfy_b200 {
+
+constexpr int kQuantBlock = COMFY_MOE_SCALE_BLOCK;
+constexpr int kLaneElems = 16;                        // 16 e4m3 bytes: one store
+constexpr int kLanesPerBlock = kQuantBlock / kLaneElems;
+
+template <typename T> struct Lane16 { uint4 raw[sizeof(T)]; };      // 16 elements of T as 16-byte words
+
+template <typename T>
+__device__ __forceinline__ void lane_values(const Lane16<T>& in, float (&v)[kLaneElems]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(in.raw);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+constexpr uint32_t kTinyBits = (127u - 100u) << 23;                 // 2^-100
+
+__device__ __forceinline__ uint4 to_e4m3(const float (&v)[kLaneElems], float top) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = __fdiv_rn(v[4 * i + j] * 0.4375f, top) * 1024.0f;
+    w[i] = static_cast<uint32_t>(f2_to_e4m3x2(q[0], q[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(q[2], q[3])) << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 32 rows x one block per CTA: eight lanes per row, so the maximum needs three shuffles, and the 32 scales of a block are
+// one line of the [blocks][rows] scale matrix (what the product's epilogue, one row per lane, reads without gaps).
+template <typename T>
+__global__ void __launch_bounds__(256)
+block_quantize_kernel(const T* __restrict__ x, long long ld, int rows, int cols, uint8_t* __restrict__ q, long long ld_q,
+                      float* __restrict__ scale, long long ld_scale) {
+  const int row = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7;
+  const int col = blockIdx.y * kQuantBlock + l * kLaneElems;
+  const bool live = row < rows && col < cols;         // cols is a multiple of 16: a lane has all of its elements or none
+  Lane16<T> in = {};
+  if (live) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + row * ld + col);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) in.raw[i] = __ldg(src + i);
+  }
+  float v[kLaneElems];
+  lane_values<T>(in, v);
+  uint32_t top = kTinyBits;
+#pragma unroll
+  for (int i = 0; i < kLaneElems; ++i) top = max(top, magnitude_bits(v[i]));
+#pragma unroll
+  for (int d = 1; d < kLanesPerBlock; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float m = __uint_as_float(top);
+  if (live) *reinterpret_cast<uint4*>(q + row * ld_q + col) = to_e4m3(v, m);
+  if (l == 0 && row < rows) scale[blockIdx.y * ld_scale + row] = __fdiv_rn(m, 448.0f);
+}
+
+// One 128 x 128 block per CTA, held in registers between the maximum and the division.
+template <typename T>
+__global__ void __launch_bounds__(256)
+block_quantize_weight_kernel(const T* __restrict__ w, long long ld, long long group_stride, int n, int k,
+                             uint8_t* __restrict__ q, float* __restrict__ scale) {
+  __shared__ uint32_t s_top[8];
+  const int l = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+  const int col = blockIdx.x * kQuantBlock + l * kLaneElems;
+  const T* src = w + blockIdx.z * group_stride;
+  Lane16<T> in[4] = {};
+  uint32_t top = kTinyBits;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = blockIdx.y * kQuantBlock + i * 32 + r0;
+    if (row < n && col < k) {
+      const uint4* p = reinterpret_cast<const uint4*>(src + row * ld + col);
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) in[i].raw[j] = __ldg(p + j);
+    }
+    float v[kLaneElems];
+    lane_values<T>(in[i], v);
+#pragma unroll
+    for (int j = 0; j < kLaneElems; ++j) top = max(top, magnitude_bits(v[j]));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, s_top[i]);
+  const float m = __uint_as_float(top);
+  if (threadIdx.x == 0) scale[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = __fdiv_rn(m, 448.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = blockIdx.y * kQuantBlock + i * 32 + r0;
+    if (row < n && col < k) {
+      float v[kLaneElems];
+      lane_values<T>(in[i], v);
+      *reinterpret_cast<uint4*>(q + (static_cast<long long>(blockIdx.z) * n + row) * k + col) = to_e4m3(v, m);
+    }
+  }
+}
+
+static int elem_bytes(int dtype) {
+  return dtype == COMFY_MOE_BF16 || dtype == COMFY_MOE_FP16 ? 2 : (dtype == COMFY_MOE_FP32 ? 4 : 0);
+}
+
+}  // namespace comfy_b200
+
+using namespace comfy_b200;
+
+extern "C" int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
+                                        float* scale, int64_t ld_scale, void* stream) {
+  const int bytes = elem_bytes(dtype);
+  if (!bytes || cols % 16) return COMFY_MOE_EUNSUPPORTED;
+  if (rows < 0 || cols <= 0) return COMFY_MOE_EINVAL;
+  if (rows == 0) return COMFY_MOE_OK;
+  if (!x || !out || !scale || !aligned16(x) || !aligned16(out) || ld_x < cols || ld_x * bytes % 16 || ld_out < cols ||
+      ld_out % 16 || ld_scale < rows)
+    return COMFY_MOE_EINVAL;
+  const int blocks = (cols + kQuantBlock - 1) / kQuantBlock;
+  if (blocks > 65535) return COMFY_MOE_EUNSUPPORTED;
+  const dim3 grid((rows + 31) / 32, blocks);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* q = static_cast<uint8_t*>(out);
+  if (dtype == COMFY_MOE_BF16)
+    block_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ld_x, rows, cols, q, ld_out, scale, ld_scale);
+  else if (dtype == COMFY_MOE_FP16)
+    block_quantize_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(x), ld_x, rows, cols, q, ld_out, scale, ld_scale);
+  else
+    block_quantize_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x), ld_x, rows, cols, q, ld_out, scale, ld_scale);
+  return check_launch();
+}
+
+extern "C" int comfy_moe_block_quantize_weight(const void* w, int64_t ld_w, int64_t w_group_stride, int dtype, int n_groups,
+                                               int out_features, int in_features, void* out, float* scale, void* stream) {
+  const int bytes = elem_bytes(dtype), n = out_features, k = in_features;
+  if (!bytes || k % 16) return COMFY_MOE_EUNSUPPORTED;
+  if (n_groups < 0 || n <= 0 || k <= 0) return COMFY_MOE_EINVAL;
+  if (n_groups == 0) return COMFY_MOE_OK;
+  if (!w || !out || !scale || !aligned16(w) || !aligned16(out) || ld_w < k || ld_w * bytes % 16 ||
+      (n_groups > 1 && w_group_stride * bytes % 16))
+    return COMFY_MOE_EINVAL;
+  const dim3 grid((k + kQuantBlock - 1) / kQuantBlock, (n + kQuantBlock - 1) / kQuantBlock, n_groups);
+  if (grid.y > 65535 || grid.z > 65535) return COMFY_MOE_EUNSUPPORTED;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* q = static_cast<uint8_t*>(out);
+  if (dtype == COMFY_MOE_BF16)
+    block_quantize_weight_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(w), ld_w, w_group_stride, n, k, q, scale);
+  else if (dtype == COMFY_MOE_FP16)
+    block_quantize_weight_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(w), ld_w, w_group_stride, n, k, q, scale);
+  else
+    block_quantize_weight_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(w), ld_w, w_group_stride, n, k, q, scale);
+  return check_launch();
+}

@@ -928,3 +928,161 @@ class _GroupedMatmul(torch.autograd.Function):
         dx = grouped_matmul_dgrad(dy, w, offsets, counts) if ctx.needs_input_grad[0] else None
         dw = grouped_matmul_wgrad(dy, x, offsets, counts) if ctx.needs_input_grad[1] else None
         return dx, dw, None, None
+
+
+# --------------------------------------------------------------------------------------- e4m3 with block scales
+def _blocks(n: int) -> int:
+    return -(-n // N.SCALE_BLOCK)
+
+
+_QUANT_CODES = {torch.bfloat16: N.BF16, torch.float16: N.FP16, torch.float32: N.FP32}
+
+
+def quantize_blocks_e4m3(x: torch.Tensor):
+    """Rows x [R, K] (bf16, fp16 or fp32, K a multiple of 16) as (xq e4m3 [R, K], scale fp32 [R, ceil(K / 128)]): a block of
+    128 elements of a row with the largest magnitude m = max(max|x|, 2^-100) holds e4m3(x * 448 / m), rounded to nearest
+    even, and the scale m / 448.  ``scale`` is the transposed view of what the product reads."""
+    _same_device(x.device, x)
+    if x.dim() != 2 or x.dtype not in _QUANT_CODES or x.shape[1] == 0 or x.shape[1] % 16:
+        raise ValueError("x must be [R, K] in bf16, fp16 or fp32 with K a multiple of 16")
+    r, k = x.shape
+    q = torch.empty((r, k), dtype=_FP8, device=x.device)
+    scale = torch.empty((_blocks(k), r), dtype=torch.float32, device=x.device)
+    _call("comfy_moe_block_quantize", x.device, _ptr(x), _row_stride("x", x), _QUANT_CODES[x.dtype], r, k, _ptr(q), k,
+          _ptr(scale), r)
+    return q, scale.t()
+
+
+def quantize_weight_blocks_e4m3(w: torch.Tensor):
+    """Weights w [N, K] or [G, N, K] (bf16, fp16 or fp32, K a multiple of 16) as (wq e4m3 like w, scale fp32
+    [.., ceil(N / 128), ceil(K / 128)]) with one scale for each 128 x 128 block, by the rule of quantize_blocks_e4m3."""
+    _same_device(w.device, w)
+    if w.dim() not in (2, 3) or w.dtype not in _QUANT_CODES or w.shape[-1] == 0 or w.shape[-1] % 16 or w.shape[-2] == 0:
+        raise ValueError("w must be [N, K] or [G, N, K] in bf16, fp16 or fp32 with K a multiple of 16")
+    n, k = w.shape[-2:]
+    groups = w.shape[0] if w.dim() == 3 else 1
+    q = torch.empty(w.shape, dtype=_FP8, device=w.device)
+    scale = torch.empty(w.shape[:-2] + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
+    _call("comfy_moe_block_quantize_weight", w.device, _ptr(w), _row_stride("w", w),
+          _group_stride("w", w) if w.dim() == 3 else 0, _QUANT_CODES[w.dtype], groups, n, k, _ptr(q), _ptr(scale))
+    return q, scale
+
+
+def _check_block(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, width: int, dims: int, *others) -> None:
+    if w.dim() != dims or x.dim() != 2 or x.shape[1] != w.shape[width]:
+        raise ValueError(f"need rows and weights that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+    _same_device(x.device, x, w, w_scale, *others)
+    if x.dtype not in _HALF_CODES or w.dtype != _FP8:
+        raise ValueError(f"rows must be bf16 or fp16 and weights e4m3, got {x.dtype} and {w.dtype}")
+    n, k = w.shape[-2:]
+    if n % 8 or k % 16 or x.shape[1] % 16 or n == 0 or k == 0:
+        raise ValueError(f"in_features must be a multiple of 16 and out_features of 8 (of 16 for a gradient), got {k} and {n}")
+    want = tuple(w.shape[:-2]) + (_blocks(n), _blocks(k))
+    if w_scale.dtype != torch.float32 or w_scale.shape != want or not w_scale.is_contiguous():
+        raise ValueError(f"the scales must be a contiguous fp32 tensor of shape {want}")
+
+
+def _block_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: Optional[torch.Tensor],
+                   counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
+                   transpose: bool) -> torch.Tensor:
+    n, k = w.shape[-2:]
+    r, contraction = x.shape
+    res = _result(out, (r, k if transpose else n), x.dtype, x.device)
+    ld_w, ld_x, ld_out = _row_stride("weights", w), _row_stride("rows", x), _row_stride("out", res)
+    work = torch.empty(((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction),), dtype=torch.uint8,
+                       device=x.device)
+    _call("comfy_moe_block_matmul", x.device, _ptr(x), ld_x, _HALF_CODES[x.dtype], _ptr(work), _ptr(w), ld_w,
+          _group_stride("weights", w) if offsets is not None else 0, _ptr(w_scale), int(transpose), r,
+          w.shape[0] if offsets is not None else 1, n, k, _ptr(offsets), _ptr(counts), _ptr(bias), int(out is None),
+          _ptr(res), ld_out, _ptr(device_status(x.device)))
+    return res
+
+
+def _asks_for_gradient(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor],
+                       out: Optional[torch.Tensor]) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    if w.requires_grad or w_scale.requires_grad:
+        raise ValueError("block-scaled weights are frozen: neither they nor their scales have a gradient")
+    if not x.requires_grad and (bias is None or not bias.requires_grad):
+        return False
+    if out is not None:
+        raise ValueError("out cannot be given where a gradient is asked for")
+    if w.shape[-2] % 16:
+        raise ValueError(f"out_features must be a multiple of 16 for a gradient, got {w.shape[-2]}")
+    return True
+
+
+def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ (w * scales).T + bias`` in e4m3: x [.., K] (bf16 or fp16) is quantised by blocks of 128 on the way
+    (quantize_blocks_e4m3), w is e4m3 [N, K] with w_scale [ceil(N / 128), ceil(K / 128)] (quantize_weight_blocks_e4m3),
+    bias [N] in x's dtype; sums in fp32, result [.., N] in x's dtype.  Differentiable (once) in x, whose gradient is the
+    same product with the gradient of the result quantised and the weight transposed, and in bias; w is frozen."""
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    _check_block(rows, w, w_scale, 1, 2, bias)
+    if bias is not None and (bias.dtype != x.dtype or bias.shape != w.shape[:1] or not bias.is_contiguous() or
+                             bias.data_ptr() % 16):
+        raise ValueError("bias must be a contiguous vector over the output features in the rows' dtype")
+    if _asks_for_gradient(x, w, w_scale, bias, out):
+        y = _BlockLinear.apply(rows, w, w_scale, bias)
+    else:
+        flat = out if out is None or out.dim() == 2 else out.view(-1, out.shape[-1])
+        y = _block_product(rows, w, w_scale, None, None, bias, flat, False)
+        if out is not None:
+            return out
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (w.shape[0],))
+
+
+def block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dy @ (w * scales)`` in e4m3: the gradient of block_linear for x.  dy [R, N] -> [R, K]; N a multiple of 16."""
+    _check_block(dy, w, w_scale, 0, 2)
+    return _block_product(dy, w, w_scale, None, None, None, out, True)
+
+
+def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
+                         counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """block_linear by expert: ``y[r] = x[r] @ (w[g] * scales[g]).T`` for the rows r of group g.  x [R, K], w e4m3
+    [G, N, K], w_scale [G, ceil(N / 128), ceil(K / 128)]; offsets, counts, out and rows of no group as for grouped_matmul,
+    the quantised rows and the gradient (x only) as for block_linear."""
+    _check_block(x, w, w_scale, 2, 3, offsets, counts)
+    _check_ragged(offsets, counts, w.shape[0])
+    if _asks_for_gradient(x, w, w_scale, None, out):
+        return _GroupedBlockLinear.apply(x, w, w_scale, offsets, counts)
+    return _block_product(x, w, w_scale, offsets, counts, None, out, False)
+
+
+def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
+                               counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dx[r] = dy[r] @ (w[g] * scales[g])``: the gradient of grouped_block_linear for x.  dy [R, N] -> [R, K]."""
+    _check_block(dy, w, w_scale, 1, 3, offsets, counts)
+    _check_ragged(offsets, counts, w.shape[0])
+    return _block_product(dy, w, w_scale, offsets, counts, None, out, True)
+
+
+class _BlockLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, w_scale, bias):
+        ctx.save_for_backward(w, w_scale)
+        return _block_product(x, w, w_scale, None, None, bias, None, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dy = _readable(dy)
+        dx = block_linear_dgrad(dy, *ctx.saved_tensors) if ctx.needs_input_grad[0] else None
+        db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
+        return dx, None, None, db
+
+
+class _GroupedBlockLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, w_scale, offsets, counts):
+        ctx.save_for_backward(w, w_scale, offsets, counts)
+        return _block_product(x, w, w_scale, offsets, counts, None, None, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return grouped_block_linear_dgrad(_readable(dy), *ctx.saved_tensors), None, None, None, None

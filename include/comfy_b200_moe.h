@@ -384,6 +384,31 @@ int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x,
                                    const int32_t* counts, int out_dtype, void* dw, int64_t ld_dw, int64_t dw_group_stride,
                                    int32_t* status, void* stream);
 
+/* ---- e4m3 with a scale for each block of COMFY_MOE_SCALE_BLOCK ------------------------------------------------------
+ * The finer sibling of the per-tensor scales above.  A block with the largest magnitude m (at least 2^-100) holds
+ * q = e4m3(x * 448 / m), round to nearest even, and the fp32 scale m / 448; a NaN or an infinity in a block makes every
+ * product with it NaN or infinite.
+ *   comfy_moe_block_quantize         rows of activations, one scale for 1 x 128 elements: x [rows, cols] (bf16, fp16 or fp32)
+ *                                    -> out e4m3 [rows, cols], scale [blocks][rows] with leading dimension ld_scale
+ *   comfy_moe_block_quantize_weight  weights, one scale for 128 x 128: w [n_groups, out, in] -> out e4m3 (contiguous),
+ *                                    scale [n_groups, ceil(out / 128), ceil(in / 128)]
+ *   comfy_moe_block_matmul           quantises x (dtype bf16 or fp16) into `workspace` (comfy_moe_block_workspace(rows,
+ *                                    contraction) bytes, 16-byte aligned, no two calls at a time) and multiplies:
+ *                                    out[r, :] = x[r, :] . w[g]^T (+ bias);  transpose_w: out[r, :] = x[r, :] . w[g].
+ * Groups of rows, zero_unused, status: as for comfy_moe_grouped_matmul; offsets NULL with n_groups = 1 means all rows.
+ * Block products are summed in fp32 and folded, times both scales, into fp32 sums; out (and bias, contiguous) have x's
+ * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes. */
+#define COMFY_MOE_SCALE_BLOCK 128
+int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
+                             float* scale, int64_t ld_scale, void* stream);
+int comfy_moe_block_quantize_weight(const void* w, int64_t ld_w, int64_t w_group_stride, int dtype, int n_groups,
+                                    int out_features, int in_features, void* out, float* scale, void* stream);
+int64_t comfy_moe_block_workspace(int rows, int cols);
+int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, void* workspace, const void* w, int64_t ld_w,
+                           int64_t w_group_stride, const float* w_scale, int transpose_w, int rows, int n_groups,
+                           int out_features, int in_features, const int32_t* offsets, const int32_t* counts,
+                           const void* bias, int zero_unused, void* out, int64_t ld_out, int32_t* status, void* stream);
+
 /* ---- q / k / v glue of the HiDream attention processor (model.py:97-137) ------------------------------------------
  * One pass per projected tensor x [n_tokens, heads * head_dim] (bf16, row stride ld_x):
  *   n   = rms_norm(x, weight, eps) over the whole row as torch.nn.functional.rms_norm computes it for bf16 (fp32
