@@ -9,8 +9,18 @@
 //   forward: A = x (K-major), B = W[g] (K-major);   d x: A = dy (K-major), B = W[g] (MN-major);
 //   d W: A = dy, B = x, both MN-major, contraction over the group's rows.
 // A row of a tile depends on its own row of A only, so tiles of the first two may hang over the end of their group: the
-// loads take what follows, the stores leave it out.  In d W the rows behind the group are part of the sum: the MMA warp
-// overwrites them with zeros in shared memory (both operands: what stands there may be NaN) before it multiplies.
+// loads take what follows, the stores leave it out.  In d W the rows behind the group are part of the sum: a warp of its own
+// overwrites them with zeros in shared memory (both operands: what stands there may be NaN) before they are multiplied.
+//
+// kCtas = 2: two CTAs on an SM pair share one tcgen05.mma.cta_group::2 stream.  Their tile is 256 rows x 256 columns; each
+// loads its own 128 rows of A and half of B's columns, so an SM reads a third less per product than with 128 x 256 of its
+// own, and under the power cap the clock rises by as much.  Barriers as in moe_grouped_gemm_sm100.cu: full and
+// tmem_empty live in the leader, both CTAs' loads and epilogue warps signal them; empty and tmem_full exist in both and are
+// committed to by the leader's MMA warp.  In d W a group's last, partial step is loaded against a tail barrier of each
+// CTA; its tail warp zeroes what lies behind the group and announces the step, in the leader on `full`, in the other CTA on
+// the leader's `peer` barrier.  (An arrival of the other CTA at every step, so that one barrier would do, halved the rate:
+// 762 us against 412 with single CTAs at 16384 rows, 8 groups, 2048 x 8192.  Zeros by the MMA warp itself held up every
+// tile of a short group: 111 us against 108 at 2048 rows.)
 #include "ragged.cuh"
 
 namespace comfy_b200 {
@@ -22,9 +32,11 @@ constexpr int kStepK = 64;                     // contraction elements per stage
 constexpr int kABytes = kTileM * 128;
 constexpr int kMnBoxBytes = kStepK * 128;      // one box of an MN-major operand: 64 steps x 64 elements
 
-template <int kBN> struct GmmShape {
-  static constexpr int kStageBytes = kABytes + kBN * 128;
-  static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
+template <int kBN, int kCtas> struct GmmShape {
+  static constexpr int kTileRows = kTileM * kCtas;
+  static constexpr int kCols = kBN / kCtas;                        // columns of B that one CTA loads
+  static constexpr int kStageBytes = kABytes + kCols * 128;
+  static constexpr int kStages = 6;
   static constexpr int kTmemCols = 2 * kBN;    // two accumulators: the epilogue of one tile overlaps the next one's MMAs
   static constexpr int kTables = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
 };
@@ -46,43 +58,52 @@ struct alignas(64) GmmParams {
   uint32_t idesc;
 };
 
-template <int kForm, int kBN>
-__global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
-  using Shape = GmmShape<kBN>;
+template <int kForm, int kBN, int kCtas>
+__global__ void __launch_bounds__(kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, 1)
+grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
+  using Shape = GmmShape<kBN, kCtas>;
   constexpr int kStages = Shape::kStages;
   constexpr int kStageBytes = Shape::kStageBytes;
+  constexpr int kTileRows = Shape::kTileRows;
+  constexpr int kCols = Shape::kCols;
+  constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ __align__(8) uint64_t tmem_full_bar[2], tmem_empty_bar[2], drain_bar;
+  __shared__ __align__(8) uint64_t tail_bar[kStages], peer_bar[kStages];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;      // 0 = leader of the pair
+  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
   int* s_count = s_begin + p.groups;
   int* s_first = s_count + p.groups;
 
   const int n_tiles = (p.n_total + kBN - 1) / kBN;
-  const int m_tiles_w = (p.m_total + kTileM - 1) / kTileM;
+  const int m_tiles_w = (p.m_total + kTileRows - 1) / kTileRows;
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-      for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps); }
+      for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps * kCtas); }
       mbar_init(&drain_bar, 1);
+      for (int s = 0; s < kStages; ++s) { mbar_init(&tail_bar[s], 1); mbar_init(&peer_bar[s], 1); }
       fence_mbar_init();
       abort_flag = 0;
     }
     __syncwarp();
-    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTileM,
+    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTileRows,
                   kForm == kGradW ? m_tiles_w * n_tiles : n_tiles, s_begin, s_count, s_first);
   } else if (warp == 1) {
-    tmem_alloc(&tmem_slot, Shape::kTmemCols);
-    tmem_relinquish();
+    if constexpr (kPair) { tmem_alloc_pair(&tmem_slot, Shape::kTmemCols); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_slot, Shape::kTmemCols); tmem_relinquish(); }
   }
   __syncwarp();
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();     // the peer's barriers must exist before anything signals them
+  else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort_ptr = &abort_flag;
@@ -91,7 +112,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
     if (lane == 0) { atomicCAS(p.status, 0, code); abort_flag = 1; }
   };
 
-  // Tiles t = blockIdx.x, + gridDim.x, ... in the order of the groups; g only ever moves forward.
+  // Tiles t = unit, + units, ... in the order of the groups; g only ever moves forward.
   struct Tile { int m0, n0, begin, count, steps; };
   auto tile_at = [&](int t, int& g) {
     while (t >= s_first[g + 1]) ++g;
@@ -99,8 +120,8 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
     c.begin = s_begin[g];
     c.count = s_count[g];
     int m, n;
-    ragged_tile(t - s_first[g], kForm == kGradW ? m_tiles_w : (c.count + kTileM - 1) / kTileM, n_tiles, p.band, m, n);
-    c.m0 = m * kTileM;
+    ragged_tile(t - s_first[g], kForm == kGradW ? m_tiles_w : (c.count + kTileRows - 1) / kTileRows, n_tiles, p.band, m, n);
+    c.m0 = m * kTileRows;
     c.n0 = n * kBN;
     c.steps = ((kForm == kGradW ? c.count : p.k_total) + kStepK - 1) / kStepK;
     return c;
@@ -110,7 +131,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
     // ------------------------------------------------------------------ TMA producer
     uint32_t it = 0;
     bool ok = true;
-    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
+    for (int t = unit, g = 0; t < total && ok; t += units) {
       const Tile c = tile_at(t, g);
       for (int kb = 0; kb < c.steps; ++kb, ++it) {
         const int s = it % kStages;
@@ -119,22 +140,27 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
         uint8_t* a = smem + s * kStageBytes;
         uint8_t* b = a + kABytes;
         if (elect_one()) {
-          mbar_arrive_expect_tx(&full_bar[s], kStageBytes);
+          // a step is full in the leader, with both CTAs' bytes; a partial step of d W in each CTA by itself
+          const bool tail = kForm == kGradW && c.count - kb * kStepK < kStepK;
+          uint64_t* own = tail ? &tail_bar[s] : &full_bar[s];
+          if (tail || rank == 0) mbar_arrive_expect_tx(own, tail ? kStageBytes : kCtas * kStageBytes);
+          const uint32_t bar = kPair ? mapa_shared(smem_u32(own), tail ? rank : 0) : smem_u32(own);
+          const int m0 = c.m0 + rank * kTileM, n0 = c.n0 + rank * kCols;
           if constexpr (kForm == kGradW) {
 #pragma unroll
             for (int i = 0; i < kTileM / 64; ++i)
-              tma_load_2d(a + i * kMnBoxBytes, &p.map_a, &full_bar[s], c.m0 + i * 64, c.begin + kb * kStepK);
+              load_2d<kPair>(a + i * kMnBoxBytes, &p.map_a, bar, m0 + i * 64, c.begin + kb * kStepK);
 #pragma unroll
-            for (int i = 0; i < kBN / 64; ++i)
-              tma_load_2d(b + i * kMnBoxBytes, &p.map_b, &full_bar[s], c.n0 + i * 64, c.begin + kb * kStepK);
+            for (int i = 0; i < kCols / 64; ++i)
+              load_2d<kPair>(b + i * kMnBoxBytes, &p.map_b, bar, n0 + i * 64, c.begin + kb * kStepK);
           } else {
-            tma_load_2d(a, &p.map_a, &full_bar[s], kb * kStepK, c.begin + c.m0);
+            load_2d<kPair>(a, &p.map_a, bar, kb * kStepK, c.begin + m0);
             if constexpr (kForm == kForward) {
-              tma_load_3d(b, &p.map_b, &full_bar[s], kb * kStepK, c.n0, g);
+              load_3d<kPair>(b, &p.map_b, bar, kb * kStepK, n0, g);
             } else {
 #pragma unroll
-              for (int i = 0; i < kBN / 64; ++i)
-                tma_load_3d(b + i * kMnBoxBytes, &p.map_b, &full_bar[s], c.n0 + i * 64, kb * kStepK, g);
+              for (int i = 0; i < kCols / 64; ++i)
+                load_3d<kPair>(b + i * kMnBoxBytes, &p.map_b, bar, n0 + i * 64, kb * kStepK, g);
             }
           }
         }
@@ -142,10 +168,11 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
+    // ------------------------------------------------------------------ MMA issuer (of the leader)
     uint32_t it = 0, acc = 0;
+    uint32_t peers = 0;                             // bit s: parity of peer_bar[s]
     bool ok = true;
-    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
+    for (int t = unit, g = 0; t < total && ok && rank == 0; t += units) {
       const Tile c = tile_at(t, g);
       if (c.steps == 0) continue;
       const uint32_t as = acc & 1u;
@@ -159,16 +186,11 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
         ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u, abort_ptr);
         if (!ok) { give_up(kStatusRaggedMma); break; }
         uint8_t* a = smem + s * kStageBytes;
-        if constexpr (kForm == kGradW) {
-          // the last step of a group whose rows are no multiple of 64: rows of the next group, or of nobody, to zero
-          const int valid = c.count - kb * kStepK;
-          if (valid < kStepK) {
-            for (int box = 0; box < (kTileM + kBN) / 64; ++box)
-              for (int o = valid * 128 + lane * 16; o < kMnBoxBytes; o += 512)
-                *reinterpret_cast<uint4*>(a + box * kMnBoxBytes + o) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
+        if (kForm == kGradW && kPair && c.count - kb * kStepK < kStepK) {
+          ok = mbar_wait_warp(&peer_bar[s], (peers >> s) & 1u, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedMma); break; }
+          peers ^= 1u << s;
+          asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
         tc_fence_after_sync();
         if (elect_one()) {
@@ -179,18 +201,47 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
           // 16 steps of the contraction per MMA: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
           constexpr uint32_t kAdvA = kForm == kGradW ? 128 : 2, kAdvB = kForm == kForward ? 2 : 128;
 #pragma unroll
-          for (int k = 0; k < kStepK / 16; ++k)
-            umma_ss<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
-          umma_commit(&empty_bar[s]);
+          for (int k = 0; k < kStepK / 16; ++k) {
+            if constexpr (kPair) umma_ss_pair<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
+            else umma_ss<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          commit<kPair>(&empty_bar[s]);
         }
         __syncwarp();
       }
-      if (ok && elect_one()) umma_commit(&tmem_full_bar[as]);
+      if (ok && elect_one()) commit<kPair>(&tmem_full_bar[as]);
       __syncwarp();
     }
-    if (elect_one()) umma_commit(&drain_bar);       // nothing of this warp is still running when TMEM is released
-    __syncwarp();
-    mbar_wait(&drain_bar, 0, abort_ptr);
+    if (rank == 0) {                                // nothing of this warp is still running when TMEM is released
+      if (elect_one()) {
+        if constexpr (kPair) umma_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
+        else umma_commit(&drain_bar);
+      }
+      __syncwarp();
+      mbar_wait(&drain_bar, 0, abort_ptr);
+    }
+  } else if (kForm == kGradW && warp == 2 + kRaggedEpilogueWarps) {
+    // ------------------------------------------------------------------ zeros behind a group
+    uint32_t it = 0, tails = 0;                     // bit s: parity of tail_bar[s]
+    for (int t = unit, g = 0; t < total; t += units) {
+      const Tile c = tile_at(t, g);
+      it += c.steps;
+      const int valid = c.count - (c.steps - 1) * kStepK;
+      if (c.steps == 0 || valid == kStepK) continue;
+      const int s = (it - 1) % kStages;
+      if (!mbar_wait_warp(&tail_bar[s], (tails >> s) & 1u, abort_ptr)) { give_up(kStatusRaggedMma); break; }
+      tails ^= 1u << s;
+      uint8_t* a = smem + s * kStageBytes;
+      for (int box = 0; box < (kTileM + kCols) / 64; ++box)
+        for (int o = valid * 128 + lane * 16; o < kMnBoxBytes; o += 512)
+          *reinterpret_cast<uint4*>(a + box * kMnBoxBytes + o) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(&full_bar[s]);
+        else mbar_arrive_cluster(mapa_shared(smem_u32(&peer_bar[s]), 0));
+      }
+    }
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -198,7 +249,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
     uint8_t* store = smem + kStages * kStageBytes + (warp - 2) * kStoreTileBytes;
     constexpr int kChunks = kBN / 64;               // chunks of 32 columns of this warp's half
     uint32_t acc = 0;
-    for (int t = blockIdx.x, g = 0; t < total; t += gridDim.x) {
+    for (int t = unit, g = 0; t < total; t += units) {
       const Tile c = tile_at(t, g);
       uint32_t r[kChunks][32];
       if (c.steps == 0) {
@@ -217,9 +268,12 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tmem_empty_bar[as]);   // the next tile's MMAs need not wait for the stores
+        if (lane == 0) {                                 // the next tile's MMAs need not wait for the stores
+          if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty_bar[as]), 0));
+          else mbar_arrive(&tmem_empty_bar[as]);
+        }
       }
-      const int row0 = c.m0 + quarter * 32;         // inside the group (d W: inside dw[g])
+      const int row0 = c.m0 + rank * kTileM + quarter * 32;         // inside the group (d W: inside dw[g])
       const int rows_here = (kForm == kGradW ? p.m_total : c.count) - row0;
       const bool whole = rows_here >= 32;
 #pragma unroll
@@ -284,38 +338,35 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) grouped_matmul_kernel(const
     while (clock64() - t0 < 2000000LL) __nanosleep(1000);     // copies in flight may still land in shared memory
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();      // neither CTA leaves while the other may still signal it or use its TMEM
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, Shape::kTmemCols);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, Shape::kTmemCols);
+    else tmem_dealloc(tmem_base, Shape::kTmemCols);
   }
 }
 
-template <int kForm, int kBN>
+template <int kForm, int kBN, int kCtas>
 static int launch_gmm(const GmmParams& p, int sms, cudaStream_t stream) {
-  const size_t smem = GmmShape<kBN>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
-  if (cudaFuncSetAttribute(grouped_matmul_kernel<kForm, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem)) != cudaSuccess)
-    return COMFY_MOE_ECUDA;
-  grouped_matmul_kernel<kForm, kBN><<<sms, kRaggedThreads, smem, stream>>>(p);
-  return check_launch();
+  const size_t smem = GmmShape<kBN, kCtas>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
+  return launch_ragged<kCtas>(grouped_matmul_kernel<kForm, kBN, kCtas>, p,
+                              kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, smem, sms, stream);
 }
 
 template <int kForm>
-static int launch_gmm_n(int bn, const GmmParams& p, int sms, cudaStream_t stream) {
-  return bn == 256 ? launch_gmm<kForm, 256>(p, sms, stream)
-                   : (bn == 128 ? launch_gmm<kForm, 128>(p, sms, stream) : launch_gmm<kForm, 64>(p, sms, stream));
+static int launch_gmm_ctas(int ctas, const GmmParams& p, int sms, cudaStream_t stream) {
+  return ctas == 2 ? launch_gmm<kForm, 256, 2>(p, sms, stream) : launch_gmm<kForm, 128, 1>(p, sms, stream);
 }
 
-// The widest column tile that still gives every SM one: wide tiles read less per product, but a call of few tiles is over
-// when its last SM is.
-static int pick_bn(int64_t row_tiles, int64_t cols, int sms) {
-  for (int bn = 256; bn > 64; bn >>= 1)
-    if (row_tiles * ((cols + bn - 1) / bn) >= sms) return bn;
-  return 64;
+// SM pairs with 256 x 256 tiles where the groups have the rows for them, 128 x 128 tiles of single CTAs below.  Measured (us,
+// pair / single): forward at 512 rows a group 76 / 98, 256: 56 / 58, 64: 42 / 39; dx 119 / 169 (4096 rows), 50 / 44 (64);
+// dw, whose contraction is the group's rows, 100 / 173 (4096 rows), 112 / 120 (256), 92 / 80 (64).  Tiles of 64 columns, and
+// pairs with 128, were never the fastest.
+static int pick_ctas(int64_t rows, int64_t groups, int64_t pair_from) {
+  const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
+  return rows >= pair_from * busy ? 2 : 1;
 }
-
-struct Ragged2D { const void* ptr; int64_t ld, group_stride; };
 
 static bool rows_ok(const void* p, int64_t ld, int64_t cols, int elem_bytes) {
   return p && aligned16(p) && ld >= cols && ld * elem_bytes % 16 == 0 && cols * elem_bytes % 16 == 0;
@@ -329,8 +380,8 @@ static int check_gmm(int dtype, int rows, int groups, int n, int k, const int32_
   return COMFY_MOE_OK;
 }
 
-static uint32_t gmm_idesc(int dtype, int form, int bn) {
-  uint32_t d = umma_idesc<false>(kTileM, bn);
+static uint32_t gmm_idesc(int dtype, int form, int ctas) {
+  uint32_t d = umma_idesc<false>(kTileM * ctas, kTileM * ctas);
   if (dtype == COMFY_MOE_FP16) d &= ~((7u << 7) | (7u << 10));       // format 0: both operands fp16
   if (form == kGradW) d |= 1u << 15;                                 // A with its output dimension contiguous
   if (form != kForward) d |= 1u << 16;                               // B with its output dimension contiguous
@@ -360,10 +411,9 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  // every group may end in a partial tile, but no more groups than rows have any
-  const int bn = pick_bn((rows + kTileM - 1) / kTileM, cols, sms);
+  const int ctas = pick_ctas(rows, groups, 128);
   if ((rc = ragged_map(&p.map_a, t, 2, a, in, rows, 0, ld_a, 0, 64, kTileM)) != COMFY_MOE_OK) return rc;
-  if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? bn : kStepK)) != COMFY_MOE_OK)
+  if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? kTileM : kStepK)) != COMFY_MOE_OK)
     return rc;
   if ((rc = ragged_map(&p.map_out, t, 2, out, cols, rows, 0, ld_out, 0, 32, 32)) != COMFY_MOE_OK) return rc;
   p.offsets = offsets; p.counts = counts;
@@ -372,12 +422,12 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   p.groups = groups; p.rows = rows;
   p.n_total = cols; p.k_total = in;
   // a band's rows of A stay in L2 (126 MB) beside the panels of W that pass: 32 MB of them
-  const int64_t band = (32ll << 20) / (static_cast<int64_t>(kTileM) * in * 2);
+  const int64_t band = (32ll << 20) / (static_cast<int64_t>(kTileM * ctas) * in * 2);
   p.band = static_cast<int>(band < 8 ? 8 : (band > 64 ? 64 : band));
   p.zero_unused = zero_unused;
   p.fp16 = dtype == COMFY_MOE_FP16;
-  p.idesc = gmm_idesc(dtype, form, bn);
-  return form == kForward ? launch_gmm_n<kForward>(bn, p, sms, s) : launch_gmm_n<kGradX>(bn, p, sms, s);
+  p.idesc = gmm_idesc(dtype, form, ctas);
+  return form == kForward ? launch_gmm_ctas<kForward>(ctas, p, sms, s) : launch_gmm_ctas<kGradX>(ctas, p, sms, s);
 }
 
 extern "C" int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride,
@@ -414,7 +464,7 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int bn = pick_bn(static_cast<int64_t>(n_groups) * ((n + kTileM - 1) / kTileM), k, sms);
+  const int ctas = pick_ctas(rows, n_groups, 192);
   if (rows > 0) {
     if ((rc = ragged_map(&p.map_a, t, 2, dy, n, rows, 0, ld_dy, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
     if ((rc = ragged_map(&p.map_b, t, 2, x, k, rows, 0, ld_x, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
@@ -430,6 +480,6 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
   p.band = 16;
   p.fp16 = dtype == COMFY_MOE_FP16;
   p.out_fp32 = fp32;
-  p.idesc = gmm_idesc(dtype, kGradW, bn);
-  return launch_gmm_n<kGradW>(bn, p, sms, static_cast<cudaStream_t>(stream));
+  p.idesc = gmm_idesc(dtype, kGradW, ctas);
+  return launch_gmm_ctas<kGradW>(ctas, p, sms, static_cast<cudaStream_t>(stream));
 }

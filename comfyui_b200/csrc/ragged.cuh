@@ -9,7 +9,8 @@
 namespace comfy_b200 {
 
 constexpr int kRaggedMaxGroups = COMFY_MOE_RAGGED_MAX_GROUPS;
-constexpr int kRaggedThreads = 320;            // warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-9 = epilogue
+constexpr int kRaggedThreads = 320;            // warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-9 = epilogue,
+constexpr int kRaggedTailThreads = 352;        // warp 10 = zeros behind a group (where the rows are the contraction)
 constexpr int kRaggedEpilogueWarps = 8;        // two per TMEM lane quarter, each takes half of a tile's columns
 constexpr int kStoreRowBytes = 64;             // one warp's store tile: 32 rows of 64 bytes, 64-byte swizzle
 constexpr int kStoreTileBytes = 32 * kStoreRowBytes;
@@ -78,6 +79,28 @@ __device__ __forceinline__ void ragged_tile(int local, int m_tiles, int n_tiles,
   m = m0 + rem - n * in_band;
 }
 
+// Loads and commits of one CTA or of an SM pair; `bar` is an address in the shared::cluster window (a CTA's own
+// shared-memory address is one too).
+template <bool kPair>
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
+  else tma_load_2d(dst, map, bar, x, y);
+}
+template <bool kPair>
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (kPair) tma_load_3d_pair(dst, map, bar, x, y, z);
+  else tma_load_3d(dst, map, bar, x, y, z);
+}
+template <bool kPair>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (kPair) {
+    umma_commit_pair(mapa_shared(smem_u32(bar), 0));
+    umma_commit_pair(mapa_shared(smem_u32(bar), 1));
+  } else {
+    umma_commit(bar);
+  }
+}
+
 // One warp's tile of 32 rows x 64 bytes: lane l has written row l as four 16-byte pieces at `store_piece` places.
 __device__ __forceinline__ uint32_t store_piece(int row, int piece) {
   return row * kStoreRowBytes + ((piece ^ ((row >> 1) & 3)) << 4);
@@ -141,6 +164,26 @@ inline int sm100_count() {
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return -COMFY_MOE_ECUDA;
   return major == 10 ? sms : -COMFY_MOE_EDEVICE;
+}
+
+// One persistent CTA (or CTA pair) per SM (pair).
+template <int kCtas, typename Params>
+int launch_ragged(void (*kernel)(Params), const Params& p, int threads, size_t smem, int sms, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+    return COMFY_MOE_ECUDA;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(sms / kCtas * kCtas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kCtas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? check_launch() : COMFY_MOE_ECUDA;
 }
 
 }  // namespace comfy_b200

@@ -68,13 +68,13 @@ def test_sizes(cuda_device, counts, k, n, dtype):
 
 @pytest.mark.parametrize("counts", [[700, 0, 1333, 15], [2500]], ids=["four", "one"])
 def test_many_tiles(cuda_device, counts):
-    check_all(cuda_device, counts, 1536, 2056, torch.bfloat16)
+    check_all(cuda_device, counts, 2048, 2056, torch.bfloat16)
 
 
-@pytest.mark.parametrize("groups,each", [(300, 3), (1024, 1)])
-def test_many_groups(cuda_device, groups, each):
+@pytest.mark.parametrize("groups,each,k,n", [(300, 3, 64, 72), (1024, 1, 64, 72), (160, 90, 264, 264), (40, 300, 520, 776)])
+def test_many_groups(cuda_device, groups, each, k, n):
     counts = [(g * 7 + 3) % (2 * each + 1) for g in range(groups)]
-    check_all(cuda_device, counts, 64, 72, torch.bfloat16)
+    check_all(cuda_device, counts, k, n, torch.bfloat16)
 
 
 def test_rows_of_no_group_are_zero(cuda_device):
