@@ -2,22 +2,47 @@
 //   out[r, n] = sum over blocks b of  xs[r, b] ws[g][n / 128, b]  (sum over k in b of xq[r, k] wq[g][n, k])   (+ bias[n])
 // and the same with the weight transposed (the gradient of x: the contraction runs over n, and the 128 x 128 blocks
 // transpose with the weight).  A stage of shared memory is one block of the contraction: 128 bytes per row.  The scales
-// change with every block, so a block's 128 x 128 products cannot stay in one accumulator: the MMAs of a block write a
-// TMEM buffer of their own (four of them in flight), and the epilogue warps fold it into sums in registers, one FMA per
-// element and block with the product of the two scales.  Every rounding is fp32 until the last one.
+// change with every block, so a block's products cannot stay in one accumulator: the MMAs of a block write a TMEM buffer
+// of 128 x 128 per CTA, one of four, and the epilogue warps fold it into sums in registers, one FMA per element and block
+// with the product of the two scales.  Every rounding is fp32 until the last one.
+// What bounds it is the hand-over between the MMA warp and the epilogue: a wait costs either side 150 cycles even on a
+// complete barrier, a block's MMAs take 256, and a way from one CTA of a pair to the other some hundred.  So two blocks
+// share a stage, a wait, a commit and a hand-over: 8192 rows, 2560 -> 6912 took 194 us with one block at a time and takes
+// 165 (without the quantiser; 1760 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
+// need (what it hands back is tensor memory whose reads are complete), cost a thousand cycles each: 300 us.
 // Group rows, tile order and stores as in grouped_matmul_sm100.cu.
 #include "ragged.cuh"
 
 namespace comfy_b200 {
 
 constexpr int kBlk = COMFY_MOE_SCALE_BLOCK;      // elements per scale = bytes per row of a stage
-constexpr int kFpTile = 128;                     // rows and columns of a tile
+constexpr int kFpTile = 128;                     // rows and columns of a CTA's accumulator, and columns of a tile
 constexpr int kFpOperand = kFpTile * kBlk;       // 16 KB
-constexpr int kFpStageBytes = 2 * kFpOperand;
-constexpr int kFpStages = 6;
-constexpr int kFpAcc = 4;                        // TMEM buffers of 128 columns
-constexpr int kFpTables = kFpStages * kFpStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
+constexpr int kFpUnit = 2;                       // blocks of the contraction per stage, and accumulators per hand-over
+constexpr int kFpAcc = 2;                        // pairs of accumulators
+constexpr int kFpTmemCols = kFpAcc * kFpUnit * kFpTile;
+constexpr int kScaleSteps = 8, kScaleSlots = 2;  // blocks per slot of the ring of scales, slots
+constexpr int kScaleWarps = 2;
+constexpr int kFpFirst = 2 + kScaleWarps;        // the first epilogue warp
+constexpr int kFpThreads = (kFpFirst + kRaggedEpilogueWarps) * 32;
+// Registers: the epilogue's two warpgroups hold 64 sums and two steps' 128 products per thread; the first warpgroup
+// (producer, MMA issuer, scales) hands over what it does not use.
+constexpr int kFpFewRegs = 56, kFpManyRegs = 224, kFpLaunchRegs = 168;
+static_assert(kFpThreads == 384 && 128 * kFpFewRegs + 256 * kFpManyRegs <= kFpThreads * kFpLaunchRegs,
+              "the warpgroups share what the block is launched with");
 static_assert(kBlk == 128, "a stage row is one scale block and one swizzled line");
+
+// kCtas = 1: 128 x 128 tiles.  kCtas = 2: SM pairs, 256 x 128 tiles; each CTA loads its 128 rows and 64 of the columns.
+template <int kCtas> struct FpShape {
+  static constexpr int kTileRows = kFpTile * kCtas;
+  static constexpr int kCols = kFpTile / kCtas;  // columns that a CTA loads
+  static constexpr int kBBytes = kCols * kBlk;   // of one block
+  static constexpr int kStageBytes = kFpUnit * (kFpOperand + kBBytes);
+  static constexpr int kStages = kCtas == 2 ? 4 : 3;
+  static constexpr int kScales = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
+  static constexpr int kTables = kScales + kScaleSlots * kScaleSteps * kFpTile * 4;
+  static_assert(kStages > kFpAcc, "a stage's barriers are never a whole turn ahead of an epilogue warp");
+};
 
 struct alignas(64) BlockParams {
   CUtensorMap map_a, map_b, map_out;
@@ -36,38 +61,45 @@ struct alignas(64) BlockParams {
   uint32_t idesc;
 };
 
-template <bool kTransposed>
-__global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const __grid_constant__ BlockParams p) {
+template <bool kTransposed, int kCtas>
+__global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __grid_constant__ BlockParams p) {
+  using Shape = FpShape<kCtas>;
+  constexpr bool kPair = kCtas == 2;
+  constexpr int kStages = Shape::kStages, kStageBytes = Shape::kStageBytes, kTileRows = Shape::kTileRows;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[kFpStages], empty_bar[kFpStages];
-  __shared__ __align__(8) uint64_t tmem_full_bar[kFpAcc], tmem_empty_bar[kFpAcc], drain_bar;
+  __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
+  __shared__ __align__(8) uint64_t scale_full_bar[kScaleSlots], scale_empty_bar[kScaleSlots], drain_bar;
+  __shared__ int4 tile_ring[kScaleSlots];          // of the slot's tile: first row and column, rows and first row of its group
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;      // 0 = leader of the pair
+  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* s_begin = reinterpret_cast<int*>(smem + kFpTables);
+  int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
   int* s_count = s_begin + p.groups;
   int* s_first = s_count + p.groups;
   const int n_tiles = (p.n_total + kFpTile - 1) / kFpTile;
-  const int steps = (p.k_total + kBlk - 1) / kBlk;
+  const int steps = (p.k_total + kBlk - 1) / kBlk;      // blocks of the contraction
   if (warp == 0) {
     if (lane == 0) {
-      for (int s = 0; s < kFpStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-      for (int s = 0; s < kFpAcc; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps); }
+      for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1 + kRaggedEpilogueWarps * kCtas); mbar_init(&empty_bar[s], 1); }
+      for (int s = 0; s < kScaleSlots; ++s) { mbar_init(&scale_full_bar[s], kScaleWarps); mbar_init(&scale_empty_bar[s], kRaggedEpilogueWarps); }
       mbar_init(&drain_bar, 1);
       fence_mbar_init();
       abort_flag = 0;
     }
     __syncwarp();
-    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kFpTile, n_tiles, s_begin, s_count, s_first);
+    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kTileRows, n_tiles, s_begin, s_count, s_first);
   } else if (warp == 1) {
-    tmem_alloc(&tmem_slot, kFpAcc * kFpTile);
-    tmem_relinquish();
+    if constexpr (kPair) { tmem_alloc_pair(&tmem_slot, kFpTmemCols); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_slot, kFpTmemCols); tmem_relinquish(); }
   }
   __syncwarp();
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();     // the peer's barriers must exist before anything signals them
+  else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort_ptr = &abort_flag;
@@ -82,103 +114,192 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
     c.begin = s_begin[g];
     c.count = s_count[g];
     int m, n;
-    ragged_tile(t - s_first[g], (c.count + kFpTile - 1) / kFpTile, n_tiles, p.band, m, n);
-    c.m0 = m * kFpTile;
+    ragged_tile(t - s_first[g], (c.count + kTileRows - 1) / kTileRows, n_tiles, p.band, m, n);
+    c.m0 = m * kTileRows;
     c.n0 = n * kFpTile;
     return c;
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    uint32_t it = 0;
-    bool ok = true;
-    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
-      const Tile c = tile_at(t, g);
-      for (int kb = 0; kb < steps; ++kb, ++it) {
-        const int s = it % kFpStages;
-        ok = mbar_wait_warp(&empty_bar[s], ((it / kFpStages) & 1u) ^ 1u, abort_ptr);
-        if (!ok) { give_up(kStatusRaggedProducer); break; }
-        uint8_t* a = smem + s * kFpStageBytes;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&full_bar[s], kFpStageBytes);
-          tma_load_2d(a, &p.map_a, &full_bar[s], kb * kBlk, c.begin + c.m0);
-          if constexpr (kTransposed) tma_load_3d(a + kFpOperand, &p.map_b, &full_bar[s], c.n0, kb * kBlk, g);
-          else tma_load_3d(a + kFpOperand, &p.map_b, &full_bar[s], kb * kBlk, c.n0, g);
-        }
-        __syncwarp();
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    uint32_t it = 0;                               // counts stages and, alike, TMEM buffers
-    bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      for (int kb = 0; kb < steps; ++kb, ++it) {
-        const int s = it % kFpStages, as = it % kFpAcc;
-        ok = mbar_wait_warp(&tmem_empty_bar[as], ((it / kFpAcc) & 1u) ^ 1u, abort_ptr) &&
-             mbar_wait_warp(&full_bar[s], (it / kFpStages) & 1u, abort_ptr);
-        if (!ok) { give_up(kStatusRaggedMma); break; }
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t a_addr = smem_u32(smem + s * kFpStageBytes);
-          const uint64_t a_desc = umma_desc_k_sw128(a_addr);
-          const uint64_t b_desc = kTransposed ? umma_desc_mn_sw128(a_addr + kFpOperand, kFpOperand)
-                                              : umma_desc_k_sw128(a_addr + kFpOperand);
-          constexpr uint32_t kAdvB = kTransposed ? (32 * 128) >> 4 : 2;    // 32 steps of the contraction per MMA
+  float* scale_ring = reinterpret_cast<float*>(smem + Shape::kScales);      // [slot][step][row]
+  // Barriers: full[s] is complete when the stage's operands have landed AND every epilogue warp of the tile has read the
+  // accumulators that its MMAs will overwrite (they arrive kFpAcc stages ahead), and empty[s], which the MMAs complete, tells
+  // the producer that the stage is free and the epilogue that its accumulators are full.
+  if (warp < kFpFirst) {
+    regs_down<kFpFewRegs>();
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      int s = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int t = unit, g = 0; t < total && ok; t += units) {
+        const Tile c = tile_at(t, g);
+        for (int kb = 0; kb < steps; kb += kFpUnit) {
+          ok = mbar_wait_warp(&empty_bar[s], phase, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedProducer); break; }
+          uint8_t* a = smem + s * kStageBytes;
+          uint8_t* b = a + kFpUnit * kFpOperand;
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], kCtas * kStageBytes);
+            const uint32_t bar = kPair ? mapa_shared(smem_u32(&full_bar[s]), 0) : smem_u32(&full_bar[s]);
+            const int n0 = c.n0 + rank * Shape::kCols;
 #pragma unroll
-          for (int k = 0; k < kBlk / 32; ++k)
-            umma_ss<true>(tmem_base + as * kFpTile, a_desc + 2 * k, b_desc + k * kAdvB, p.idesc, k != 0 ? 1u : 0u);
-          umma_commit(&empty_bar[s]);
-          umma_commit(&tmem_full_bar[as]);
+            for (int u = 0; u < kFpUnit; ++u) {          // (a block behind the last one reads as zeros)
+              const int k0 = (kb + u) * kBlk;
+              load_2d<kPair>(a + u * kFpOperand, &p.map_a, bar, k0, c.begin + c.m0 + rank * kFpTile);
+              load_3d<kPair>(b + u * Shape::kBBytes, &p.map_b, bar, kTransposed ? n0 : k0, kTransposed ? k0 : n0, g);
+            }
+          }
+          __syncwarp();
+          s = s + 1 == kStages ? 0 : s + 1;
+          phase ^= s == 0;
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer (of the leader)
+      int s = 0, acc = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = unit; t < total && ok && rank == 0; t += units) {
+        for (int kb = 0; kb < steps; kb += kFpUnit) {
+          ok = mbar_wait_warp(&full_bar[s], phase, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedMma); break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            // 32 steps of the contraction per MMA: 32 bytes along a K-major row, 32 rows of an MN-major box
+            constexpr uint32_t kAdvB = kTransposed ? (32 * Shape::kCols) >> 4 : 2;
+            const uint32_t a_addr = smem_u32(smem + s * kStageBytes), b_addr = a_addr + kFpUnit * kFpOperand;
+            const uint64_t a_desc = umma_desc_k_sw128(a_addr);
+            const uint64_t b_desc = kTransposed ? (kPair ? umma_desc_mn_sw64(b_addr) : umma_desc_mn_sw128(b_addr, kFpOperand))
+                                                : umma_desc_k_sw128(b_addr);
+#pragma unroll
+            for (int u = 0; u < kFpUnit; ++u) {
+              const uint32_t d_tmem = tmem_base + (acc * kFpUnit + u) * kFpTile;
+#pragma unroll
+              for (int k = 0; k < kBlk / 32; ++k) {
+                const uint64_t ad = a_desc + u * (kFpOperand >> 4) + 2 * k, bd = b_desc + u * (Shape::kBBytes >> 4) + k * kAdvB;
+                if constexpr (kPair) umma_ss_pair<true>(d_tmem, ad, bd, p.idesc, k != 0 ? 1u : 0u);
+                else umma_ss<true>(d_tmem, ad, bd, p.idesc, k != 0 ? 1u : 0u);
+              }
+            }
+            commit<kPair>(&empty_bar[s]);
+          }
+          __syncwarp();
+          acc = (acc + 1) % kFpAcc;
+          s = s + 1 == kStages ? 0 : s + 1;
+          phase ^= s == 0;
+        }
+      }
+      if (rank == 0) {                                // nothing of this warp is still running when TMEM is released
+        if (elect_one()) {
+          if constexpr (kPair) umma_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
+          else umma_commit(&drain_bar);
         }
         __syncwarp();
+        mbar_wait(&drain_bar, 0, abort_ptr);
+      }
+    } else {
+      // ------------------------------------------------------------------ scales: xs[row, block] ws[column block, block]
+      // One slot holds eight steps of a tile's 128 rows of this CTA.  These warps run ahead of the epilogue, across tiles, so
+      // that nobody waits for a load from global memory, which takes longer than a step.
+      uint32_t slot = 0;
+      bool ok = true;
+      for (int t = unit, g = 0; t < total && ok; t += units) {
+        const Tile c = tile_at(t, g);
+        const float* ws = p.ws + g * p.ws_group + static_cast<long long>(c.n0 / kBlk) * p.ws_n;
+        for (int kb = 0; kb < steps; kb += kScaleSteps, ++slot) {
+          const int q = slot % kScaleSlots;
+          ok = mbar_wait_warp(&scale_empty_bar[q], ((slot / kScaleSlots) & 1u) ^ 1u, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedEpilogue); break; }
+          float w[kScaleSteps];
+#pragma unroll
+          for (int i = 0; i < kScaleSteps; ++i) w[i] = kb + i < steps ? __ldg(ws + static_cast<long long>(kb + i) * p.ws_k) : 0.f;
+#pragma unroll
+          for (int v = 0; v < kFpTile / (32 * kScaleWarps); ++v) {
+            const int row = ((warp - 2) + v * kScaleWarps) * 32 + lane;
+            const int in_group = c.m0 + rank * kFpTile + row;
+            const float* xs = p.xs + c.begin + in_group;
+            float x[kScaleSteps];
+#pragma unroll
+            for (int i = 0; i < kScaleSteps; ++i)
+              x[i] = kb + i < steps && in_group < c.count ? __ldg(xs + (kb + i) * p.ld_xs) : 0.f;
+#pragma unroll
+            for (int i = 0; i < kScaleSteps; ++i) scale_ring[(q * kScaleSteps + i) * kFpTile + row] = x[i] * w[i];
+          }
+          if (warp == 2 && lane == 0) tile_ring[q] = make_int4(c.m0, c.n0, c.count, c.begin);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_full_bar[q]);
+        }
       }
     }
-    if (elect_one()) umma_commit(&drain_bar);       // nothing of this warp is still running when TMEM is released
-    __syncwarp();
-    mbar_wait(&drain_bar, 0, abort_ptr);
   } else {
-    // ------------------------------------------------------------------ epilogue: one row and 64 columns per thread
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    regs_up<kFpManyRegs>();
+    // ------------------------------------------------------------------ epilogue: one row and half of the columns per thread
+    const int quarter = warp & 3, half = (warp - kFpFirst) >> 2;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
-    uint8_t* store = smem + kFpStages * kFpStageBytes + (warp - 2) * kStoreTileBytes;
-    uint32_t it = 0;
+    uint8_t* store = smem + kStages * kStageBytes + (warp - kFpFirst) * kStoreTileBytes;
+    const uint32_t full_addr = kPair ? mapa_shared(smem_u32(full_bar), 0) : smem_u32(full_bar);
+    int back = 0;                                // stage of the step whose accumulator is handed back next
+    auto hand_back = [&]() {
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster_relaxed(full_addr + 8 * back);
+        else mbar_arrive(&full_bar[back]);
+      }
+      back = back + 1 == kStages ? 0 : back + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kFpAcc; ++i) hand_back();     // the first steps find their accumulators free
+    int stage = 0, acc = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x, g = 0; t < total && ok; t += gridDim.x) {
-      const Tile c = tile_at(t, g);
-      const int row0 = c.m0 + quarter * 32;
-      const int rows_here = c.count - row0;
-      const bool live = lane < rows_here;
-      const float* xs = p.xs + c.begin + row0 + lane;
-      const float* ws = p.ws + g * p.ws_group + static_cast<long long>(c.n0 / kBlk) * p.ws_n;
+    for (int t = unit; t < total && ok; t += units) {
       float sum[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0.f;
-      float xs_next = live ? __ldg(xs) : 0.f, ws_next = __ldg(ws);
-      for (int kb = 0; kb < steps; ++kb, ++it) {
-        const float scale = xs_next * ws_next;
-        if (kb + 1 < steps) {
-          xs_next = live ? __ldg(xs + (kb + 1) * p.ld_xs) : 0.f;
-          ws_next = __ldg(ws + static_cast<long long>(kb + 1) * p.ws_k);
+      int4 tile = make_int4(0, 0, 0, 0);
+      const float* scales = nullptr;
+      for (int kb = 0; kb < steps; kb += kFpUnit) {
+        if (kb % kScaleSteps == 0) {
+          ok = mbar_wait_warp(&scale_full_bar[slot], slot_phase, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedEpilogue); break; }
+          scales = scale_ring + slot * kScaleSteps * kFpTile + quarter * 32 + lane;
+          tile = tile_ring[slot];
         }
-        const uint32_t as = it % kFpAcc;
-        ok = mbar_wait_warp(&tmem_full_bar[as], (it / kFpAcc) & 1u, abort_ptr);
+        float scale[kFpUnit];
+#pragma unroll
+        for (int u = 0; u < kFpUnit; ++u) scale[u] = scales[u * kFpTile];
+        scales += kFpUnit * kFpTile;
+        ok = mbar_wait_warp(&empty_bar[stage], phase, abort_ptr);
         if (!ok) { give_up(kStatusRaggedEpilogue); break; }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        phase ^= stage == 0;
         tc_fence_after_sync();
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(lane_base + as * kFpTile, r[0]);
-        tmem_ld_32x32b_x32(lane_base + as * kFpTile + 32, r[1]);
+        uint32_t r[kFpUnit][2][32];
+#pragma unroll
+        for (int u = 0; u < kFpUnit; ++u) {
+          tmem_ld_32x32b_x32(lane_base + (acc * kFpUnit + u) * kFpTile, r[u][0]);
+          tmem_ld_32x32b_x32(lane_base + (acc * kFpUnit + u) * kFpTile + 32, r[u][1]);
+        }
+        acc = (acc + 1) % kFpAcc;
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tmem_empty_bar[as]);
+        hand_back();
 #pragma unroll
-        for (int i = 0; i < 64; ++i) sum[i] = fmaf(__uint_as_float(r[i >> 5][i & 31]), scale, sum[i]);
+        for (int u = 0; u < kFpUnit; ++u)
+#pragma unroll
+          for (int j = 0; j < 64; ++j) sum[j] = fmaf(__uint_as_float(r[u][j >> 5][j & 31]), scale[u], sum[j]);
+        if (kb % kScaleSteps == kScaleSteps - kFpUnit || kb + kFpUnit >= steps) {
+          if (lane == 0) mbar_arrive(&scale_empty_bar[slot]);      // (the warp has met since it read its scales)
+          slot = slot + 1 == kScaleSlots ? 0 : slot + 1;
+          slot_phase ^= slot == 0;
+        }
       }
-      if (!ok || rows_here <= 0) continue;
+      if (!ok) break;
+      const int row0 = tile.x + rank * kFpTile + quarter * 32, rows_here = tile.z - row0;
+      if (rows_here <= 0) continue;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int col = c.n0 + half * 64 + i * 32;
+        const int col = tile.y + half * 64 + i * 32;
         if (col >= p.n_total) continue;
         if (lane == 0) bulk_wait_read_all();
         __syncwarp();
@@ -188,12 +309,12 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = sum[i * 32 + q * 8 + j];
           if (p.bias != nullptr && col + q * 8 < p.n_total) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.bias) + (col + q * 8) / 8);
-            const uint32_t b[4] = {raw.x, raw.y, raw.z, raw.w};
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.bias) + col / 8 + q);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&b[j]))
-                                      : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
+              const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                                      : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
               v[2 * j] += f.x;
               v[2 * j + 1] += f.y;
             }
@@ -208,7 +329,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&p.map_out, store, col, c.begin + row0);
+            tma_store_2d(&p.map_out, store, col, tile.w + row0);
             bulk_commit_group();
           }
         } else {
@@ -217,7 +338,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
           for (int k = 0; k < 4; ++k) {
             const int row = k * 8 + (lane >> 2), piece = lane & 3;
             if (row < rows_here && col + piece * 8 < p.n_total)
-              *reinterpret_cast<uint4*>(p.out + static_cast<long long>(c.begin + row0 + row) * p.ld_out + 2 * (col + piece * 8)) =
+              *reinterpret_cast<uint4*>(p.out + static_cast<long long>(tile.w + row0 + row) * p.ld_out + 2 * (col + piece * 8)) =
                   *reinterpret_cast<const uint4*>(store + store_piece(row, piece));
           }
         }
@@ -226,7 +347,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
     if (lane == 0) bulk_wait_all();
     if (p.zero_unused)
       zero_rows_between(s_begin, s_count, p.groups, p.rows, p.out, p.ld_out, 2 * p.n_total,
-                        blockIdx.x * kRaggedEpilogueWarps + warp - 2, gridDim.x * kRaggedEpilogueWarps);
+                        blockIdx.x * kRaggedEpilogueWarps + warp - kFpFirst, gridDim.x * kRaggedEpilogueWarps);
   }
 
   // ------------------------------------------------------------------ teardown
@@ -236,21 +357,25 @@ __global__ void __launch_bounds__(kRaggedThreads, 1) block_matmul_kernel(const _
     while (clock64() - t0 < 2000000LL) __nanosleep(1000);     // copies in flight may still land in shared memory
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();      // neither CTA leaves while the other may still signal it or use its TMEM
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, kFpAcc * kFpTile);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, kFpTmemCols);
+    else tmem_dealloc(tmem_base, kFpTmemCols);
   }
 }
 
-template <bool kTransposed>
+template <bool kTransposed, int kCtas>
 static int launch_block(const BlockParams& p, int sms, cudaStream_t stream) {
-  const size_t smem = kFpTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
-  if (cudaFuncSetAttribute(block_matmul_kernel<kTransposed>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem)) != cudaSuccess)
-    return COMFY_MOE_ECUDA;
-  block_matmul_kernel<kTransposed><<<sms, kRaggedThreads, smem, stream>>>(p);
-  return check_launch();
+  // the warpgroups' register shares have to be there at launch, or the larger ones would wait for good
+  static const int regs = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, block_matmul_kernel<kTransposed, kCtas>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs < kFpLaunchRegs) return COMFY_MOE_EUNSUPPORTED;
+  const size_t smem = FpShape<kCtas>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
+  return launch_ragged<kCtas>(block_matmul_kernel<kTransposed, kCtas>, p, kFpThreads, smem, sms, stream);
 }
 
 static int64_t scale_offset(int64_t rows, int64_t cols) { return (rows * cols + 255) / 256 * 256; }
@@ -287,6 +412,7 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   }
   if (!w || !w_scale || !aligned16(w) || ld_w < k || ld_w % 16 || (n_groups > 1 && (w_group_stride <= 0 || w_group_stride % 16)))
     return COMFY_MOE_EINVAL;
+  const int ctas = rows >= 128 * (n_groups < rows ? n_groups : rows) ? 2 : 1;     // pairs where groups have the rows for them
   const int sms = sm100_count();
   if (sms < 0) return -sms;
   uint8_t* q = static_cast<uint8_t*>(workspace);
@@ -297,7 +423,8 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if ((rc = ragged_map(&p.map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, in, rows, 0, in, 0, kBlk, kFpTile)) != COMFY_MOE_OK ||
-      (rc = ragged_map(&p.map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, n, n_groups, ld_w, w_group_stride, kBlk, kFpTile)) != COMFY_MOE_OK ||
+      (rc = ragged_map(&p.map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, n, n_groups, ld_w, w_group_stride,
+                       transpose_w ? kFpTile / ctas : kBlk, transpose_w ? kBlk : kFpTile / ctas)) != COMFY_MOE_OK ||
       (rc = ragged_map(&p.map_out, t, 2, out, cols, rows, 0, ld_out, 0, 32, 32)) != COMFY_MOE_OK)
     return rc;
   const int nb = (n + kBlk - 1) / kBlk, kb = (k + kBlk - 1) / kBlk;
@@ -310,10 +437,11 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out * 2;
   p.status = status;
   p.groups = n_groups; p.rows = rows; p.n_total = cols; p.k_total = in;
-  const int64_t band = (32ll << 20) / (static_cast<int64_t>(kFpTile) * in);   // 32 MB of rows stay in L2
-  p.band = static_cast<int>(band < 8 ? 8 : (band > 64 ? 64 : band));
   p.zero_unused = zero_unused;
   p.fp16 = dtype == COMFY_MOE_FP16;
-  p.idesc = umma_idesc<true>(kFpTile, kFpTile) | (transpose_w ? 1u << 16 : 0u);
-  return transpose_w ? launch_block<true>(p, sms, s) : launch_block<false>(p, sms, s);
+  const int64_t band = (32ll << 20) / (static_cast<int64_t>(kFpTile * ctas) * in);   // 32 MB of rows stay in L2
+  p.band = static_cast<int>(band < 8 ? 8 : (band > 64 ? 64 : band));
+  p.idesc = umma_idesc<true>(kFpTile * ctas, kFpTile) | (transpose_w ? 1u << 16 : 0u);
+  if (ctas == 2) return transpose_w ? launch_block<true, 2>(p, sms, s) : launch_block<false, 2>(p, sms, s);
+  return transpose_w ? launch_block<true, 1>(p, sms, s) : launch_block<false, 1>(p, sms, s);
 }

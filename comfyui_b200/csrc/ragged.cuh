@@ -93,12 +93,8 @@ __device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint3
 }
 template <bool kPair>
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  if constexpr (kPair) {
-    umma_commit_pair(mapa_shared(smem_u32(bar), 0));
-    umma_commit_pair(mapa_shared(smem_u32(bar), 1));
-  } else {
-    umma_commit(bar);
-  }
+  if constexpr (kPair) umma_commit_both(bar);
+  else umma_commit(bar);
 }
 
 // One warp's tile of 32 rows x 64 bytes: lane l has written row l as four 16-byte pieces at `store_piece` places.

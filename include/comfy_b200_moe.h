@@ -370,7 +370,7 @@ int comfy_moe_grouped_linear(int n_groups, const ComfyMoeLinearGroup* h_groups, 
  * in fp32 and rounded once.  Rows of `out` / `dx` that belong to no group are zeroed if zero_unused is set, else not
  * touched.  Leading dimensions and group strides in elements; every row and group starts on 16 bytes; in_features and
  * out_features are multiples of 8; n_groups <= COMFY_MOE_RAGGED_MAX_GROUPS.  status: a status block. */
-#define COMFY_MOE_RAGGED_MAX_GROUPS 1024
+#define COMFY_MOE_RAGGED_MAX_GROUPS 768
 int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride, int dtype,
                              int rows, int n_groups, int out_features, int in_features, const int32_t* offsets,
                              const int32_t* counts, int zero_unused, void* out, int64_t ld_out, int32_t* status,

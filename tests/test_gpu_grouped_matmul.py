@@ -71,7 +71,7 @@ def test_many_tiles(cuda_device, counts):
     check_all(cuda_device, counts, 2048, 2056, torch.bfloat16)
 
 
-@pytest.mark.parametrize("groups,each,k,n", [(300, 3, 64, 72), (1024, 1, 64, 72), (160, 90, 264, 264), (40, 300, 520, 776)])
+@pytest.mark.parametrize("groups,each,k,n", [(300, 3, 64, 72), (768, 1, 64, 72), (160, 90, 264, 264), (40, 300, 520, 776)])
 def test_many_groups(cuda_device, groups, each, k, n):
     counts = [(g * 7 + 3) % (2 * each + 1) for g in range(groups)]
     check_all(cuda_device, counts, k, n, torch.bfloat16)
