@@ -27,10 +27,11 @@ SOURCES = [
     "grouped_matmul_sm100.cu",
     "block_quantize.cu",
     "block_matmul_sm100.cu",
+    "few_rows.cu",
     "weight_ingest.cu",
     "moe_c_api.cu",
 ]
-HEADERS = ["moe_common.cuh", "moe_gate.cuh", "ptx_sm100.cuh", "ragged.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
+HEADERS = ["moe_common.cuh", "moe_gate.cuh", "ptx_sm100.cuh", "ragged.cuh", "few_rows.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
 
 
 def _nvcc() -> str:

@@ -11,6 +11,7 @@
 // 165 (without the quantiser; 1760 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
 // need (what it hands back is tensor memory whose reads are complete), cost a thousand cycles each: 300 us.
 // Group rows, tile order and stores as in grouped_matmul_sm100.cu.
+#include "few_rows.cuh"
 #include "ragged.cuh"
 
 namespace comfy_b200 {
@@ -401,7 +402,8 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   if (n_groups > kRaggedMaxGroups || k % 16 || in % 16 || cols % 8) return COMFY_MOE_EUNSUPPORTED;
   if (n_groups != 1 && !offsets) return COMFY_MOE_EINVAL;
   if (rows == 0) return COMFY_MOE_OK;
-  if (!x || !workspace || !out || !aligned16(x) || !aligned16(workspace) || !aligned16(out) || ld_x < in || ld_x % 8 ||
+  const bool few = !transpose_w && rows <= kFewRowsBlock && k <= kFewBlockMaxK;
+  if (!x || (!workspace && !few) || !out || !aligned16(x) || !aligned16(workspace) || !aligned16(out) || ld_x < in || ld_x % 8 ||
       ld_out < cols || ld_out % 8 || (bias && !aligned16(bias)))
     return COMFY_MOE_EINVAL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -415,6 +417,18 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   const int ctas = rows >= 128 * (n_groups < rows ? n_groups : rows) ? 2 : 1;     // pairs where groups have the rows for them
   const int sms = sm100_count();
   if (sms < 0) return -sms;
+  const int nb = (n + kBlk - 1) / kBlk, kb = (k + kBlk - 1) / kBlk;
+  if (few) {
+    FewParams f;
+    memset(&f, 0, sizeof(f));
+    f.x = static_cast<const uint8_t*>(x); f.w = static_cast<const uint8_t*>(w); f.out = static_cast<uint8_t*>(out);
+    f.offsets = offsets; f.counts = counts;
+    f.ws = w_scale; f.ws_group = static_cast<long long>(nb) * kb;
+    f.bias = bias;
+    f.ld_x = ld_x * 2; f.ld_w = ld_w; f.w_group = w_group_stride; f.ld_out = ld_out * 2;
+    f.groups = n_groups; f.rows = rows; f.n = n; f.k = k; f.zero_unused = zero_unused;
+    return launch_few_rows_block(f, dtype == COMFY_MOE_FP16, s);
+  }
   uint8_t* q = static_cast<uint8_t*>(workspace);
   float* xs = reinterpret_cast<float*>(q + scale_offset(rows, in));
   int rc = comfy_moe_block_quantize(x, ld_x, dtype, rows, in, q, in, xs, rows, stream);
@@ -427,7 +441,6 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
                        transpose_w ? kFpTile / ctas : kBlk, transpose_w ? kBlk : kFpTile / ctas)) != COMFY_MOE_OK ||
       (rc = ragged_map(&p.map_out, t, 2, out, cols, rows, 0, ld_out, 0, 32, 32)) != COMFY_MOE_OK)
     return rc;
-  const int nb = (n + kBlk - 1) / kBlk, kb = (k + kBlk - 1) / kBlk;
   p.offsets = offsets; p.counts = counts;
   p.xs = xs; p.ld_xs = rows;
   p.ws = w_scale; p.ws_group = static_cast<long long>(nb) * kb;

@@ -1,0 +1,268 @@
+// Products of a few rows with weights that are read once: the single-token form of the grouped products and of the
+// block-scaled ones.  At up to 16 rows the weights are all there is to move (2 flops per byte and row), so the work is cut
+// for HBM: a block takes 16 output columns of one group over the whole contraction, its eight warps the chunks of it in
+// turns, and every lane keeps several 16-byte loads of weights in flight, ten rows' worth of lines per warp.  The
+// arithmetic is one mma.sync tile: 16 output columns x 8 rows, A = weights, B = rows, both operands in the registers that
+// the loads filled: the tile's steps of the contraction may come in any order as long as both sides agree, so a lane's 16
+// contiguous bytes serve two MMAs without a shuffle or shared memory.  (tcgen05 would need both operands in shared memory
+// and 128 rows of one of them.)  The warps' partial sums are joined in a fixed order: the result is the same every time.
+#include <algorithm>
+
+#include "few_rows.cuh"
+#include "ragged.cuh"
+
+namespace comfy_b200 {
+
+constexpr int kFewWarps = 8;
+constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kFewCols = 16;                   // output columns per block
+
+// The rows of one group, by the rule of ragged_ranges; the same in every lane of a warp.
+__device__ __forceinline__ void few_range(const FewParams& p, int g, int& begin, int& count) {
+  const int lane = threadIdx.x & 31;
+  if (!p.offsets) {
+    begin = 0;
+    count = p.rows;
+  } else {
+    int reach = 0;
+    for (int i = lane; i <= g; i += 32) reach = max(reach, min(max(p.offsets[i], 0), p.rows));
+    begin = __reduce_max_sync(0xffffffffu, reach);
+    count = max(begin, min(max(p.offsets[g + 1], 0), p.rows)) - begin;
+  }
+  if (p.counts) count = min(count, max(p.counts[g], 0));
+}
+
+__device__ __forceinline__ uint4 load_once(const void* p) {     // streamed: read by this block only
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint2 load_row(const void* p) {      // (volatile: behind the loads of weights that precede it)
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16x8x32_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Joins the warps' 16 x 8 kTiles sums (in the order of the warps) and writes rows [row0, row0 + live) of the result.
+template <typename T, int kTiles>
+__device__ __forceinline__ void few_store(const FewParams& p, float (&part)[kFewWarps][kFewCols][8 * kTiles + 1],
+                                          const float (&c)[kTiles][4], int row0, int live, int n0) {
+  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) {
+    part[warp][g][j * 8 + 2 * t] = c[j][0];
+    part[warp][g][j * 8 + 2 * t + 1] = c[j][1];
+    part[warp][g + 8][j * 8 + 2 * t] = c[j][2];
+    part[warp][g + 8][j * 8 + 2 * t + 1] = c[j][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kFewCols * 8 * kTiles; i += kFewThreads) {
+    const int col = i % kFewCols, row = i / kFewCols;
+    if (row >= live || n0 + col >= p.n) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) sum += part[w][col][row];
+    if (p.bias) sum += to_float(static_cast<const T*>(p.bias)[n0 + col]);
+    reinterpret_cast<T*>(p.out + static_cast<long long>(row0 + row) * p.ld_out)[n0 + col] = from_float<T>(sum);
+  }
+}
+
+// Block (0, groups): the rows of no group.
+__device__ __forceinline__ void few_zero(const FewParams& p, int* tables) {
+  if (blockIdx.x != 0) return;
+  int *begin = tables, *count = tables + p.groups, *first = tables + 2 * p.groups;
+  if (threadIdx.x < 32) ragged_ranges(p.offsets, p.counts, p.groups, p.rows, 1, 1, begin, count, first);
+  __syncthreads();
+  zero_rows_between(begin, count, p.groups, p.rows, p.out, p.ld_out, 2 * p.n, threadIdx.x >> 5, kFewWarps);
+}
+
+template <typename T, int kTiles>
+__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p) {
+  extern __shared__ int tables[];
+  __shared__ float part[kFewWarps][kFewCols][8 * kTiles + 1];
+  const int grp = blockIdx.y;
+  if (grp == p.groups) { few_zero(p, tables); return; }
+  int begin, count;
+  few_range(p, grp, begin, count);
+  if (count == 0) return;
+  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  const int n0 = blockIdx.x * kFewCols;
+  const uint8_t* w0 = p.w + grp * p.w_group + static_cast<long long>(n0 + g) * p.ld_w;
+  const bool col0 = n0 + g < p.n, col1 = n0 + g + 8 < p.n;
+  constexpr int kChunk = 32;                   // elements of the contraction per warp and turn: 64 bytes of a row
+  constexpr int kFlight = 5;                   // turns whose loads are in flight together
+  const int chunks = (p.k + kChunk - 1) / kChunk;
+  float c[kTiles][4] = {};
+  for (int i0 = warp; i0 < chunks; i0 += kFewWarps * kFlight) {
+    uint4 w[kFlight][2], x[kFlight][kTiles];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int k0 = (i0 + i * kFewWarps) * kChunk + t * 8;            // K is a multiple of 8: a lane has all 8 or none
+      const bool in = k0 < p.k;
+      w[i][0] = in && col0 ? load_once(w0 + 2 * k0) : make_uint4(0, 0, 0, 0);
+      w[i][1] = in && col1 ? load_once(w0 + 8 * p.ld_w + 2 * k0) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        const int row = j * 8 + g;
+        x[i][j] = in && row < count ? __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(begin + row) * p.ld_x + 2 * k0))
+                                    : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i)
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        mma_16x8x16<T>(c[j], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, x[i][j].x, x[i][j].y);
+        mma_16x8x16<T>(c[j], w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, x[i][j].z, x[i][j].w);
+      }
+  }
+  few_store<T, kTiles>(p, part, c, begin, count, n0);
+}
+
+// Block-scaled: the block's weights are on their way while its warps quantise the rows (by the rule of block_quantize.cu),
+// each the blocks that it multiplies; a block's 16 x 8 products are folded, scaled, into the warp's sums.
+constexpr int kFewBlk = COMFY_MOE_SCALE_BLOCK;
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewParams p) {
+  extern __shared__ __align__(16) uint8_t xq[];            // [blocks of the contraction][8 rows][128]
+  __shared__ float part[kFewWarps][kFewCols][9];
+  const int grp = blockIdx.y;
+  if (grp == p.groups) { few_zero(p, reinterpret_cast<int*>(xq)); return; }
+  int begin, count;
+  few_range(p, grp, begin, count);
+  if (count == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * kFewCols;
+  const uint8_t* w0 = p.w + grp * p.w_group + static_cast<long long>(n0 + g) * p.ld_w;
+  const bool col0 = n0 + g < p.n, col1 = n0 + g + 8 < p.n;
+  const int blocks = (p.k + kFewBlk - 1) / kFewBlk;
+  const float* ws = p.ws + grp * p.ws_group + static_cast<long long>(n0 / kFewBlk) * blocks;
+  constexpr int kFlight = 3;                   // blocks whose weights are in flight together
+  float sum[1][4] = {};
+  for (int b0 = warp; b0 < blocks; b0 += kFewWarps * kFlight) {
+    uint4 w[kFlight][2][2];
+    float scale[kFlight];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int b = b0 + i * kFewWarps;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k0 = b * kFewBlk + s * 64 + t * 16;                    // K is a multiple of 16
+        const bool in = b < blocks && k0 < p.k;
+        w[i][s][0] = in && col0 ? load_once(w0 + k0) : make_uint4(0, 0, 0, 0);
+        w[i][s][1] = in && col1 ? load_once(w0 + 8 * p.ld_w + k0) : make_uint4(0, 0, 0, 0);
+      }
+      scale[i] = b < blocks ? __ldg(ws + b) : 0.f;
+    }
+    float xs[kFlight][2] = {};                 // scales of rows 2 t and 2 t + 1, this lane's columns of the product
+    for (int row = 0; row < count; ++row) {
+      const uint8_t* src = p.x + static_cast<long long>(begin + row) * p.ld_x;
+      uint2 raw[kFlight];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const int k0 = (b0 + i * kFewWarps) * kFewBlk + lane * 4;
+        raw[i] = k0 < p.k ? load_row(src + 2 * k0) : make_uint2(0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const T* e = reinterpret_cast<const T*>(&raw[i]);
+        float v[4];
+        uint32_t top = (127u - 100u) << 23;                              // 2^-100
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          v[q] = to_float(e[q]);
+          top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const float m = __uint_as_float(top);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __fdiv_rn(v[q] * 0.4375f, m) * 1024.0f;
+        if (b0 + i * kFewWarps < blocks)
+          reinterpret_cast<uint32_t*>(xq + ((b0 + i * kFewWarps) * 8 + row) * kFewBlk)[lane] =
+              static_cast<uint32_t>(f2_to_e4m3x2(v[0], v[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(v[2], v[3])) << 16);
+        const float s = __fdiv_rn(m, 448.0f);
+        if (row == 2 * t) xs[i][0] = s;
+        if (row == 2 * t + 1) xs[i][1] = s;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int b = b0 + i * kFewWarps;
+      float c[4] = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint4 x = b < blocks && g < count
+                            ? *reinterpret_cast<const uint4*>(xq + (b * 8 + g) * kFewBlk + s * 64 + t * 16)
+                            : make_uint4(0, 0, 0, 0);
+        mma_16x8x32_e4m3(c, w[i][s][0].x, w[i][s][1].x, w[i][s][0].y, w[i][s][1].y, x.x, x.y);
+        mma_16x8x32_e4m3(c, w[i][s][0].z, w[i][s][1].z, w[i][s][0].w, w[i][s][1].w, x.z, x.w);
+      }
+      // (a row or a block that is not there has zeros and the scale 0)
+      sum[0][0] = fmaf(c[0], xs[i][0] * scale[i], sum[0][0]);
+      sum[0][1] = fmaf(c[1], xs[i][1] * scale[i], sum[0][1]);
+      sum[0][2] = fmaf(c[2], xs[i][0] * scale[i], sum[0][2]);
+      sum[0][3] = fmaf(c[3], xs[i][1] * scale[i], sum[0][3]);
+    }
+  }
+  few_store<T, 1>(p, part, sum, begin, count, n0);
+}
+
+template <typename Kernel>
+static int launch_few(Kernel kernel, const FewParams& p, size_t smem, cudaStream_t stream) {
+  const dim3 grid((p.n + kFewCols - 1) / kFewCols, p.groups + (p.zero_unused && p.offsets ? 1 : 0));
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+    return COMFY_MOE_ECUDA;
+  kernel<<<grid, kFewThreads, smem, stream>>>(p);
+  return check_launch();
+}
+
+static size_t few_tables(const FewParams& p) {
+  return p.zero_unused && p.offsets ? (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) : 0;
+}
+
+int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
+  if (p.rows <= 8)
+    return fp16 ? launch_few(few_rows_kernel<__half, 1>, p, few_tables(p), stream)
+                : launch_few(few_rows_kernel<__nv_bfloat16, 1>, p, few_tables(p), stream);
+  return fp16 ? launch_few(few_rows_kernel<__half, 2>, p, few_tables(p), stream)
+              : launch_few(few_rows_kernel<__nv_bfloat16, 2>, p, few_tables(p), stream);
+}
+
+int launch_few_rows_block(const FewParams& p, bool fp16, cudaStream_t stream) {
+  const size_t smem = std::max(static_cast<size_t>((p.k + kFewBlk - 1) / kFewBlk) * 8 * kFewBlk, few_tables(p));
+  return fp16 ? launch_few(few_rows_block_kernel<__half>, p, smem, stream)
+              : launch_few(few_rows_block_kernel<__nv_bfloat16>, p, smem, stream);
+}
+
+}  // namespace comfy_b200

@@ -21,6 +21,7 @@
 // the leader's `peer` barrier.  (An arrival of the other CTA at every step, so that one barrier would do, halved the rate:
 // 762 us against 412 with single CTAs at 16384 rows, 8 groups, 2048 x 8192.  Zeros by the MMA warp itself held up every
 // tile of a short group: 111 us against 108 at 2048 rows.)
+#include "few_rows.cuh"
 #include "ragged.cuh"
 
 namespace comfy_b200 {
@@ -408,6 +409,15 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   if (!rows_ok(w, ld_w, k, 2) || (groups > 1 && (w_group_stride % 8 || w_group_stride < 0))) return COMFY_MOE_EINVAL;
   const int sms = sm100_count();
   if (sms < 0) return -sms;
+  if (form == kForward && rows <= kFewRows) {
+    FewParams f;
+    memset(&f, 0, sizeof(f));
+    f.x = static_cast<const uint8_t*>(a); f.w = static_cast<const uint8_t*>(w); f.out = static_cast<uint8_t*>(out);
+    f.offsets = offsets; f.counts = counts;
+    f.ld_x = ld_a * 2; f.ld_w = ld_w * 2; f.w_group = w_group_stride * 2; f.ld_out = ld_out * 2;
+    f.groups = groups; f.rows = rows; f.n = n; f.k = k; f.zero_unused = zero_unused;
+    return launch_few_rows(f, dtype == COMFY_MOE_FP16, s);
+  }
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

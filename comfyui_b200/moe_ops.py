@@ -778,48 +778,66 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 
 
 # --------------------------------------------------------------------------------------- products over ragged rows
+# These calls last from a few microseconds on, so the way to the C entry points is kept short: plain integers instead of
+# ctypes objects, one pass of checks, no context manager where the tensors are on the current device.
 _HALF_CODES = {torch.bfloat16: N.BF16, torch.float16: N.FP16}
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)       # the same without a Stream object
+
+
+def _call(name: str, index: int, *args) -> None:
     """One C entry point on the current stream of the tensors' device, which need not be the current device."""
     fn = getattr(N.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, _stream())
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream())
-    if rc != N.OK:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
         N.check(name, rc)
 
 
-def _same_device(dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("the sm_100a kernels need CUDA tensors; there is no CPU path")
-        if t.device != dev:
-            raise ValueError(f"all tensors of a call live on one device, got {dev} and {t.device}")
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
-def _row_stride(what: str, t: torch.Tensor) -> int:
-    """Elements from one row of t [.., rows, cols] to the next, where the kernels can read and write it as it is."""
-    ld = t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
-    unit = 16 // t.element_size()
-    if (t.shape[-1] > 1 and t.stride(-1) != 1) or t.shape[-1] % unit or ld % unit or ld < t.shape[-1] or t.data_ptr() % 16:
+def _place(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the one device that all tensors of a call live on."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if index >= 0 and t.is_cuda:
+                raise ValueError(f"all tensors of a call live on one device, got {first.device} and {t.device}")
+            index = -1
+    if index < 0 or not first.is_cuda:
+        raise ValueError("the sm_100a kernels need CUDA tensors; there is no CPU path")
+    return index
+
+
+def _row_stride(what: str, t: torch.Tensor, unit: int) -> int:
+    """Elements from one row of t [.., rows, cols] to the next, where the kernels can read and write it as it is: `unit`
+    elements are 16 bytes."""
+    cols = t.size(-1)
+    ld = cols if t.size(-2) <= 1 else t.stride(-2)
+    if cols % unit or ld % unit or ld < cols or t.data_ptr() % 16 or (t.stride(-1) != 1 and cols > 1):
         raise ValueError(f"{what}: rows must be contiguous, of a multiple of {unit} elements, and start on 16 bytes; "
                          f"got shape {tuple(t.shape)}, strides {t.stride()}")
     return ld
 
 
-def _group_stride(what: str, t: torch.Tensor) -> int:
+def _group_stride(what: str, t: torch.Tensor, unit: int) -> int:
     """Elements from one group of t [G, rows, cols] to the next."""
-    if t.shape[0] <= 1:
+    if t.size(0) <= 1:
         return 0
-    if t.stride(0) <= 0 or t.stride(0) * t.element_size() % 16:
+    step = t.stride(0)
+    if step <= 0 or step % unit:
         raise ValueError(f"{what}: groups must start on 16 bytes; got strides {t.stride()}")
-    return t.stride(0)
+    return step
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -833,37 +851,41 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
 def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups: int) -> None:
     if groups > N.RAGGED_MAX_GROUPS:
         raise ValueError(f"at most {N.RAGGED_MAX_GROUPS} groups, got {groups}")
-    if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_contiguous():
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.size(0) != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be a contiguous int32 vector of {groups + 1} elements")
     if counts is not None and (counts.dtype != torch.int32 or counts.shape != (groups,) or not counts.is_contiguous()):
         raise ValueError(f"counts must be a contiguous int32 vector of {groups} elements")
 
 
-def _check_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
-                   width: int) -> None:
-    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[width]:
-        raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _same_device(x.device, x, w, offsets, counts)
-    if x.dtype not in _HALF_CODES or w.dtype != x.dtype:
-        raise ValueError(f"rows and weights must both be bf16 or both fp16, got {x.dtype} and {w.dtype}")
-    _check_ragged(offsets, counts, w.shape[0])
-
-
-def _result(out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+def _result(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if out.shape != shape or out.dtype != dtype or out.device != dev:
-        raise ValueError(f"out must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
+        return like.new_empty((rows, cols))
+    if out.shape != (rows, cols) or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"out must be a {like.dtype} tensor of shape {(rows, cols)} on {like.device}")
     return out
 
 
+def _once(what: str) -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once: its gradient has no gradient")
+
+
 def _rows_by_group(name: str, a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
-                   out: Optional[torch.Tensor], cols: int) -> torch.Tensor:
+                   out: Optional[torch.Tensor], width: int) -> torch.Tensor:
+    """grouped_matmul (width 2) or its gradient for the rows (width 1)."""
+    if a.dim() != 2 or w.dim() != 3 or a.size(1) != w.size(width):
+        raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(a.shape)} and {tuple(w.shape)}")
+    index = _place(a, w, offsets, counts)
+    code = _HALF_CODES.get(a.dtype)
+    if code is None or w.dtype != a.dtype:
+        raise ValueError(f"rows and weights must both be bf16 or both fp16, got {a.dtype} and {w.dtype}")
     g, n, k = w.shape
-    res = _result(out, (a.shape[0], cols), a.dtype, a.device)
-    _call(name, a.device, _ptr(a), _row_stride("rows", a), _ptr(w), _row_stride("weights", w), _group_stride("weights", w),
-          _HALF_CODES[a.dtype], a.shape[0], g, n, k, _ptr(offsets), _ptr(counts), int(out is None), _ptr(res),
-          _row_stride("out", res), _ptr(device_status(a.device)))
+    _check_ragged(offsets, counts, g)
+    r = a.size(0)
+    res = _result(out, a, r, n if width == 2 else k)
+    _call(name, index, a.data_ptr(), _row_stride("rows", a, 8), w.data_ptr(), _row_stride("weights", w, 8),
+          _group_stride("weights", w, 8), code, r, g, n, k, offsets.data_ptr(), _address(counts), out is None,
+          res.data_ptr(), _row_stride("out", res, 8), device_status(a.device).data_ptr())
     return res
 
 
@@ -871,46 +893,49 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``y[r] = x[r] @ w[g].T`` for the rows r of group g = rows offsets[g] .. offsets[g + 1], of which the first counts[g]
     where ``counts`` is given (the routing plan's expert_offsets and expert_counts).  x [R, K], w [G, N, K], both bf16 or
-    both fp16, y [R, N]; offsets int32 [G + 1], counts int32 [G], on the device and never read by the host.  Rows of no
-    group are zero in a result that this function makes, and stay as they were in ``out``.  Differentiable in x and w
-    (once); a group without rows has the gradient 0."""
-    _check_grouped(x, w, offsets, counts, 2)
+    both fp16, K and N multiples of 8, y [R, N]; offsets int32 [G + 1], counts int32 [G], on the device and never read by
+    the host.  Rows of no group are zero in a result that this function makes, and stay as they were in ``out``.
+    Differentiable in x and w (once); a group without rows has the gradient 0."""
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         if out is not None:
             raise ValueError("grouped_matmul: out cannot be given where a gradient is asked for")
         return _GroupedMatmul.apply(x, w, offsets, counts)
-    return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, out, w.shape[1])
+    return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, out, 2)
 
 
 def grouped_matmul_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dx[r] = dy[r] @ w[g]``: the gradient of grouped_matmul for x.  dy [R, N] -> [R, K]; rows of no group as there."""
-    _check_grouped(dy, w, offsets, counts, 1)
-    return _rows_by_group("comfy_moe_grouped_matmul_dgrad", dy, w, offsets, counts, out, w.shape[2])
+    return _rows_by_group("comfy_moe_grouped_matmul_dgrad", dy, w, offsets, counts, out, 1)
 
 
 def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
                          out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``dw[g] = sum over the rows r of group g of dy[r].T x[r]``: the gradient of grouped_matmul for w.  dy [R, N],
     x [R, K] -> [G, N, K] in ``out_dtype`` (x's dtype, or fp32), summed in fp32."""
-    if dy.dim() != 2 or x.dim() != 2 or dy.shape[0] != x.shape[0]:
+    if dy.dim() != 2 or x.dim() != 2 or dy.size(0) != x.size(0):
         raise ValueError(f"need dy [R, N] and x [R, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
-    groups = offsets.numel() - 1
-    _same_device(x.device, x, dy, offsets, counts)
-    if x.dtype not in _HALF_CODES or dy.dtype != x.dtype:
+    g, (r, n), k = offsets.numel() - 1, dy.shape, x.size(1)
+    index = _place(x, dy, offsets, counts, out)
+    code = _HALF_CODES.get(x.dtype)
+    if code is None or dy.dtype != x.dtype:
         raise ValueError(f"dy and x must both be bf16 or both fp16, got {dy.dtype} and {x.dtype}")
-    _check_ragged(offsets, counts, groups)
+    _check_ragged(offsets, counts, g)
     dt = out_dtype or (x.dtype if out is None else out.dtype)
     if dt not in (x.dtype, torch.float32):
         raise ValueError(f"the gradient of the weights comes in {x.dtype} or fp32, not {dt}")
-    res = _result(out, (groups, dy.shape[1], x.shape[1]), dt, x.device)
-    if groups:
-        ld, gs = _row_stride("out", res), _group_stride("out", res)
-        if groups > 1 and gs < res.shape[1] * ld:
-            raise ValueError("out: groups must not overlap")
-        _call("comfy_moe_grouped_matmul_wgrad", x.device, _ptr(dy), _row_stride("dy", dy), _ptr(x), _row_stride("x", x),
-              _HALF_CODES[x.dtype], x.shape[0], groups, dy.shape[1], x.shape[1], _ptr(offsets), _ptr(counts),
-              N.FP32 if dt == torch.float32 else _HALF_CODES[dt], _ptr(res), ld, gs, _ptr(device_status(x.device)))
+    res = x.new_empty((g, n, k), dtype=dt) if out is None else out
+    if res.shape != (g, n, k) or res.dtype != dt:
+        raise ValueError(f"out must be a {dt} tensor of shape {(g, n, k)}")
+    if g == 0:
+        return res
+    unit = 16 // res.element_size()
+    ld, step = _row_stride("out", res, unit), _group_stride("out", res, unit)
+    if g > 1 and step < n * ld:
+        raise ValueError("out: groups must not overlap")
+    _call("comfy_moe_grouped_matmul_wgrad", index, dy.data_ptr(), _row_stride("dy", dy, 8), x.data_ptr(),
+          _row_stride("x", x, 8), code, r, g, n, k, offsets.data_ptr(), _address(counts),
+          N.FP32 if dt == torch.float32 else code, res.data_ptr(), ld, step, device_status(x.device).data_ptr())
     return res
 
 
@@ -918,11 +943,11 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, counts):
         ctx.save_for_backward(x, w, offsets, counts)
-        return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, None, w.shape[1])
+        return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, None, 2)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("grouped_matmul")
         x, w, offsets, counts = ctx.saved_tensors
         dy = _readable(dy)
         dx = grouped_matmul_dgrad(dy, w, offsets, counts) if ctx.needs_input_grad[0] else None
@@ -942,59 +967,70 @@ def quantize_blocks_e4m3(x: torch.Tensor):
     """Rows x [R, K] (bf16, fp16 or fp32, K a multiple of 16) as (xq e4m3 [R, K], scale fp32 [R, ceil(K / 128)]): a block of
     128 elements of a row with the largest magnitude m = max(max|x|, 2^-100) holds e4m3(x * 448 / m), rounded to nearest
     even, and the scale m / 448.  ``scale`` is the transposed view of what the product reads."""
-    _same_device(x.device, x)
+    index = _place(x)
     if x.dim() != 2 or x.dtype not in _QUANT_CODES or x.shape[1] == 0 or x.shape[1] % 16:
         raise ValueError("x must be [R, K] in bf16, fp16 or fp32 with K a multiple of 16")
     r, k = x.shape
     q = torch.empty((r, k), dtype=_FP8, device=x.device)
     scale = torch.empty((_blocks(k), r), dtype=torch.float32, device=x.device)
-    _call("comfy_moe_block_quantize", x.device, _ptr(x), _row_stride("x", x), _QUANT_CODES[x.dtype], r, k, _ptr(q), k,
-          _ptr(scale), r)
+    _call("comfy_moe_block_quantize", index, x.data_ptr(), _row_stride("x", x, 16 // x.element_size()),
+          _QUANT_CODES[x.dtype], r, k, q.data_ptr(), k, scale.data_ptr(), r)
     return q, scale.t()
 
 
 def quantize_weight_blocks_e4m3(w: torch.Tensor):
     """Weights w [N, K] or [G, N, K] (bf16, fp16 or fp32, K a multiple of 16) as (wq e4m3 like w, scale fp32
     [.., ceil(N / 128), ceil(K / 128)]) with one scale for each 128 x 128 block, by the rule of quantize_blocks_e4m3."""
-    _same_device(w.device, w)
+    index = _place(w)
     if w.dim() not in (2, 3) or w.dtype not in _QUANT_CODES or w.shape[-1] == 0 or w.shape[-1] % 16 or w.shape[-2] == 0:
         raise ValueError("w must be [N, K] or [G, N, K] in bf16, fp16 or fp32 with K a multiple of 16")
     n, k = w.shape[-2:]
     groups = w.shape[0] if w.dim() == 3 else 1
+    unit = 16 // w.element_size()
     q = torch.empty(w.shape, dtype=_FP8, device=w.device)
     scale = torch.empty(w.shape[:-2] + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
-    _call("comfy_moe_block_quantize_weight", w.device, _ptr(w), _row_stride("w", w),
-          _group_stride("w", w) if w.dim() == 3 else 0, _QUANT_CODES[w.dtype], groups, n, k, _ptr(q), _ptr(scale))
+    _call("comfy_moe_block_quantize_weight", index, w.data_ptr(), _row_stride("w", w, unit),
+          _group_stride("w", w, unit) if w.dim() == 3 else 0, _QUANT_CODES[w.dtype], groups, n, k, q.data_ptr(),
+          scale.data_ptr())
     return q, scale
-
-
-def _check_block(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, width: int, dims: int, *others) -> None:
-    if w.dim() != dims or x.dim() != 2 or x.shape[1] != w.shape[width]:
-        raise ValueError(f"need rows and weights that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _same_device(x.device, x, w, w_scale, *others)
-    if x.dtype not in _HALF_CODES or w.dtype != _FP8:
-        raise ValueError(f"rows must be bf16 or fp16 and weights e4m3, got {x.dtype} and {w.dtype}")
-    n, k = w.shape[-2:]
-    if n % 8 or k % 16 or x.shape[1] % 16 or n == 0 or k == 0:
-        raise ValueError(f"in_features must be a multiple of 16 and out_features of 8 (of 16 for a gradient), got {k} and {n}")
-    want = tuple(w.shape[:-2]) + (_blocks(n), _blocks(k))
-    if w_scale.dtype != torch.float32 or w_scale.shape != want or not w_scale.is_contiguous():
-        raise ValueError(f"the scales must be a contiguous fp32 tensor of shape {want}")
 
 
 def _block_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: Optional[torch.Tensor],
                    counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
                    transpose: bool) -> torch.Tensor:
-    n, k = w.shape[-2:]
+    """The four block-scaled products: dense (offsets None) or by expert, of the rows or of their gradient (transpose)."""
+    dims = 2 if offsets is None else 3
+    if w.dim() != dims or x.dim() != 2 or x.size(1) != w.size(-2 if transpose else -1):
+        raise ValueError(f"need rows and weights that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+    index = _place(x, w, w_scale, offsets, counts, bias)
+    code = _HALF_CODES.get(x.dtype)
+    if code is None or w.dtype != _FP8:
+        raise ValueError(f"rows must be bf16 or fp16 and weights e4m3, got {x.dtype} and {w.dtype}")
     r, contraction = x.shape
-    res = _result(out, (r, k if transpose else n), x.dtype, x.device)
-    ld_w, ld_x, ld_out = _row_stride("weights", w), _row_stride("rows", x), _row_stride("out", res)
-    work = torch.empty(((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction),), dtype=torch.uint8,
-                       device=x.device)
-    _call("comfy_moe_block_matmul", x.device, _ptr(x), ld_x, _HALF_CODES[x.dtype], _ptr(work), _ptr(w), ld_w,
-          _group_stride("weights", w) if offsets is not None else 0, _ptr(w_scale), int(transpose), r,
-          w.shape[0] if offsets is not None else 1, n, k, _ptr(offsets), _ptr(counts), _ptr(bias), int(out is None),
-          _ptr(res), ld_out, _ptr(device_status(x.device)))
+    n, k = w.size(-2), w.size(-1)
+    if n % 8 or k % 16 or contraction % 16 or n == 0 or k == 0:
+        raise ValueError(f"in_features must be a multiple of 16 and out_features of 8 (of 16 for a gradient), got {k} and {n}")
+    nb, kb = _blocks(n), _blocks(k)
+    if w_scale.dtype != torch.float32 or w_scale.shape != ((nb, kb) if offsets is None else (w.size(0), nb, kb)) or \
+            not w_scale.is_contiguous():
+        raise ValueError(f"the scales must be a contiguous fp32 tensor [.., {nb}, {kb}] for each group")
+    groups = step = 1
+    if offsets is not None:
+        groups = w.size(0)
+        _check_ragged(offsets, counts, groups)
+        step = _group_stride("weights", w, 16)
+    if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.size(0) != n or not bias.is_contiguous() or
+                             bias.data_ptr() % 16):
+        raise ValueError("bias must be a contiguous vector over the output features in the rows' dtype")
+    res = _result(out, x, r, k if transpose else n)
+    work = None
+    if transpose or r > N.FEW_ROWS_BLOCK or k > N.FEW_ROWS_BLOCK_MAX_K:      # the quantised rows and their scales
+        work = torch.empty((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction), dtype=torch.uint8,
+                           device=x.device)
+    _call("comfy_moe_block_matmul", index, x.data_ptr(), _row_stride("rows", x, 8), code, _address(work), w.data_ptr(),
+          _row_stride("weights", w, 16), step, w_scale.data_ptr(), transpose, r, groups, n, k, _address(offsets),
+          _address(counts), _address(bias), out is None, res.data_ptr(), _row_stride("out", res, 8),
+          device_status(x.device).data_ptr())
     return res
 
 
@@ -1017,13 +1053,10 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ (w * scales).T + bias`` in e4m3: x [.., K] (bf16 or fp16) is quantised by blocks of 128 on the way
     (quantize_blocks_e4m3), w is e4m3 [N, K] with w_scale [ceil(N / 128), ceil(K / 128)] (quantize_weight_blocks_e4m3),
-    bias [N] in x's dtype; sums in fp32, result [.., N] in x's dtype.  Differentiable (once) in x, whose gradient is the
-    same product with the gradient of the result quantised and the weight transposed, and in bias; w is frozen."""
+    bias [N] in x's dtype; K a multiple of 16, N of 8 (of 16 where a gradient is asked for); sums in fp32, result [.., N]
+    in x's dtype.  Differentiable (once) in x, whose gradient is the same product with the gradient of the result
+    quantised and the weight transposed, and in bias; w is frozen."""
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    _check_block(rows, w, w_scale, 1, 2, bias)
-    if bias is not None and (bias.dtype != x.dtype or bias.shape != w.shape[:1] or not bias.is_contiguous() or
-                             bias.data_ptr() % 16):
-        raise ValueError("bias must be a contiguous vector over the output features in the rows' dtype")
     if _asks_for_gradient(x, w, w_scale, bias, out):
         y = _BlockLinear.apply(rows, w, w_scale, bias)
     else:
@@ -1031,13 +1064,12 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
         y = _block_product(rows, w, w_scale, None, None, bias, flat, False)
         if out is not None:
             return out
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (w.shape[0],))
+    return y if rows is x else y.view(x.shape[:-1] + (w.shape[0],))
 
 
 def block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dy @ (w * scales)`` in e4m3: the gradient of block_linear for x.  dy [R, N] -> [R, K]; N a multiple of 16."""
-    _check_block(dy, w, w_scale, 0, 2)
     return _block_product(dy, w, w_scale, None, None, None, out, True)
 
 
@@ -1046,8 +1078,6 @@ def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor
     """block_linear by expert: ``y[r] = x[r] @ (w[g] * scales[g]).T`` for the rows r of group g.  x [R, K], w e4m3
     [G, N, K], w_scale [G, ceil(N / 128), ceil(K / 128)]; offsets, counts, out and rows of no group as for grouped_matmul,
     the quantised rows and the gradient (x only) as for block_linear."""
-    _check_block(x, w, w_scale, 2, 3, offsets, counts)
-    _check_ragged(offsets, counts, w.shape[0])
     if _asks_for_gradient(x, w, w_scale, None, out):
         return _GroupedBlockLinear.apply(x, w, w_scale, offsets, counts)
     return _block_product(x, w, w_scale, offsets, counts, None, out, False)
@@ -1056,8 +1086,6 @@ def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor
 def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
                                counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dx[r] = dy[r] @ (w[g] * scales[g])``: the gradient of grouped_block_linear for x.  dy [R, N] -> [R, K]."""
-    _check_block(dy, w, w_scale, 1, 3, offsets, counts)
-    _check_ragged(offsets, counts, w.shape[0])
     return _block_product(dy, w, w_scale, offsets, counts, None, out, True)
 
 
@@ -1068,10 +1096,10 @@ class _BlockLinear(torch.autograd.Function):
         return _block_product(x, w, w_scale, None, None, bias, None, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("block_linear")
         dy = _readable(dy)
-        dx = block_linear_dgrad(dy, *ctx.saved_tensors) if ctx.needs_input_grad[0] else None
+        dx = _block_product(dy, *ctx.saved_tensors, None, None, None, None, True) if ctx.needs_input_grad[0] else None
         db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, db
 
@@ -1083,6 +1111,6 @@ class _GroupedBlockLinear(torch.autograd.Function):
         return _block_product(x, w, w_scale, offsets, counts, None, None, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return grouped_block_linear_dgrad(_readable(dy), *ctx.saved_tensors), None, None, None, None
+        _once("grouped_block_linear")
+        return _block_product(_readable(dy), *ctx.saved_tensors, None, None, True), None, None, None, None

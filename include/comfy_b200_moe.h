@@ -393,12 +393,16 @@ int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x,
  *   comfy_moe_block_quantize_weight  weights, one scale for 128 x 128: w [n_groups, out, in] -> out e4m3 (contiguous),
  *                                    scale [n_groups, ceil(out / 128), ceil(in / 128)]
  *   comfy_moe_block_matmul           quantises x (dtype bf16 or fp16) into `workspace` (comfy_moe_block_workspace(rows,
- *                                    contraction) bytes, 16-byte aligned, no two calls at a time) and multiplies:
+ *                                    contraction) bytes, 16-byte aligned, no two calls at a time; not used, and NULL will
+ *                                    do, for at most COMFY_MOE_FEW_ROWS_BLOCK rows of at most COMFY_MOE_FEW_ROWS_BLOCK_MAX_K
+ *                                    elements without transpose_w) and multiplies:
  *                                    out[r, :] = x[r, :] . w[g]^T (+ bias);  transpose_w: out[r, :] = x[r, :] . w[g].
  * Groups of rows, zero_unused, status: as for comfy_moe_grouped_matmul; offsets NULL with n_groups = 1 means all rows.
  * Block products are summed in fp32 and folded, times both scales, into fp32 sums; out (and bias, contiguous) have x's
  * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes. */
 #define COMFY_MOE_SCALE_BLOCK 128
+#define COMFY_MOE_FEW_ROWS_BLOCK 8
+#define COMFY_MOE_FEW_ROWS_BLOCK_MAX_K 24576
 int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
                              float* scale, int64_t ld_scale, void* stream);
 int comfy_moe_block_quantize_weight(const void* w, int64_t ld_w, int64_t w_group_stride, int dtype, int n_groups,

@@ -152,7 +152,7 @@ def close(got, ref, mag, terms, what):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("n,k", [(16, 16), (128, 128), (144, 400), (264, 1040), (2064, 2560)])
-@pytest.mark.parametrize("rows", [1, 9, 33, 128, 300])
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 33, 128, 300])
 def test_dense(cuda_device, rows, n, k, dtype):
     from comfyui_b200 import moe_ops as M
 
@@ -170,13 +170,14 @@ def test_dense(cuda_device, rows, n, k, dtype):
     M.check_all_status()
 
 
-@pytest.mark.parametrize("counts", [[1], [2, 0, 1], [3, 0, 130], [127, 128, 129, 1], [700, 0, 33, 515], [1] * 40],
+@pytest.mark.parametrize("counts", [[1], [2, 0, 1], [0, 8], [3, 0, 130], [127, 128, 129, 1], [700, 0, 33, 515], [1] * 40],
                          ids=lambda c: "-".join(map(str, c))[:20])
+@pytest.mark.parametrize("gap", [0, 1, 7])
 @pytest.mark.parametrize("n,k", [(272, 400), (528, 1040)])
-def test_by_expert(cuda_device, counts, n, k):
+def test_by_expert(cuda_device, counts, n, k, gap):
     from comfyui_b200 import moe_ops as M
 
-    dev, gap = cuda_device, 7
+    dev = cuda_device
     gen = torch.Generator(device=dev).manual_seed(len(counts) + n)
     rows, g = sum(counts) + 2 * gap, len(counts)
     x = torch.randn((rows, k), generator=gen, device=dev).bfloat16()
@@ -190,10 +191,10 @@ def test_by_expert(cuda_device, counts, n, k):
         close(y[lo:hi], *product(x[lo:hi], w[i], ws[i], None, x.dtype), k, f"y of group {i}")
         close(dx[lo:hi], *product(dy[lo:hi], w[i], ws[i], None, x.dtype, True), n, f"dx of group {i}")
     for t in (y, dx):
-        assert (t[:gap] == 0).all() and (t[-gap:] == 0).all()
+        assert (t[:gap] == 0).all() and (t[rows - gap:] == 0).all()
     out = torch.full_like(y, 7.0)
     M.grouped_block_linear(x, w, ws, offsets, out=out)
-    assert torch.equal(out[gap:-gap], y[gap:-gap]) and (out[:gap] == 7).all() and (out[-gap:] == 7).all()
+    assert torch.equal(out[gap:rows - gap], y[gap:rows - gap]) and (out[:gap] == 7).all() and (out[rows - gap:] == 7).all()
     # fewer rows than the offsets leave room for, with values that are not finite in what is left out
     most = torch.tensor([c // 2 for c in counts], dtype=torch.int32, device=dev)
     used = torch.zeros(rows, dtype=torch.bool, device=dev)

@@ -316,3 +316,31 @@ def test_refusals(cuda_device):
     ]:
         with pytest.raises(ValueError, match=match):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("k,n", [(8, 8), (264, 1000), (2560, 6912)])
+@pytest.mark.parametrize("counts,gap", [([1], 0), ([0, 1, 0, 1], 0), ([8], 0), ([5, 0, 4], 0), ([16], 0), ([0, 3, 0], 2), ([15, 1], 0)],
+                         ids=str)
+def test_few_rows(cuda_device, counts, gap, k, n, dtype):
+    """The form that streams the weights for up to 16 rows, and the same call cut out of a longer batch."""
+    from comfyui_b200 import moe_ops as M
+
+    x, w, _, offsets = make(cuda_device, counts, k, n, dtype, gap=gap)
+    ends = offsets.tolist()
+    ranges = list(zip(ends[:-1], ends[1:]))
+    ref = by_group(x, w, ranges, len(x), n, lambda a, b: a @ b.t())
+    y = M.grouped_matmul(x, w, offsets)
+    close(y, *ref, k, "y")
+    long = torch.cat([x, torch.full((64, k), float("nan"), device=x.device, dtype=dtype)])
+    close(M.grouped_matmul(long, w, offsets)[:len(x)], *ref, k, "y of a longer batch")
+    if gap:
+        out = torch.full((len(x), n), 7.0, dtype=dtype, device=x.device)
+        M.grouped_matmul(x, w, offsets, out=out)
+        assert torch.equal(out[gap:-gap], y[gap:-gap]) and (out[:gap] == 7).all() and (out[-gap:] == 7).all()
+        assert (y[:gap] == 0).all() and (y[-gap:] == 0).all()
+    most = torch.tensor([c // 2 for c in counts], dtype=torch.int32, device=x.device)
+    half = M.grouped_matmul(x, w, offsets, most)
+    for (lo, _), c in zip(ranges, counts):
+        assert torch.equal(half[lo:lo + c // 2], y[lo:lo + c // 2]) and (half[lo + c // 2:lo + c] == 0).all()
+    assert torch.equal(M.grouped_matmul(x, w, offsets), y)
