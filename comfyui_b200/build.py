@@ -31,7 +31,7 @@ SOURCES = [
     "weight_ingest.cu",
     "moe_c_api.cu",
 ]
-HEADERS = ["moe_common.cuh", "moe_gate.cuh", "ptx_sm100.cuh", "ragged.cuh", "few_rows.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
+HEADERS = ["moe_common.cuh", "moe_gate.cuh", "ptx_sm100.cuh", "ragged.cuh", "few_rows.cuh", "block_scale.cuh", os.path.join("..", "..", "include", "comfy_b200_moe.h")]
 
 
 def _nvcc() -> str:

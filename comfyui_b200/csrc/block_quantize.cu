@@ -1,14 +1,6 @@
 // e4m3 with a scale for each block of 128: the activation quantiser (blocks of 1 x 128 along a row) and the weight
-// quantiser (blocks of 128 x 128).  For a block with the largest magnitude m = max(max|x|, 2^-100):
-//   scale = m / 448 (fp32),   q = e4m3(x * 448 / m), round to nearest even.
-// x * 448 / m is formed as ((x * 0.4375) / m) * 1024: the product with 7/16 and the last one are exact (bf16, fp16), so there
-// is one rounding, of the quotient, and it never moves a value onto or over a border between two e4m3 values: a quotient
-// of numbers of at most 11 bits that is no border itself is further from it than half a step of fp32.  (x * (1 / scale)
-// would round ties such as x = 0.75 m either way.)  The floor 2^-100 keeps the scales and their products out of the
-// subnormal range; a block of zeros has zeros.  The maximum is taken on the bit patterns, so a NaN or an infinity wins it
-// and reaches every result the block takes part in: its scale is then NaN or infinite, and so is a product with it.
-// Both are bound by HBM: 3 bytes per element (read 2, written 1).
-#include "moe_common.cuh"
+// quantiser (blocks of 128 x 128), by the rule of block_scale.cuh.  Both are bound by HBM: 3 bytes per element of bf16.
+#include "block_scale.cuh"
 
 namespace comfy_b200 {
 
@@ -39,16 +31,14 @@ __device__ __forceinline__ void lane_values(const Lane16<T>& in, float (&v)[kLan
   }
 }
 
-__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-constexpr uint32_t kTinyBits = (127u - 100u) << 23;                 // 2^-100
-
-__device__ __forceinline__ uint4 to_e4m3(const float (&v)[kLaneElems], float top) {
+template <bool kShort>
+__device__ __forceinline__ uint4 to_e4m3(const float (&v)[kLaneElems], const BlockScale& s) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = __fdiv_rn(v[4 * i + j] * 0.4375f, top) * 1024.0f;
+    for (int j = 0; j < 4; ++j) q[j] = block_quotient<kShort>(s, v[4 * i + j]);
     w[i] = static_cast<uint32_t>(f2_to_e4m3x2(q[0], q[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(q[2], q[3])) << 16);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -76,9 +66,9 @@ block_quantize_kernel(const T* __restrict__ x, long long ld, int rows, int cols,
   for (int i = 0; i < kLaneElems; ++i) top = max(top, magnitude_bits(v[i]));
 #pragma unroll
   for (int d = 1; d < kLanesPerBlock; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float m = __uint_as_float(top);
-  if (live) *reinterpret_cast<uint4*>(q + row * ld_q + col) = to_e4m3(v, m);
-  if (l == 0 && row < rows) scale[blockIdx.y * ld_scale + row] = __fdiv_rn(m, 448.0f);
+  const BlockScale s = block_scale(top);
+  if (live) *reinterpret_cast<uint4*>(q + row * ld_q + col) = to_e4m3<sizeof(T) == 2>(v, s);
+  if (l == 0 && row < rows) scale[blockIdx.y * ld_scale + row] = stored_scale(s);
 }
 
 // One 128 x 128 block per CTA, held in registers between the maximum and the division.
@@ -110,15 +100,15 @@ block_quantize_weight_kernel(const T* __restrict__ w, long long ld, long long gr
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, s_top[i]);
-  const float m = __uint_as_float(top);
-  if (threadIdx.x == 0) scale[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = __fdiv_rn(m, 448.0f);
+  const BlockScale s = block_scale(top);
+  if (threadIdx.x == 0) scale[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = stored_scale(s);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = blockIdx.y * kQuantBlock + i * 32 + r0;
     if (row < n && col < k) {
       float v[kLaneElems];
       lane_values<T>(in[i], v);
-      *reinterpret_cast<uint4*>(q + (static_cast<long long>(blockIdx.z) * n + row) * k + col) = to_e4m3(v, m);
+      *reinterpret_cast<uint4*>(q + (static_cast<long long>(blockIdx.z) * n + row) * k + col) = to_e4m3<sizeof(T) == 2>(v, s);
     }
   }
 }

@@ -8,6 +8,7 @@
 // and 128 rows of one of them.)  The warps' partial sums are joined in a fixed order: the result is the same every time.
 #include <algorithm>
 
+#include "block_scale.cuh"
 #include "few_rows.cuh"
 #include "ragged.cuh"
 
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p
   few_store<T, kTiles>(p, part, c, begin, count, n0);
 }
 
-// Block-scaled: the block's weights are on their way while its warps quantise the rows (by the rule of block_quantize.cu),
+// Block-scaled: the block's weights are on their way while its warps quantise the rows (by the rule of block_scale.cuh),
 // each the blocks that it multiplies; a block's 16 x 8 products are folded, scaled, into the warp's sums.
 constexpr int kFewBlk = COMFY_MOE_SCALE_BLOCK;
 
@@ -196,20 +197,20 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewPa
       for (int i = 0; i < kFlight; ++i) {
         const T* e = reinterpret_cast<const T*>(&raw[i]);
         float v[4];
-        uint32_t top = (127u - 100u) << 23;                              // 2^-100
+        uint32_t top = kTinyBits;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           v[q] = to_float(e[q]);
-          top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
+          top = max(top, magnitude_bits(v[q]));
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        const float m = __uint_as_float(top);
+        const BlockScale bs = block_scale(top);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = __fdiv_rn(v[q] * 0.4375f, m) * 1024.0f;
+        for (int q = 0; q < 4; ++q) v[q] = block_quotient<true>(bs, v[q]);
         if (b0 + i * kFewWarps < blocks)
           reinterpret_cast<uint32_t*>(xq + ((b0 + i * kFewWarps) * 8 + row) * kFewBlk)[lane] =
               static_cast<uint32_t>(f2_to_e4m3x2(v[0], v[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(v[2], v[3])) << 16);
-        const float s = __fdiv_rn(m, 448.0f);
+        const float s = stored_scale(bs);
         if (row == 2 * t) xs[i][0] = s;
         if (row == 2 * t + 1) xs[i][1] = s;
       }

@@ -79,6 +79,22 @@ def test_every_ratio_of_two_bf16_numbers(cuda_device):
     assert torch.equal(bytes_of(q), bytes_of(want)) and torch.equal(scale, want_scale.float())
 
 
+@pytest.mark.parametrize("top", [1024, 1025, 1365, 1366, 1535, 1792, 1793, 2047], ids=str)
+def test_every_significand_of_fp16(cuda_device, top):
+    """x / m for all 11-bit significands of x over the powers of two that e4m3 covers, and both signs."""
+    from comfyui_b200 import moe_ops as M
+
+    dev = cuda_device
+    sig = torch.arange(1024, 2048, device=dev).double()
+    x = sig[None, :] / (2.0 ** torch.arange(19, device=dev).double())[:, None] * 4.0
+    x = torch.cat([x, -x]).flatten()
+    x = torch.nn.functional.pad(x, (0, -x.numel() % (BLOCK - 1))).view(-1, BLOCK - 1)
+    x = torch.cat([torch.full((len(x), 1), 8.0 * top, device=dev, dtype=torch.float64), x.clamp(-8.0 * top, 8.0 * top)], 1).half()
+    q, scale = M.quantize_blocks_e4m3(x)
+    want, want_scale = quantised(x)
+    assert torch.equal(bytes_of(q), bytes_of(want)) and torch.equal(scale, want_scale.float())
+
+
 def test_fp32_rows(cuda_device):
     """fp32 values: the quotient's one rounding may move a value onto a border, by less than 2^-23 of it."""
     from comfyui_b200 import moe_ops as M
