@@ -8,6 +8,8 @@ What is mirrored (same names, arguments and behaviour, Linear only — the MoE p
 * ``fp8_linear`` (``:314-358``), ``fp8_ops.Linear`` (``:360-377``), ``scaled_fp8_ops(...)`` (``:379-428``);
 * ``pick_operations`` (``:449-473``).
 
+``block_scaled_fp8_ops(...)`` is a namespace of the same kind for weights with one scale per 128 x 128 block.
+
 What is new: the dispatch shim at the bottom.  ``hidream_moe_forward`` / ``hidream_moe_infer`` /
 ``hidream_gate`` / ``swiglu_ffn_forward`` check, on every call, whether the module's current weights
 can be handed to the sm_100a kernels (bf16, or e4m3 with per-tensor scales; resident on the input's
@@ -266,6 +268,58 @@ def scaled_fp8_ops(fp8_matrix_mult=False, scale_input=False, override_dtype=None
                     self.weight = torch.nn.Parameter(q, requires_grad=False)
 
     return scaled_fp8_op
+
+
+def _spread_block_scales(scale: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """One factor per element from one per 128 x 128 block."""
+    return scale.repeat_interleave(128, -2)[..., :rows, :].repeat_interleave(128, -1)[..., :cols]
+
+
+def block_scaled_fp8_ops(fp8_matrix_mult=True):
+    """Namespace factory for block-scaled fp8 weights, the finer sibling of ``scaled_fp8_ops``: ``weight`` e4m3 plus a
+    ``scale_weight`` of one fp32 factor for each 128 x 128 block, [ceil(out / 128), ceil(in / 128)].  With
+    ``fp8_matrix_mult`` (and activations in bf16 or fp16 on a B200) a Linear multiplies in e4m3, its input quantised by
+    blocks of 128 on the way (``moe_ops.block_linear``); otherwise the weight is scaled back and multiplied in the
+    activation's dtype.  The weights are frozen; a gradient reaches the input and the bias."""
+    use_kernel = fp8_matrix_mult
+
+    class block_scaled_fp8_op(manual_cast):
+        class Linear(manual_cast.Linear):
+            def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
+                super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+                self.weight = torch.nn.Parameter(torch.empty((out_features, in_features), device=device, dtype=FP8),
+                                                 requires_grad=False)
+                self.scale_weight = torch.nn.Parameter(
+                    torch.ones((-(-out_features // 128), -(-in_features // 128)), device=device, dtype=torch.float32),
+                    requires_grad=False)
+
+            def forward_comfy_cast_weights(self, input):
+                if use_kernel:
+                    out = block_linear_forward(self, input)
+                    if out is not None:
+                        return out
+                weight, bias = cast_bias_weight(self, input)
+                return F.linear(input, self.convert_weight(weight), bias)
+
+            def convert_weight(self, weight, inplace=False, **kwargs):
+                scale = _spread_block_scales(self.scale_weight, *weight.shape).to(device=weight.device, dtype=weight.dtype)
+                if inplace:
+                    weight *= scale
+                    return weight
+                return weight * scale
+
+            def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
+                scaled = weight / _spread_block_scales(self.scale_weight, *weight.shape).to(device=weight.device,
+                                                                                           dtype=weight.dtype)
+                q = stochastic_rounding(scaled, self.weight.dtype, seed=seed)
+                if return_weight:
+                    return q
+                if inplace_update:
+                    self.weight.data.copy_(q)
+                else:
+                    self.weight = torch.nn.Parameter(q, requires_grad=False)
+
+    return block_scaled_fp8_op
 
 
 _FP8_FORMATS = {torch.float8_e4m3fn: (4, 3, 7), torch.float8_e5m2: (5, 2, 15)}     # exponent bits, mantissa bits, bias
@@ -623,6 +677,34 @@ def swiglu_ffn_forward(ffn, x: torch.Tensor) -> Optional[torch.Tensor]:
         x2 = moe_ops.quantize_e4m3(x2, pack.scale_in13)     # the activation quantiser of comfy/ops.py:338-343
     _, y, _, _ = moe_ops.grouped_swiglu([], pack, None, None, None, x2, check_status=CHECK_STATUS_EVERY_CALL)
     return y.view(x.shape)
+
+
+# ---- block-scaled fp8 Linear -------------------------------------------------------------------------------------
+def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
+    """A Linear of ``block_scaled_fp8_ops`` on the block-scaled product, or None when this call is not eligible: bf16 or
+    fp16 input on a B200 with the weight and its scales beside it, no patch closures, in_features a multiple of 16,
+    out_features of 8 (of 16 where a gradient is asked for)."""
+    w, s, b = lin.weight, lin.scale_weight, lin.bias
+    if not ENABLE_SM100_KERNELS or lin.weight_function or lin.bias_function or not x.is_cuda or \
+            x.dtype not in (torch.bfloat16, torch.float16) or not model_management.is_sm100(x.device):
+        return None
+    if w.dtype != FP8 or w.device != x.device or s.device != x.device or s.dtype != torch.float32 or \
+            w.shape[1] % 16 or w.shape[0] % 8 or not w.is_contiguous() or w.data_ptr() % 16 or not s.is_contiguous():
+        return None
+    grad = torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad))
+    if grad and w.shape[0] % 16:
+        return None
+    if b is not None:
+        b = model_management.cast_to(b, dtype=x.dtype, device=x.device)
+        if b.data_ptr() % 16:
+            return None
+    rows = x.reshape(-1, x.shape[-1])
+    if rows.stride(-1) != 1 or rows.data_ptr() % 16 or (rows.shape[0] > 1 and (rows.stride(0) % 8 or rows.stride(0) < rows.shape[1])):
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    from . import moe_ops
+
+    with _Range("comfyui_b200::block_linear"):
+        return moe_ops.block_linear(rows, w, s, b).view(x.shape[:-1] + (w.shape[0],))
 
 
 # ---- q / k / v glue of the HiDream attention processor ----------------------------------------------------------

@@ -198,3 +198,83 @@ def layer_args(layer: moe_ops.LayerPack):
 
     return ([f.w1 for f in ffns], [f.w3 for f in ffns], [f.w2 for f in ffns], col("scale_w1"), col("scale_w3"),
             col("scale_w2"), col("scale_in13"), col("scale_in2"))
+
+
+# ---- products by expert and with block scales: the tensor-level functions of moe_ops as operators, for tracing --------
+def _no_grad(fn, *args, **kwargs):
+    with torch.no_grad():
+        return fn(*args, **kwargs)
+
+
+@torch.library.custom_op("comfyui_b200::grouped_matmul", mutates_args=())
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                   counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """moe_ops.grouped_matmul: rows x [R, K] by expert against w [G, N, K]."""
+    return _no_grad(moe_ops.grouped_matmul, x, w, offsets, counts)
+
+
+@grouped_matmul.register_fake
+def _(x, w, offsets, counts=None):
+    return x.new_empty((x.shape[0], w.shape[1]))
+
+
+@torch.library.custom_op("comfyui_b200::grouped_matmul_dgrad", mutates_args=())
+def grouped_matmul_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                         counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """moe_ops.grouped_matmul_dgrad of a gradient of any layout."""
+    return _no_grad(moe_ops.grouped_matmul_dgrad, moe_ops._readable(dy), w, offsets, counts)
+
+
+@grouped_matmul_dgrad.register_fake
+def _(dy, w, offsets, counts=None):
+    return dy.new_empty((dy.shape[0], w.shape[2]))
+
+
+@torch.library.custom_op("comfyui_b200::grouped_matmul_wgrad", mutates_args=())
+def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
+                         counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """moe_ops.grouped_matmul_wgrad of a gradient of any layout, in x's dtype."""
+    return _no_grad(moe_ops.grouped_matmul_wgrad, moe_ops._readable(dy), x, offsets, counts)
+
+
+@grouped_matmul_wgrad.register_fake
+def _(dy, x, offsets, counts=None):
+    return x.new_empty((offsets.shape[0] - 1, dy.shape[1], x.shape[1]))
+
+
+def _grouped_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _grouped_backward(ctx, dy):
+    x, w, offsets, counts = ctx.saved_tensors
+    ops = torch.ops.comfyui_b200
+    return (ops.grouped_matmul_dgrad(dy, w, offsets, counts) if ctx.needs_input_grad[0] else None,
+            ops.grouped_matmul_wgrad(dy, x, offsets, counts) if ctx.needs_input_grad[1] else None, None, None)
+
+
+grouped_matmul.register_autograd(_grouped_backward, setup_context=_grouped_setup)
+
+
+@torch.library.custom_op("comfyui_b200::block_linear", mutates_args=())
+def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """moe_ops.block_linear: x [.., K] against e4m3 w [N, K] with block scales."""
+    return _no_grad(moe_ops.block_linear, x, w, w_scale, bias)
+
+
+@block_linear.register_fake
+def _(x, w, w_scale, bias=None):
+    return x.new_empty(x.shape[:-1] + (w.shape[0],))
+
+
+@torch.library.custom_op("comfyui_b200::grouped_block_linear", mutates_args=())
+def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
+                         counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """moe_ops.grouped_block_linear: rows x [R, K] by expert against e4m3 w [G, N, K] with block scales."""
+    return _no_grad(moe_ops.grouped_block_linear, x, w, w_scale, offsets, counts)
+
+
+@grouped_block_linear.register_fake
+def _(x, w, w_scale, offsets, counts=None):
+    return x.new_empty((x.shape[0], w.shape[1]))

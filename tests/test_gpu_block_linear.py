@@ -358,3 +358,85 @@ def test_refusals(cuda_device):
             call()
     with pytest.raises(ValueError, match="frozen"):
         M.block_linear(x, w, ws.clone().requires_grad_(True))
+
+
+def test_linear_of_the_namespace(cuda_device):
+    """ops.block_scaled_fp8_ops: a Linear on the kernel, beside its composition; bias and input gradients; fallbacks."""
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import ops
+
+    dev, n, k = cuda_device, 144, 272
+    gen = torch.Generator(device=dev).manual_seed(3)
+    lin = ops.block_scaled_fp8_ops().Linear(k, n, device=dev, dtype=torch.bfloat16)
+    w, ws = M.quantize_weight_blocks_e4m3(torch.randn((n, k), generator=gen, device=dev))
+    bias = torch.randn((n,), generator=gen, device=dev).bfloat16()
+    lin.load_state_dict({"weight": w, "scale_weight": ws, "bias": bias}, strict=True)
+    x = torch.randn((2, 9, k), generator=gen, device=dev).bfloat16().requires_grad_(True)
+    y = lin(x)
+    assert y.shape == (2, 9, n) and torch.equal(y, M.block_linear(x.detach(), w, ws, bias))
+    dy = torch.randn(y.shape, generator=gen, device=dev).bfloat16()
+    dx, db = torch.autograd.grad(y, (x, lin.bias), dy)
+    assert torch.equal(dx.view(-1, k), M.block_linear_dgrad(dy.view(-1, n), w, ws))
+    close(db[None], dy.double().sum((0, 1))[None], dy.double().abs().sum((0, 1))[None], 18, "bias")
+    wide = torch.randn((2, 9, k + 3), generator=gen, device=dev).bfloat16()[..., 3:]          # rows that no kernel reads
+    with torch.no_grad():
+        assert torch.equal(lin(wide), lin(wide.contiguous()))
+        f32 = lin(x.float())                                                                   # the composition
+        assert f32.dtype == torch.float32
+        torch.testing.assert_close(f32, x.float() @ full(w, ws, BLOCK).float().t() + bias.float(), rtol=1e-4, atol=1e-3)
+        lin.weight_function = [lambda t: 0 * t]
+        assert torch.equal(lin(x), bias.expand(2, 9, n))
+
+
+def test_a_layer_of_the_namespace(cuda_device):
+    """The mixture-of-experts module built with block-scaled Linears: finite, and near the layer with the weights scaled back."""
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import ops
+    from comfyui_b200.ldm.hidream.model import MOEFeedForwardSwiGLU
+
+    dev, dim, hidden = cuda_device, 512, 1024
+    gen = torch.Generator(device=dev).manual_seed(5)
+    layer = MOEFeedForwardSwiGLU(dim, hidden, 4, 2, dtype=torch.bfloat16, device=dev, operations=ops.block_scaled_fp8_ops())
+    plain = MOEFeedForwardSwiGLU(dim, hidden, 4, 2, dtype=torch.bfloat16, device=dev, operations=ops.disable_weight_init)
+    state, back = {}, {}
+    for name, p in layer.state_dict().items():
+        if name.endswith("scale_weight"):
+            continue
+        t = 0.05 * torch.randn(p.shape, generator=gen, device=dev)
+        if p.dtype == torch.float8_e4m3fn:
+            w, s = M.quantize_weight_blocks_e4m3(t)
+            state[name], state[name.replace("weight", "scale_weight")] = w, s
+            back[name] = full(w, s, BLOCK).bfloat16()
+        else:
+            state[name] = back[name] = t.bfloat16()
+    layer.load_state_dict(state, strict=True)
+    plain.load_state_dict(back, strict=True)
+    x = torch.randn((2, 150, dim), generator=gen, device=dev).bfloat16()
+    with torch.inference_mode():
+        y, ref = layer(x), plain(x)
+    # what differs is the rounding of each product's input to e4m3: 2^-4 of a value at most, a third of that in the mean
+    # square (the error is spread evenly over a step, half a step at most), over two products in a row: 2^-4 / 3 x sqrt(2) < 0.03,
+    # and as much again for the share that the non-linear product of the first two adds
+    err = (y.double() - ref.double()).norm() / ref.double().norm()
+    assert torch.isfinite(y).all() and err < 0.06, err
+
+
+def test_registered_operators(cuda_device):
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import torch_ops  # noqa: F401
+
+    dev, n, k = cuda_device, 144, 272
+    gen = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn((50, k), generator=gen, device=dev).bfloat16()
+    w = torch.randn((2, n, k), generator=gen, device=dev).bfloat16()
+    wq, ws = M.quantize_weight_blocks_e4m3(w)
+    off = torch.tensor([0, 20, 50], dtype=torch.int32, device=dev)
+    ops = torch.ops.comfyui_b200
+    assert torch.equal(ops.grouped_matmul(x, w, off), M.grouped_matmul(x, w, off))
+    assert torch.equal(ops.block_linear(x, wq[0], ws[0]), M.block_linear(x, wq[0], ws[0]))
+    assert torch.equal(ops.grouped_block_linear(x, wq, ws, off), M.grouped_block_linear(x, wq, ws, off))
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    got = torch.autograd.grad(ops.grouped_matmul(x, w, off).sum(), (x, w))
+    want = torch.autograd.grad(M.grouped_matmul(x, w, off).sum(), (x, w))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
