@@ -375,8 +375,7 @@ static int launch_block(const BlockParams& p, int sms, cudaStream_t stream) {
     return cudaFuncGetAttributes(&a, block_matmul_kernel<kTransposed, kCtas>) == cudaSuccess ? a.numRegs : 0;
   }();
   if (regs < kFpLaunchRegs) return COMFY_MOE_EUNSUPPORTED;
-  const size_t smem = FpShape<kCtas>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
-  return launch_ragged<kCtas>(block_matmul_kernel<kTransposed, kCtas>, p, kFpThreads, smem, sms, stream);
+  return launch_ragged<block_matmul_kernel<kTransposed, kCtas>, kCtas>(p, kFpThreads, FpShape<kCtas>::kTables, sms, stream);
 }
 
 static int64_t scale_offset(int64_t rows, int64_t cols) { return (rows * cols + 255) / 256 * 256; }

@@ -238,32 +238,34 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewPa
   few_store<T, 1>(p, part, sum, begin, count, n0);
 }
 
-template <typename Kernel>
-static int launch_few(Kernel kernel, const FewParams& p, size_t smem, cudaStream_t stream) {
+template <auto kKernel>
+static int launch_few(const FewParams& p, size_t smem, size_t most, cudaStream_t stream) {
   const dim3 grid((p.n + kFewCols - 1) / kFewCols, p.groups + (p.zero_unused && p.offsets ? 1 : 0));
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-    return COMFY_MOE_ECUDA;
-  kernel<<<grid, kFewThreads, smem, stream>>>(p);
+  if (smem > 32 * 1024) {                      // beyond what a kernel may have unasked, beside its static part
+    const int rc = allow_shared_memory<kKernel>(most);
+    if (rc != COMFY_MOE_OK) return rc;
+  }
+  kKernel<<<grid, kFewThreads, smem, stream>>>(p);
   return check_launch();
 }
 
 static size_t few_tables(const FewParams& p) {
-  return p.zero_unused && p.offsets ? (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) : 0;
+  return p.zero_unused && p.offsets ? ragged_tables(p.groups) : 0;
 }
 
 int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
   if (p.rows <= 8)
-    return fp16 ? launch_few(few_rows_kernel<__half, 1>, p, few_tables(p), stream)
-                : launch_few(few_rows_kernel<__nv_bfloat16, 1>, p, few_tables(p), stream);
-  return fp16 ? launch_few(few_rows_kernel<__half, 2>, p, few_tables(p), stream)
-              : launch_few(few_rows_kernel<__nv_bfloat16, 2>, p, few_tables(p), stream);
+    return fp16 ? launch_few<few_rows_kernel<__half, 1>>(p, few_tables(p), 0, stream)
+                : launch_few<few_rows_kernel<__nv_bfloat16, 1>>(p, few_tables(p), 0, stream);
+  return fp16 ? launch_few<few_rows_kernel<__half, 2>>(p, few_tables(p), 0, stream)
+              : launch_few<few_rows_kernel<__nv_bfloat16, 2>>(p, few_tables(p), 0, stream);
 }
 
 int launch_few_rows_block(const FewParams& p, bool fp16, cudaStream_t stream) {
   const size_t smem = std::max(static_cast<size_t>((p.k + kFewBlk - 1) / kFewBlk) * 8 * kFewBlk, few_tables(p));
-  return fp16 ? launch_few(few_rows_block_kernel<__half>, p, smem, stream)
-              : launch_few(few_rows_block_kernel<__nv_bfloat16>, p, smem, stream);
+  constexpr size_t most = static_cast<size_t>(kFewBlockMaxK) * 8;
+  return fp16 ? launch_few<few_rows_block_kernel<__half>>(p, smem, most, stream)
+              : launch_few<few_rows_block_kernel<__nv_bfloat16>>(p, smem, most, stream);
 }
 
 }  // namespace comfy_b200

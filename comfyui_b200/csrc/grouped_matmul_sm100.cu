@@ -350,9 +350,8 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
 
 template <int kForm, int kBN, int kCtas>
 static int launch_gmm(const GmmParams& p, int sms, cudaStream_t stream) {
-  const size_t smem = GmmShape<kBN, kCtas>::kTables + (3 * static_cast<size_t>(p.groups) + 1) * sizeof(int) + 1024;
-  return launch_ragged<kCtas>(grouped_matmul_kernel<kForm, kBN, kCtas>, p,
-                              kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, smem, sms, stream);
+  return launch_ragged<grouped_matmul_kernel<kForm, kBN, kCtas>, kCtas>(
+      p, kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, GmmShape<kBN, kCtas>::kTables, sms, stream);
 }
 
 template <int kForm>

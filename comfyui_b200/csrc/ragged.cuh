@@ -154,24 +154,44 @@ inline int ragged_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes
 // Number of SMs of the current device, or a negative value where it is no sm_100.  A thread that has not launched anything
 // yet (autograd's, in a backward pass) has no context that the tensor-map encoder could use: cudaSetDevice makes it one.
 inline int sm100_count() {
-  int dev = 0, major = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess ||
+  static thread_local int known = -1, sms = 0;
+  int dev = 0, major = 0, count = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -COMFY_MOE_ECUDA;
+  if (dev == known) return sms;
+  if (cudaSetDevice(dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return -COMFY_MOE_ECUDA;
-  return major == 10 ? sms : -COMFY_MOE_EDEVICE;
+  known = dev;
+  sms = major == 10 ? count : -COMFY_MOE_EDEVICE;
+  return sms;
 }
 
-// One persistent CTA (or CTA pair) per SM (pair).
-template <int kCtas, typename Params>
-int launch_ragged(void (*kernel)(Params), const Params& p, int threads, size_t smem, int sms, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+// Opts a kernel in to `bytes` of dynamic shared memory, once per thread and device.
+template <auto kKernel>
+int allow_shared_memory(size_t bytes) {
+  static thread_local int done = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return COMFY_MOE_ECUDA;
+  if (dev == done) return COMFY_MOE_OK;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess)
     return COMFY_MOE_ECUDA;
+  done = dev;
+  return COMFY_MOE_OK;
+}
+
+constexpr size_t ragged_tables(int groups) { return (3 * static_cast<size_t>(groups) + 1) * sizeof(int); }
+
+// One persistent CTA (or CTA pair) per SM (pair); `fixed` bytes of shared memory besides the groups' tables.
+template <auto kKernel, int kCtas, typename Params>
+int launch_ragged(const Params& p, int threads, size_t fixed, int sms, cudaStream_t stream) {
+  const int rc = allow_shared_memory<kKernel>(fixed + ragged_tables(kRaggedMaxGroups) + 1024);
+  if (rc != COMFY_MOE_OK) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(sms / kCtas * kCtas));
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = fixed + ragged_tables(p.groups) + 1024;      // (1024: the stages start on a multiple of it)
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -179,7 +199,7 @@ int launch_ragged(void (*kernel)(Params), const Params& p, int threads, size_t s
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? check_launch() : COMFY_MOE_ECUDA;
+  return cudaLaunchKernelEx(&cfg, kKernel, p) == cudaSuccess ? check_launch() : COMFY_MOE_ECUDA;
 }
 
 }  // namespace comfy_b200

@@ -842,6 +842,8 @@ def _group_stride(what: str, t: torch.Tensor, unit: int) -> int:
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """A gradient as autograd hands it over (possibly expanded or transposed), as rows that the kernels can read."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     unit = 16 // t.element_size()
     ok = t.stride(-1) == 1 and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0)) and \
         t.data_ptr() % 16 == 0
@@ -870,9 +872,10 @@ def _once(what: str) -> None:
         raise RuntimeError(f"{what} is differentiable once: its gradient has no gradient")
 
 
-def _rows_by_group(name: str, a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
-                   out: Optional[torch.Tensor], width: int) -> torch.Tensor:
-    """grouped_matmul (width 2) or its gradient for the rows (width 1)."""
+def _grouped_sizes(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
+                   width: int) -> tuple:
+    """What the C entry points want to know of checked rows and weights: (device index, dtype code, rows, groups, N, K,
+    row stride of a, row and group stride of w)."""
     if a.dim() != 2 or w.dim() != 3 or a.size(1) != w.size(width):
         raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(a.shape)} and {tuple(w.shape)}")
     index = _place(a, w, offsets, counts)
@@ -881,11 +884,20 @@ def _rows_by_group(name: str, a: torch.Tensor, w: torch.Tensor, offsets: torch.T
         raise ValueError(f"rows and weights must both be bf16 or both fp16, got {a.dtype} and {w.dtype}")
     g, n, k = w.shape
     _check_ragged(offsets, counts, g)
-    r = a.size(0)
-    res = _result(out, a, r, n if width == 2 else k)
-    _call(name, index, a.data_ptr(), _row_stride("rows", a, 8), w.data_ptr(), _row_stride("weights", w, 8),
-          _group_stride("weights", w, 8), code, r, g, n, k, offsets.data_ptr(), _address(counts), out is None,
-          res.data_ptr(), _row_stride("out", res, 8), device_status(a.device).data_ptr())
+    return (index, code, a.size(0), g, n, k, _row_stride("rows", a, 8), _row_stride("weights", w, 8),
+            _group_stride("weights", w, 8))
+
+
+def _rows_by_group(name: str, sizes: tuple, a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                   counts: Optional[torch.Tensor], out: Optional[torch.Tensor], cols: int) -> torch.Tensor:
+    index, code, r, g, n, k, ld_a, ld_w, step = sizes
+    if out is None:
+        res, ld = a.new_empty((r, cols)), cols
+    else:
+        res = _result(out, a, r, cols)
+        ld = _row_stride("out", res, 8)
+    _call(name, index, a.data_ptr(), ld_a, w.data_ptr(), ld_w, step, code, r, g, n, k, offsets.data_ptr(), _address(counts),
+          out is None, res.data_ptr(), ld, device_status(a.device).data_ptr())
     return res
 
 
@@ -900,13 +912,15 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
         if out is not None:
             raise ValueError("grouped_matmul: out cannot be given where a gradient is asked for")
         return _GroupedMatmul.apply(x, w, offsets, counts)
-    return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, out, 2)
+    sizes = _grouped_sizes(x, w, offsets, counts, 2)
+    return _rows_by_group("comfy_moe_grouped_matmul", sizes, x, w, offsets, counts, out, sizes[4])
 
 
 def grouped_matmul_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dx[r] = dy[r] @ w[g]``: the gradient of grouped_matmul for x.  dy [R, N] -> [R, K]; rows of no group as there."""
-    return _rows_by_group("comfy_moe_grouped_matmul_dgrad", dy, w, offsets, counts, out, 1)
+    sizes = _grouped_sizes(dy, w, offsets, counts, 1)
+    return _rows_by_group("comfy_moe_grouped_matmul_dgrad", sizes, dy, w, offsets, counts, out, sizes[5])
 
 
 def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -943,15 +957,27 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, counts):
         ctx.save_for_backward(x, w, offsets, counts)
-        return _rows_by_group("comfy_moe_grouped_matmul", x, w, offsets, counts, None, 2)
+        ctx.sizes = sizes = _grouped_sizes(x, w, offsets, counts, 2)
+        return _rows_by_group("comfy_moe_grouped_matmul", sizes, x, w, offsets, counts, None, sizes[4])
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_matmul")
         x, w, offsets, counts = ctx.saved_tensors
+        index, code, r, g, n, k, ld_x, ld_w, step = ctx.sizes      # checked by the forward pass; dy has the result's shape
+        need_x, need_w = ctx.needs_input_grad[:2]
         dy = _readable(dy)
-        dx = grouped_matmul_dgrad(dy, w, offsets, counts) if ctx.needs_input_grad[0] else None
-        dw = grouped_matmul_wgrad(dy, x, offsets, counts) if ctx.needs_input_grad[1] else None
+        ld_dy = n if r <= 1 else dy.stride(0)
+        dx = dw = None
+        if need_x:
+            sizes = (index, code, r, g, n, k, ld_dy, ld_w, step)
+            dx = _rows_by_group("comfy_moe_grouped_matmul_dgrad", sizes, dy, w, offsets, counts, None, k)
+        if need_w:
+            dw = x.new_empty((g, n, k))
+            if g:
+                _call("comfy_moe_grouped_matmul_wgrad", index, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, r, g, n, k,
+                      offsets.data_ptr(), _address(counts), code, dw.data_ptr(), k, n * k,
+                      device_status(x.device).data_ptr())
         return dx, dw, None, None
 
 
@@ -995,12 +1021,11 @@ def quantize_weight_blocks_e4m3(w: torch.Tensor):
     return q, scale
 
 
-def _block_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: Optional[torch.Tensor],
-                   counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
-                   transpose: bool) -> torch.Tensor:
-    """The four block-scaled products: dense (offsets None) or by expert, of the rows or of their gradient (transpose)."""
-    dims = 2 if offsets is None else 3
-    if w.dim() != dims or x.dim() != 2 or x.size(1) != w.size(-2 if transpose else -1):
+def _block_sizes(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: Optional[torch.Tensor],
+                 counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], transpose: bool) -> tuple:
+    """What the C entry point wants to know of checked operands: (device index, dtype code, rows, groups, N, K, row stride
+    of x, row and group stride of w).  offsets None: one group, w [N, K]; transpose: x is a gradient [R, N]."""
+    if w.dim() != (2 if offsets is None else 3) or x.dim() != 2 or x.size(1) != w.size(-2 if transpose else -1):
         raise ValueError(f"need rows and weights that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
     index = _place(x, w, w_scale, offsets, counts, bias)
     code = _HALF_CODES.get(x.dtype)
@@ -1022,15 +1047,25 @@ def _block_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offs
     if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.size(0) != n or not bias.is_contiguous() or
                              bias.data_ptr() % 16):
         raise ValueError("bias must be a contiguous vector over the output features in the rows' dtype")
-    res = _result(out, x, r, k if transpose else n)
+    return index, code, r, groups, n, k, _row_stride("rows", x, 8), _row_stride("weights", w, 16), step
+
+
+def _block_product(sizes: tuple, x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: Optional[torch.Tensor],
+                   counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
+                   transpose: bool) -> torch.Tensor:
+    index, code, r, groups, n, k, ld_x, ld_w, step = sizes
+    contraction, cols = (n, k) if transpose else (k, n)
+    if out is None:
+        res, ld = x.new_empty((r, cols)), cols
+    else:
+        res = _result(out, x, r, cols)
+        ld = _row_stride("out", res, 8)
     work = None
     if transpose or r > N.FEW_ROWS_BLOCK or k > N.FEW_ROWS_BLOCK_MAX_K:      # the quantised rows and their scales
-        work = torch.empty((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction), dtype=torch.uint8,
-                           device=x.device)
-    _call("comfy_moe_block_matmul", index, x.data_ptr(), _row_stride("rows", x, 8), code, _address(work), w.data_ptr(),
-          _row_stride("weights", w, 16), step, w_scale.data_ptr(), transpose, r, groups, n, k, _address(offsets),
-          _address(counts), _address(bias), out is None, res.data_ptr(), _row_stride("out", res, 8),
-          device_status(x.device).data_ptr())
+        work = x.new_empty((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction), dtype=torch.uint8)
+    _call("comfy_moe_block_matmul", index, x.data_ptr(), ld_x, code, _address(work), w.data_ptr(), ld_w, step,
+          w_scale.data_ptr(), transpose, r, groups, n, k, _address(offsets), _address(counts), _address(bias), out is None,
+          res.data_ptr(), ld, device_status(x.device).data_ptr())
     return res
 
 
@@ -1061,7 +1096,8 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
         y = _BlockLinear.apply(rows, w, w_scale, bias)
     else:
         flat = out if out is None or out.dim() == 2 else out.view(-1, out.shape[-1])
-        y = _block_product(rows, w, w_scale, None, None, bias, flat, False)
+        sizes = _block_sizes(rows, w, w_scale, None, None, bias, False)
+        y = _block_product(sizes, rows, w, w_scale, None, None, bias, flat, False)
         if out is not None:
             return out
     return y if rows is x else y.view(x.shape[:-1] + (w.shape[0],))
@@ -1070,7 +1106,7 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
 def block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dy @ (w * scales)`` in e4m3: the gradient of block_linear for x.  dy [R, N] -> [R, K]; N a multiple of 16."""
-    return _block_product(dy, w, w_scale, None, None, None, out, True)
+    return _block_product(_block_sizes(dy, w, w_scale, None, None, None, True), dy, w, w_scale, None, None, None, out, True)
 
 
 def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
@@ -1080,26 +1116,36 @@ def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor
     the quantised rows and the gradient (x only) as for block_linear."""
     if _asks_for_gradient(x, w, w_scale, None, out):
         return _GroupedBlockLinear.apply(x, w, w_scale, offsets, counts)
-    return _block_product(x, w, w_scale, offsets, counts, None, out, False)
+    sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
+    return _block_product(sizes, x, w, w_scale, offsets, counts, None, out, False)
 
 
 def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
                                counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dx[r] = dy[r] @ (w[g] * scales[g])``: the gradient of grouped_block_linear for x.  dy [R, N] -> [R, K]."""
-    return _block_product(dy, w, w_scale, offsets, counts, None, out, True)
+    sizes = _block_sizes(dy, w, w_scale, offsets, counts, None, True)
+    return _block_product(sizes, dy, w, w_scale, offsets, counts, None, out, True)
+
+
+def _block_backward(ctx, dy: torch.Tensor, w, w_scale, offsets, counts) -> torch.Tensor:
+    index, code, r, groups, n, k, _, ld_w, step = ctx.sizes        # checked by the forward pass; dy has the result's shape
+    sizes = (index, code, r, groups, n, k, n if r <= 1 else dy.stride(0), ld_w, step)
+    return _block_product(sizes, dy, w, w_scale, offsets, counts, None, None, True)
 
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, bias):
         ctx.save_for_backward(w, w_scale)
-        return _block_product(x, w, w_scale, None, None, bias, None, False)
+        ctx.sizes = sizes = _block_sizes(x, w, w_scale, None, None, bias, False)
+        return _block_product(sizes, x, w, w_scale, None, None, bias, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("block_linear")
+        w, w_scale = ctx.saved_tensors
         dy = _readable(dy)
-        dx = _block_product(dy, *ctx.saved_tensors, None, None, None, None, True) if ctx.needs_input_grad[0] else None
+        dx = _block_backward(ctx, dy, w, w_scale, None, None) if ctx.needs_input_grad[0] else None
         db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, db
 
@@ -1108,9 +1154,10 @@ class _GroupedBlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, offsets, counts):
         ctx.save_for_backward(w, w_scale, offsets, counts)
-        return _block_product(x, w, w_scale, offsets, counts, None, None, False)
+        ctx.sizes = sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
+        return _block_product(sizes, x, w, w_scale, offsets, counts, None, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_block_linear")
-        return _block_product(_readable(dy), *ctx.saved_tensors, None, None, True), None, None, None, None
+        return _block_backward(ctx, _readable(dy), *ctx.saved_tensors), None, None, None, None
