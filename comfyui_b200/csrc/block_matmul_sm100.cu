@@ -159,6 +159,10 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
       // ------------------------------------------------------------------ MMA issuer (of the leader)
       int s = 0, acc = 0;
       uint32_t phase = 0;
+      const uint32_t a_addr = smem_u32(smem), b_addr = a_addr + kFpUnit * kFpOperand;
+      const uint64_t a_first = umma_desc_k_sw128(a_addr);
+      const uint64_t b_first = kTransposed ? (kPair ? umma_desc_mn_sw64(b_addr) : umma_desc_mn_sw128(b_addr, kFpOperand))
+                                           : umma_desc_k_sw128(b_addr);
       bool ok = true;
       for (int t = unit; t < total && ok && rank == 0; t += units) {
         for (int kb = 0; kb < steps; kb += kFpUnit) {
@@ -168,10 +172,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
           if (elect_one()) {
             // 32 steps of the contraction per MMA: 32 bytes along a K-major row, 32 rows of an MN-major box
             constexpr uint32_t kAdvB = kTransposed ? (32 * Shape::kCols) >> 4 : 2;
-            const uint32_t a_addr = smem_u32(smem + s * kStageBytes), b_addr = a_addr + kFpUnit * kFpOperand;
-            const uint64_t a_desc = umma_desc_k_sw128(a_addr);
-            const uint64_t b_desc = kTransposed ? (kPair ? umma_desc_mn_sw64(b_addr) : umma_desc_mn_sw128(b_addr, kFpOperand))
-                                                : umma_desc_k_sw128(b_addr);
+            const uint64_t a_desc = a_first + s * (kStageBytes >> 4), b_desc = b_first + s * (kStageBytes >> 4);
 #pragma unroll
             for (int u = 0; u < kFpUnit; ++u) {
               const uint32_t d_tmem = tmem_base + (acc * kFpUnit + u) * kFpTile;
@@ -249,51 +250,49 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
     };
 #pragma unroll
     for (int i = 0; i < kFpAcc; ++i) hand_back();     // the first steps find their accumulators free
-    int stage = 0, acc = 0, slot = 0;
-    uint32_t phase = 0, slot_phase = 0;
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0, acc_addr = lane_base;      // (accumulators alternate: TMEM's columns begin at 0)
     bool ok = true;
     for (int t = unit; t < total && ok; t += units) {
       float sum[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0.f;
       int4 tile = make_int4(0, 0, 0, 0);
-      const float* scales = nullptr;
-      for (int kb = 0; kb < steps; kb += kFpUnit) {
-        if (kb % kScaleSteps == 0) {
-          ok = mbar_wait_warp(&scale_full_bar[slot], slot_phase, abort_ptr);
-          if (!ok) { give_up(kStatusRaggedEpilogue); break; }
-          scales = scale_ring + slot * kScaleSteps * kFpTile + quarter * 32 + lane;
-          tile = tile_ring[slot];
-        }
-        float scale[kFpUnit];
-#pragma unroll
-        for (int u = 0; u < kFpUnit; ++u) scale[u] = scales[u * kFpTile];
-        scales += kFpUnit * kFpTile;
-        ok = mbar_wait_warp(&empty_bar[stage], phase, abort_ptr);
+      for (int kb = 0; kb < steps && ok; kb += kScaleSteps) {
+        ok = mbar_wait_warp(&scale_full_bar[slot], slot_phase, abort_ptr);
         if (!ok) { give_up(kStatusRaggedEpilogue); break; }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-        phase ^= stage == 0;
-        tc_fence_after_sync();
-        uint32_t r[kFpUnit][2][32];
+        const float* scales = scale_ring + slot * kScaleSteps * kFpTile + quarter * 32 + lane;
+        tile = tile_ring[slot];
 #pragma unroll
-        for (int u = 0; u < kFpUnit; ++u) {
-          tmem_ld_32x32b_x32(lane_base + (acc * kFpUnit + u) * kFpTile, r[u][0]);
-          tmem_ld_32x32b_x32(lane_base + (acc * kFpUnit + u) * kFpTile + 32, r[u][1]);
+        for (int v = 0; v < kScaleSteps; v += kFpUnit) {
+          if (kb + v >= steps) break;
+          ok = mbar_wait_warp(&empty_bar[stage], phase, abort_ptr);
+          if (!ok) { give_up(kStatusRaggedEpilogue); break; }
+          stage = stage + 1 == kStages ? 0 : stage + 1;
+          phase ^= stage == 0;
+          tc_fence_after_sync();
+          uint32_t r[kFpUnit][2][32];
+          float scale[kFpUnit];
+#pragma unroll
+          for (int u = 0; u < kFpUnit; ++u) {
+            tmem_ld_32x32b_x32(acc_addr + u * kFpTile, r[u][0]);
+            tmem_ld_32x32b_x32(acc_addr + u * kFpTile + 32, r[u][1]);
+            scale[u] = scales[(v + u) * kFpTile];
+          }
+          acc_addr ^= kFpUnit * kFpTile;
+          tmem_ld_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          hand_back();
+#pragma unroll
+          for (int u = 0; u < kFpUnit; ++u)
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sum[j] = fmaf(__uint_as_float(r[u][j >> 5][j & 31]), scale[u], sum[j]);
         }
-        acc = (acc + 1) % kFpAcc;
-        tmem_ld_wait();
-        tc_fence_before_sync();
         __syncwarp();
-        hand_back();
-#pragma unroll
-        for (int u = 0; u < kFpUnit; ++u)
-#pragma unroll
-          for (int j = 0; j < 64; ++j) sum[j] = fmaf(__uint_as_float(r[u][j >> 5][j & 31]), scale[u], sum[j]);
-        if (kb % kScaleSteps == kScaleSteps - kFpUnit || kb + kFpUnit >= steps) {
-          if (lane == 0) mbar_arrive(&scale_empty_bar[slot]);      // (the warp has met since it read its scales)
-          slot = slot + 1 == kScaleSlots ? 0 : slot + 1;
-          slot_phase ^= slot == 0;
-        }
+        if (lane == 0) mbar_arrive(&scale_empty_bar[slot]);
+        slot = slot + 1 == kScaleSlots ? 0 : slot + 1;
+        slot_phase ^= slot == 0;
       }
       if (!ok) break;
       const int row0 = tile.x + rank * kFpTile + quarter * 32, rows_here = tile.z - row0;
