@@ -297,34 +297,40 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
       if (!ok) break;
       const int row0 = tile.x + rank * kFpTile + quarter * 32, rows_here = tile.z - row0;
       if (rows_here <= 0) continue;
+      const int col0 = tile.y + half * 64;
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (col0 + q * 8 >= p.n_total) break;
+          const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.bias) + col0 / 8 + q);
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                                    : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+            sum[q * 8 + 2 * j] += f.x;
+            sum[q * 8 + 2 * j + 1] += f.y;
+          }
+        }
+      }
+      uint32_t packed[32];
+      if (p.fp16) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) packed[j] = pack_f16x2(sum[2 * j], sum[2 * j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) packed[j] = pack_bf16x2(sum[2 * j], sum[2 * j + 1]);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int col = tile.y + half * 64 + i * 32;
-        if (col >= p.n_total) continue;
+        const int col = col0 + i * 32;
+        if (col >= p.n_total) break;
         if (lane == 0) bulk_wait_read_all();
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = sum[i * 32 + q * 8 + j];
-          if (p.bias != nullptr && col + q * 8 < p.n_total) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.bias) + col / 8 + q);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
-                                      : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-              v[2 * j] += f.x;
-              v[2 * j + 1] += f.y;
-            }
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = p.fp16 ? pack_f16x2(v[2 * j], v[2 * j + 1]) : pack_bf16x2(v[2 * j], v[2 * j + 1]);
-          *reinterpret_cast<uint4*>(store + store_piece(lane, q)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(store + store_piece(lane, q)) =
+              make_uint4(packed[i * 16 + q * 4], packed[i * 16 + q * 4 + 1], packed[i * 16 + q * 4 + 2], packed[i * 16 + q * 4 + 3]);
         if (rows_here >= 32) {
           fence_proxy_async_smem();
           __syncwarp();
