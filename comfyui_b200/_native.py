@@ -21,7 +21,7 @@ MAX_EXPERTS = 8
 STATIC_MAX_TOKENS = 131072
 STATUS_WORDS = 4         # [0] sticky device status, [1] near-ties of the last gate call, [2] e4m3 overflows, [3] reserved
 SCALE_BLOCK = 128            # COMFY_MOE_SCALE_BLOCK: elements along a row that share a scale
-FEW_ROWS_BLOCK, FEW_ROWS_BLOCK_MAX_K = 8, 24576      # COMFY_MOE_FEW_ROWS_BLOCK*: calls that need no workspace
+FEW_ROWS_BLOCK, FEW_ROWS_BLOCK_MAX_K = 2, 65536      # COMFY_MOE_FEW_ROWS_BLOCK*: calls that need no workspace
 RAGGED_MAX_GROUPS = 768      # COMFY_MOE_RAGGED_MAX_GROUPS: groups of one call over ragged rows
 LINEAR_MAX_MAPS = 22     # COMFY_MOE_LINEAR_MAX_MAPS: distinct operands of one comfy_moe_grouped_linear call
 MAX_RANKS = 8

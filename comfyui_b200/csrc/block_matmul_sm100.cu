@@ -8,7 +8,7 @@
 // What bounds it is the hand-over between the MMA warp and the epilogue: a wait costs either side 150 cycles even on a
 // complete barrier, a block's MMAs take 256, and a way from one CTA of a pair to the other some hundred.  So two blocks
 // share a stage, a wait, a commit and a hand-over: 8192 rows, 2560 -> 6912 took 194 us with one block at a time and takes
-// 165 (without the quantiser; 1760 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
+// 160 (without the quantiser; 1810 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
 // need (what it hands back is tensor memory whose reads are complete), cost a thousand cycles each: 300 us.
 // Group rows, tile order and stores as in grouped_matmul_sm100.cu.
 #include "few_rows.cuh"
@@ -406,8 +406,8 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   if (n_groups > kRaggedMaxGroups || k % 16 || in % 16 || cols % 8) return COMFY_MOE_EUNSUPPORTED;
   if (n_groups != 1 && !offsets) return COMFY_MOE_EINVAL;
   if (rows == 0) return COMFY_MOE_OK;
-  const bool few = !transpose_w && rows <= kFewRowsBlock && k <= kFewBlockMaxK;
-  if (!x || (!workspace && !few) || !out || !aligned16(x) || !aligned16(workspace) || !aligned16(out) || ld_x < in || ld_x % 8 ||
+  const bool quantise_inside = !transpose_w && rows <= kFewRowsQuantise && k <= kFewQuantiseMaxK;
+  if (!x || (!workspace && !quantise_inside) || !out || !aligned16(x) || !aligned16(workspace) || !aligned16(out) || ld_x < in || ld_x % 8 ||
       ld_out < cols || ld_out % 8 || (bias && !aligned16(bias)))
     return COMFY_MOE_EINVAL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -422,21 +422,24 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   const int sms = sm100_count();
   if (sms < 0) return -sms;
   const int nb = (n + kBlk - 1) / kBlk, kb = (k + kBlk - 1) / kBlk;
-  if (few) {
+  uint8_t* q = static_cast<uint8_t*>(workspace);
+  float* xs = quantise_inside ? nullptr : reinterpret_cast<float*>(q + scale_offset(rows, in));
+  int rc = quantise_inside ? COMFY_MOE_OK : comfy_moe_block_quantize(x, ld_x, dtype, rows, in, q, in, xs, rows, stream);
+  if (rc != COMFY_MOE_OK) return rc;
+  if (!transpose_w && rows <= kFewRowsBlock) {
     FewParams f;
     memset(&f, 0, sizeof(f));
-    f.x = static_cast<const uint8_t*>(x); f.w = static_cast<const uint8_t*>(w); f.out = static_cast<uint8_t*>(out);
+    f.x = quantise_inside ? static_cast<const uint8_t*>(x) : q;
+    f.ld_x = quantise_inside ? ld_x * 2 : in;
+    f.xs = xs; f.ld_xs = rows;
+    f.w = static_cast<const uint8_t*>(w); f.out = static_cast<uint8_t*>(out);
     f.offsets = offsets; f.counts = counts;
     f.ws = w_scale; f.ws_group = static_cast<long long>(nb) * kb;
     f.bias = bias;
-    f.ld_x = ld_x * 2; f.ld_w = ld_w; f.w_group = w_group_stride; f.ld_out = ld_out * 2;
+    f.ld_w = ld_w; f.w_group = w_group_stride; f.ld_out = ld_out * 2;
     f.groups = n_groups; f.rows = rows; f.n = n; f.k = k; f.zero_unused = zero_unused;
     return launch_few_rows_block(f, dtype == COMFY_MOE_FP16, s);
   }
-  uint8_t* q = static_cast<uint8_t*>(workspace);
-  float* xs = reinterpret_cast<float*>(q + scale_offset(rows, in));
-  int rc = comfy_moe_block_quantize(x, ld_x, dtype, rows, in, q, in, xs, rows, stream);
-  if (rc != COMFY_MOE_OK) return rc;
   BlockParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

@@ -6,7 +6,7 @@
 // x * (448 / m), two roundings and thus at most two units of 2^-24 off, is rounded to 21 significant bits first: that
 // moves a value back onto the border where the quotient is one, and never onto or over one where it is not; the conversion
 // then rounds as it would the exact quotient.  A full division per element makes the quantiser bound by instructions
-// (17 us for 8192 x 2560 against NEW).  fp32 values keep the division: ((x * 0.4375) / m) * 1024 has one rounding.
+// (17 us for 8192 x 2560 against 12.7).  fp32 values keep the division: ((x * 0.4375) / m) * 1024 has one rounding.
 // The floor 2^-100 keeps the scales and their products out of the subnormal range; a block of zeros has zeros.  The maximum is
 // taken on the bit patterns, so a NaN or an infinity wins it and reaches every result the block takes part in: its scale
 // is then NaN or infinite.

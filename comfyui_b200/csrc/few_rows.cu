@@ -1,11 +1,14 @@
 // Products of a few rows with weights that are read once: the single-token form of the grouped products and of the
 // block-scaled ones.  At up to 16 rows the weights are all there is to move (2 flops per byte and row), so the work is cut
 // for HBM: a block takes 16 output columns of one group over the whole contraction, its eight warps the chunks of it in
-// turns, and every lane keeps several 16-byte loads of weights in flight, ten rows' worth of lines per warp.  The
-// arithmetic is one mma.sync tile: 16 output columns x 8 rows, A = weights, B = rows, both operands in the registers that
-// the loads filled: the tile's steps of the contraction may come in any order as long as both sides agree, so a lane's 16
-// contiguous bytes serve two MMAs without a shuffle or shared memory.  (tcgen05 would need both operands in shared memory
-// and 128 rows of one of them.)  The warps' partial sums are joined in a fixed order: the result is the same every time.
+// turns, and every lane keeps up to ten 16-byte loads of weights in flight.  The arithmetic is one mma.sync tile per eight
+// rows: 16 output columns x 8 rows, A = weights, B = rows, both operands in the registers that the loads filled: the
+// tile's steps of the contraction may come in any order as long as both sides agree, so a lane's 16 contiguous bytes serve
+// two MMAs without a shuffle or shared memory.  (tcgen05 would need both operands in shared memory and 128 rows of one of
+// them.)  The warps' partial sums are joined in a fixed order: the result is the same every time.
+// Measured (device time, us, cold weights, against the tcgen05 kernels): bf16 2560 -> 6912, one group, 1 row 9.9 / 18.5, 16
+// rows 12.7 / 17.7 (HBM: 5.4); four groups, 8 rows 23.5 / 43.2 (all of them busy: 21.6); eight groups 2048 -> 8192, 16 rows
+// 54.4 / 64.1 (41).
 #include <algorithm>
 
 #include "block_scale.cuh"
@@ -148,13 +151,16 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p
   few_store<T, kTiles>(p, part, c, begin, count, n0);
 }
 
-// Block-scaled: the block's weights are on their way while its warps quantise the rows (by the rule of block_scale.cuh),
-// each the blocks that it multiplies; a block's 16 x 8 products are folded, scaled, into the warp's sums.
+// Block-scaled.  kQuantise: one or two rows are quantised here, by every block again (by the rule of block_scale.cuh; each
+// warp the blocks that it multiplies), while its weights are on their way: no workspace, one launch.  That costs 1.2 us a
+// row at 2560 -> 6912, a launch of the quantiser 1.7 us and the host 3 us, so from three rows on, up to eight, they come
+// quantised.  Measured as above: one group, 1 row 8.5 / 12.7, 8 rows 8.5 / 12.7 (HBM: 2.7); four groups, 8 rows 19.8 / 30.3;
+// 1024 -> 1024, 8 rows 4.9 / 8.5.  (16 rows, two tiles: 12.1 / 12.4, four groups 28.1 / 30.4, eight 50 / 40: left to tcgen05.)
 constexpr int kFewBlk = COMFY_MOE_SCALE_BLOCK;
 
-template <typename T>
+template <typename T, bool kQuantise>
 __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewParams p) {
-  extern __shared__ __align__(16) uint8_t xq[];            // [blocks of the contraction][8 rows][128]
+  extern __shared__ __align__(16) uint8_t xq[];            // kQuantise: [blocks of the contraction][rows][128]
   __shared__ float part[kFewWarps][kFewCols][9];
   const int grp = blockIdx.y;
   if (grp == p.groups) { few_zero(p, reinterpret_cast<int*>(xq)); return; }
@@ -185,46 +191,61 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewPa
       scale[i] = b < blocks ? __ldg(ws + b) : 0.f;
     }
     float xs[kFlight][2] = {};                 // scales of rows 2 t and 2 t + 1, this lane's columns of the product
-    for (int row = 0; row < count; ++row) {
-      const uint8_t* src = p.x + static_cast<long long>(begin + row) * p.ld_x;
-      uint2 raw[kFlight];
+    if constexpr (kQuantise) {
+      for (int row = 0; row < count; ++row) {
+        const uint8_t* src = p.x + static_cast<long long>(begin + row) * p.ld_x;
+        uint2 raw[kFlight];
 #pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        const int k0 = (b0 + i * kFewWarps) * kFewBlk + lane * 4;
-        raw[i] = k0 < p.k ? load_row(src + 2 * k0) : make_uint2(0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        const T* e = reinterpret_cast<const T*>(&raw[i]);
-        float v[4];
-        uint32_t top = kTinyBits;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          v[q] = to_float(e[q]);
-          top = max(top, magnitude_bits(v[q]));
+        for (int i = 0; i < kFlight; ++i) {
+          const int k0 = (b0 + i * kFewWarps) * kFewBlk + lane * 4;
+          raw[i] = k0 < p.k ? load_row(src + 2 * k0) : make_uint2(0, 0);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const BlockScale bs = block_scale(top);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = block_quotient<true>(bs, v[q]);
-        if (b0 + i * kFewWarps < blocks)
-          reinterpret_cast<uint32_t*>(xq + ((b0 + i * kFewWarps) * 8 + row) * kFewBlk)[lane] =
-              static_cast<uint32_t>(f2_to_e4m3x2(v[0], v[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(v[2], v[3])) << 16);
-        const float s = stored_scale(bs);
-        if (row == 2 * t) xs[i][0] = s;
-        if (row == 2 * t + 1) xs[i][1] = s;
+        for (int i = 0; i < kFlight; ++i) {
+          const T* e = reinterpret_cast<const T*>(&raw[i]);
+          float v[4];
+          uint32_t top = kTinyBits;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[q] = to_float(e[q]);
+            top = max(top, magnitude_bits(v[q]));
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          const BlockScale bs = block_scale(top);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = block_quotient<true>(bs, v[q]);
+          if (b0 + i * kFewWarps < blocks)
+            reinterpret_cast<uint32_t*>(xq + ((b0 + i * kFewWarps) * kFewRowsQuantise + row) * kFewBlk)[lane] =
+                static_cast<uint32_t>(f2_to_e4m3x2(v[0], v[1])) | (static_cast<uint32_t>(f2_to_e4m3x2(v[2], v[3])) << 16);
+          const float s = stored_scale(bs);
+          if (row == 2 * t) xs[i][0] = s;
+          if (row == 2 * t + 1) xs[i][1] = s;
+        }
       }
+      __syncwarp();
+    } else {
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int b = b0 + i * kFewWarps, row = 2 * t + h;
+          if (b < blocks && row < count) xs[i][h] = __ldg(p.xs + b * p.ld_xs + begin + row);
+        }
     }
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
       const int b = b0 + i * kFewWarps;
       float c[4] = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const uint4 x = b < blocks && g < count
-                            ? *reinterpret_cast<const uint4*>(xq + (b * 8 + g) * kFewBlk + s * 64 + t * 16)
-                            : make_uint4(0, 0, 0, 0);
+        const int k0 = b * kFewBlk + s * 64 + t * 16;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (g < count && k0 < p.k) {
+          if constexpr (kQuantise)
+            x = *reinterpret_cast<const uint4*>(xq + (b * kFewRowsQuantise + g) * kFewBlk + s * 64 + t * 16);
+          else
+            x = __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(begin + g) * p.ld_x + k0));
+        }
         mma_16x8x32_e4m3(c, w[i][s][0].x, w[i][s][1].x, w[i][s][0].y, w[i][s][1].y, x.x, x.y);
         mma_16x8x32_e4m3(c, w[i][s][0].z, w[i][s][1].z, w[i][s][0].w, w[i][s][1].w, x.z, x.w);
       }
@@ -261,11 +282,18 @@ int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
               : launch_few<few_rows_kernel<__nv_bfloat16, 2>>(p, few_tables(p), 0, stream);
 }
 
+template <typename T>
+static int launch_block_typed(const FewParams& p, cudaStream_t stream) {
+  if (p.xs == nullptr) {
+    const size_t rows = static_cast<size_t>((p.k + kFewBlk - 1) / kFewBlk) * kFewRowsQuantise * kFewBlk;
+    return launch_few<few_rows_block_kernel<T, true>>(p, std::max(rows, few_tables(p)),
+                                                         static_cast<size_t>(kFewQuantiseMaxK) * kFewRowsQuantise, stream);
+  }
+  return launch_few<few_rows_block_kernel<T, false>>(p, few_tables(p), 0, stream);
+}
+
 int launch_few_rows_block(const FewParams& p, bool fp16, cudaStream_t stream) {
-  const size_t smem = std::max(static_cast<size_t>((p.k + kFewBlk - 1) / kFewBlk) * 8 * kFewBlk, few_tables(p));
-  constexpr size_t most = static_cast<size_t>(kFewBlockMaxK) * 8;
-  return fp16 ? launch_few<few_rows_block_kernel<__half>>(p, smem, most, stream)
-              : launch_few<few_rows_block_kernel<__nv_bfloat16>>(p, smem, most, stream);
+  return fp16 ? launch_block_typed<__half>(p, stream) : launch_block_typed<__nv_bfloat16>(p, stream);
 }
 
 }  // namespace comfy_b200

@@ -4,9 +4,9 @@
 
 namespace comfy_b200 {
 
-constexpr int kFewRows = 16;                   // rows that one pass over bf16 / fp16 weights serves
-constexpr int kFewRowsBlock = COMFY_MOE_FEW_ROWS_BLOCK;            // over block-scaled weights
-constexpr int kFewBlockMaxK = COMFY_MOE_FEW_ROWS_BLOCK_MAX_K;      // whose quantised rows fit into shared memory
+constexpr int kFewRows = 16, kFewRowsBlock = 8;                      // rows that one pass over the weights serves
+constexpr int kFewRowsQuantise = COMFY_MOE_FEW_ROWS_BLOCK;           // block-scaled, quantised on the way
+constexpr int kFewQuantiseMaxK = COMFY_MOE_FEW_ROWS_BLOCK_MAX_K;     // what of them fits into shared memory
 
 struct FewParams {
   const uint8_t* x;
@@ -14,10 +14,11 @@ struct FewParams {
   uint8_t* out;
   const int32_t* offsets;
   const int32_t* counts;
-  const float* ws;                             // block-scaled: scales of the weights
+  const float* ws;                             // block-scaled: scales of the weights,
+  const float* xs;                             // and of the rows [blocks][ld_xs], if x holds quantised ones
   const void* bias;
   long long ld_x, ld_w, w_group, ld_out;       // bytes
-  long long ws_group;
+  long long ws_group, ld_xs;
   int groups, rows, n, k, zero_unused;
 };
 

@@ -401,8 +401,8 @@ int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x,
  * Block products are summed in fp32 and folded, times both scales, into fp32 sums; out (and bias, contiguous) have x's
  * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes. */
 #define COMFY_MOE_SCALE_BLOCK 128
-#define COMFY_MOE_FEW_ROWS_BLOCK 8
-#define COMFY_MOE_FEW_ROWS_BLOCK_MAX_K 24576
+#define COMFY_MOE_FEW_ROWS_BLOCK 2
+#define COMFY_MOE_FEW_ROWS_BLOCK_MAX_K 65536
 int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
                              float* scale, int64_t ld_scale, void* stream);
 int comfy_moe_block_quantize_weight(const void* w, int64_t ld_w, int64_t w_group_stride, int dtype, int n_groups,

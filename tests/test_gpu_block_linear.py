@@ -168,7 +168,7 @@ def close(got, ref, mag, terms, what):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("n,k", [(16, 16), (128, 128), (144, 400), (264, 1040), (2064, 2560)])
-@pytest.mark.parametrize("rows", [1, 3, 8, 9, 33, 128, 300])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 16, 17, 33, 128, 300])
 def test_dense(cuda_device, rows, n, k, dtype):
     from comfyui_b200 import moe_ops as M
 
@@ -186,7 +186,7 @@ def test_dense(cuda_device, rows, n, k, dtype):
     M.check_all_status()
 
 
-@pytest.mark.parametrize("counts", [[1], [2, 0, 1], [0, 8], [3, 0, 130], [127, 128, 129, 1], [700, 0, 33, 515], [1] * 40],
+@pytest.mark.parametrize("counts", [[1], [0, 2], [2, 0, 1], [0, 8], [9, 0, 5], [16], [3, 0, 130], [127, 128, 129, 1], [700, 0, 33, 515], [1] * 40],
                          ids=lambda c: "-".join(map(str, c))[:20])
 @pytest.mark.parametrize("gap", [0, 1, 7])
 @pytest.mark.parametrize("n,k", [(272, 400), (528, 1040)])
@@ -240,6 +240,9 @@ def test_strides_and_shapes(cuda_device):
     assert torch.equal(out[:, 8:8 + n], y.view(-1, n)) and (out[:, :8] == 0).all() and (out[:, 8 + n:] == 0).all()
     assert torch.equal(M.block_linear(x.transpose(1, 2), w, ws), y.transpose(1, 2))
     assert M.block_linear(x[:0], w, ws).shape == (0, 5, 7, n)
+    assert torch.equal(M.block_linear(x[0, 0, 0], w, ws), M.block_linear(x[0, 0, :1], w, ws)[0])
+    into = torch.empty_like(y)
+    assert M.block_linear(x, w, ws, out=into) is into and torch.equal(into, y)
 
 
 def test_gradients_through_autograd(cuda_device):
@@ -263,6 +266,9 @@ def test_gradients_through_autograd(cuda_device):
     assert torch.equal(dx, M.block_linear_dgrad(torch.ones_like(dy), w[0], ws[0]))
     dx, = torch.autograd.grad(M.grouped_block_linear(x, w, ws, offsets), x, dy)
     assert torch.equal(dx, want_g) and (dx[:1] == 0).all() and (dx[30:] == 0).all()
+    for call in (lambda: M.block_linear(x, w[0], ws[0]), lambda: M.grouped_block_linear(x, w, ws, offsets)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(call(), x, dy, create_graph=True)
     # the gradient is that of the product with the quantised operands: <dx, u> = <q(dy) w, u> for any direction u
     u = torch.randn((33, k), generator=gen, device=dev, dtype=torch.float64)
     q, s = quantised(dy)

@@ -173,6 +173,21 @@ def test_no_rows_and_no_groups(cuda_device):
     assert (M.grouped_matmul(x, w, offsets) == 0).all()
 
 
+def test_all_rows_of_no_group(cuda_device):
+    """Every tile list empty: results are zeros, a given one is not touched, the weights' gradient is zero."""
+    from comfyui_b200 import moe_ops as M
+
+    x, w, dy, _ = make(cuda_device, [300, 0], 264, 136, torch.bfloat16)
+    x[:], dy[:] = float("nan"), float("nan")
+    for offsets, counts in (([0, 0, 0], None), ([300, 300, 300], None), ([7, 100, 300], [0, -3])):
+        off = torch.tensor(offsets, dtype=torch.int32, device=cuda_device)
+        cnt = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=cuda_device)
+        assert (M.grouped_matmul(x, w, off, cnt) == 0).all() and (M.grouped_matmul_dgrad(dy, w, off, cnt) == 0).all()
+        assert (M.grouped_matmul_wgrad(dy, x, off, cnt) == 0).all()
+        out = torch.full_like(dy, 7.0)
+        assert (M.grouped_matmul(x, w, off, cnt, out=out) == 7).all()
+
+
 def test_values_that_are_not_finite_stay_in_their_rows(cuda_device):
     from comfyui_b200 import moe_ops as M
 
@@ -208,6 +223,8 @@ def test_gradients_through_autograd(cuda_device):
     assert torch.equal(got, want_dx)
     with torch.no_grad():
         assert not M.grouped_matmul(x, w, offsets).requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(M.grouped_matmul(x, w, offsets), x, dy, create_graph=True)
     with pytest.raises(ValueError, match="out cannot be given"):
         M.grouped_matmul(x, w, offsets, out=torch.empty_like(dy))
 
