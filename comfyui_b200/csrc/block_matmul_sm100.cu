@@ -8,7 +8,7 @@
 // What bounds it is the hand-over between the MMA warp and the epilogue: a wait costs either side 150 cycles even on a
 // complete barrier, a block's MMAs take 256, and a way from one CTA of a pair to the other some hundred.  So two blocks
 // share a stage, a wait, a commit and a hand-over: 8192 rows, 2560 -> 6912 took 194 us with one block at a time and takes
-// 160 (without the quantiser; 1810 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
+// 156 (without the quantiser; 1860 TFLOP/s).  Arrivals at the leader with release semantics, which such a barrier does not
 // need (what it hands back is tensor memory whose reads are complete), cost a thousand cycles each: 300 us.
 // Group rows, tile order and stores as in grouped_matmul_sm100.cu.
 #include "few_rows.cuh"
@@ -39,8 +39,10 @@ template <int kCtas> struct FpShape {
   static constexpr int kCols = kFpTile / kCtas;  // columns that a CTA loads
   static constexpr int kBBytes = kCols * kBlk;   // of one block
   static constexpr int kStageBytes = kFpUnit * (kFpOperand + kBBytes);
-  static constexpr int kStages = kCtas == 2 ? 4 : 3;
-  static constexpr int kScales = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
+  static constexpr int kStages = 3;
+  static constexpr int kStoreTiles = kCtas;      // of an epilogue warp: pairs have room to store both halves without a wait between
+  static constexpr int kStoreBytes = kStoreTiles * kStoreTileBytes;
+  static constexpr int kScales = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreBytes;
   static constexpr int kTables = kScales + kScaleSlots * kScaleSteps * kFpTile * 4;
   static_assert(kStages > kFpAcc, "a stage's barriers are never a whole turn ahead of an epilogue warp");
 };
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
     // ------------------------------------------------------------------ epilogue: one row and half of the columns per thread
     const int quarter = warp & 3, half = (warp - kFpFirst) >> 2;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
-    uint8_t* store = smem + kStages * kStageBytes + (warp - kFpFirst) * kStoreTileBytes;
+    uint8_t* store = smem + kStages * kStageBytes + (warp - kFpFirst) * Shape::kStoreBytes;
     const uint32_t full_addr = kPair ? mapa_shared(smem_u32(full_bar), 0) : smem_u32(full_bar);
     int back = 0;                                // stage of the step whose accumulator is handed back next
     auto hand_back = [&]() {
@@ -325,17 +327,20 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
       for (int i = 0; i < 2; ++i) {
         const int col = col0 + i * 32;
         if (col >= p.n_total) break;
-        if (lane == 0) bulk_wait_read_all();
-        __syncwarp();
+        uint8_t* store_i = store + i % Shape::kStoreTiles * kStoreTileBytes;
+        if (i % Shape::kStoreTiles == 0) {
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(store + store_piece(lane, q)) =
+          *reinterpret_cast<uint4*>(store_i + store_piece(lane, q)) =
               make_uint4(packed[i * 16 + q * 4], packed[i * 16 + q * 4 + 1], packed[i * 16 + q * 4 + 2], packed[i * 16 + q * 4 + 3]);
         if (rows_here >= 32) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&p.map_out, store, col, tile.w + row0);
+            tma_store_2d(&p.map_out, store_i, col, tile.w + row0);
             bulk_commit_group();
           }
         } else {
@@ -345,7 +350,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
             const int row = k * 8 + (lane >> 2), piece = lane & 3;
             if (row < rows_here && col + piece * 8 < p.n_total)
               *reinterpret_cast<uint4*>(p.out + static_cast<long long>(tile.w + row0 + row) * p.ld_out + 2 * (col + piece * 8)) =
-                  *reinterpret_cast<const uint4*>(store + store_piece(row, piece));
+                  *reinterpret_cast<const uint4*>(store_i + store_piece(row, piece));
           }
         }
       }
