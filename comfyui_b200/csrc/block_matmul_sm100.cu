@@ -385,7 +385,8 @@ static int launch_block(const BlockParams& p, int sms, cudaStream_t stream) {
     return cudaFuncGetAttributes(&a, block_matmul_kernel<kTransposed, kCtas>) == cudaSuccess ? a.numRegs : 0;
   }();
   if (regs < kFpLaunchRegs) return COMFY_MOE_EUNSUPPORTED;
-  return launch_ragged<block_matmul_kernel<kTransposed, kCtas>, kCtas>(p, kFpThreads, FpShape<kCtas>::kTables, sms, stream);
+  return launch_ragged<block_matmul_kernel<kTransposed, kCtas>>(p, kFpThreads, FpShape<kCtas>::kTables, kCtas,
+                                                                sms / kCtas * kCtas, stream);
 }
 
 static int64_t scale_offset(int64_t rows, int64_t cols) { return (rows * cols + 255) / 256 * 256; }

@@ -12,6 +12,7 @@
 // loads take what follows, the stores leave it out.  In d W the rows behind the group are part of the sum: a warp of its own
 // overwrites them with zeros in shared memory (both operands: what stands there may be NaN) before they are multiplied.
 //
+// kSplit: a cluster shares each tile's contraction (few tiles, long contraction: plan_gmm).
 // kCtas = 2: two CTAs on an SM pair share one tcgen05.mma.cta_group::2 stream.  Their tile is 256 rows x 256 columns; each
 // loads its own 128 rows of A and half of B's columns, so an SM reads a third less per product than with 128 x 256 of its
 // own, and under the power cap the clock rises by as much.  Barriers as in moe_grouped_gemm_sm100.cu: full and
@@ -21,6 +22,8 @@
 // the leader's `peer` barrier.  (An arrival of the other CTA at every step, so that one barrier would do, halved the rate:
 // 762 us against 412 with single CTAs at 16384 rows, 8 groups, 2048 x 8192.  Zeros by the MMA warp itself held up every
 // tile of a short group: 111 us against 108 at 2048 rows.)
+#include <type_traits>
+
 #include "few_rows.cuh"
 #include "ragged.cuh"
 
@@ -33,13 +36,16 @@ constexpr int kStepK = 64;                     // contraction elements per stage
 constexpr int kABytes = kTileM * 128;
 constexpr int kMnBoxBytes = kStepK * 128;      // one box of an MN-major operand: 64 steps x 64 elements
 
-template <int kBN, int kCtas> struct GmmShape {
-  static constexpr int kTileRows = kTileM * kCtas;
-  static constexpr int kCols = kBN / kCtas;                        // columns of B that one CTA loads
-  static constexpr int kStageBytes = kABytes + kCols * 128;
-  static constexpr int kStages = 6;
-  static constexpr int kTmemCols = 2 * kBN;    // two accumulators: the epilogue of one tile overlaps the next one's MMAs
-  static constexpr int kTables = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
+constexpr int kStageBytes = 2 * kABytes;        // 128 rows of A, 128 columns of B
+constexpr int kPartBytes = 128 * 128 * 4;      // one CTA's sums of a tile (kSplit)
+
+template <int kCtas, bool kSplit> struct GmmShape {
+  static constexpr int kTile = kTileM * kCtas;   // rows and columns
+  static constexpr int kStages = kSplit ? 4 : 6;
+  static constexpr int kTmemCols = 2 * kTile;  // two accumulators: the epilogue of one tile overlaps the next one's MMAs
+  static constexpr int kParts = kStages * kStageBytes;
+  static constexpr int kStores = kParts + (kSplit ? kPartBytes : 0);
+  static constexpr int kTables = kStores + kRaggedEpilogueWarps * kStoreTileBytes;
 };
 
 struct alignas(64) GmmParams {
@@ -48,54 +54,58 @@ struct alignas(64) GmmParams {
   const int32_t* counts;
   uint8_t* out;
   int32_t* status;
-  long long ld_out;                            // bytes
+  long long ld_out, out_group;                 // bytes (d W: out_group from one expert to the next)
   int groups, rows;                            // rows of the buffers
   int m_total;                                 // d W: rows of dw[g] (N); otherwise unused
   int n_total;                                 // output columns
   int k_total;                                 // contraction length (d W: the group's rows, unused)
   int band;                                    // row tiles per band of the tile order
+  int split;                                   // CTAs that share a tile's contraction (kSplit)
   int zero_unused;
   int fp16, out_fp32;
   uint32_t idesc;
 };
 
-template <int kForm, int kBN, int kCtas>
+template <int kForm, int kCtas, bool kSplit>
 __global__ void __launch_bounds__(kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, 1)
 grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
-  using Shape = GmmShape<kBN, kCtas>;
+  using Shape = GmmShape<kCtas, kSplit>;
   constexpr int kStages = Shape::kStages;
-  constexpr int kStageBytes = Shape::kStageBytes;
-  constexpr int kTileRows = Shape::kTileRows;
-  constexpr int kCols = Shape::kCols;
+  constexpr int kTile = Shape::kTile;
   constexpr bool kPair = kCtas == 2;
+  static_assert(!kPair || !kSplit, "a contraction is split among single CTAs");
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ __align__(8) uint64_t tmem_full_bar[2], tmem_empty_bar[2], drain_bar;
   __shared__ __align__(8) uint64_t tail_bar[kStages], peer_bar[kStages];
+  __shared__ __align__(8) uint64_t parts_full_bar, parts_empty_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;      // 0 = leader of the pair
-  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
+  const int split = kSplit ? p.split : 1, part = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / (kCtas * split), units = gridDim.x / (kCtas * split);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
   int* s_count = s_begin + p.groups;
   int* s_first = s_count + p.groups;
 
-  const int n_tiles = (p.n_total + kBN - 1) / kBN;
-  const int m_tiles_w = (p.m_total + kTileRows - 1) / kTileRows;
+  const int n_tiles = (p.n_total + kTile - 1) / kTile;
+  const int m_tiles_w = (p.m_total + kTile - 1) / kTile;
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
       for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps * kCtas); }
       mbar_init(&drain_bar, 1);
       for (int s = 0; s < kStages; ++s) { mbar_init(&tail_bar[s], 1); mbar_init(&peer_bar[s], 1); }
+      mbar_init(&parts_full_bar, kRaggedEpilogueWarps * split);
+      mbar_init(&parts_empty_bar, kRaggedEpilogueWarps * split);
       fence_mbar_init();
       abort_flag = 0;
     }
     __syncwarp();
-    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTileRows,
+    ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTile,
                   kForm == kGradW ? m_tiles_w * n_tiles : n_tiles, s_begin, s_count, s_first);
   } else if (warp == 1) {
     if constexpr (kPair) { tmem_alloc_pair(&tmem_slot, Shape::kTmemCols); tmem_relinquish_pair(); }
@@ -103,7 +113,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   }
   __syncwarp();
   tc_fence_before_sync();
-  if constexpr (kPair) cluster_sync_all();     // the peer's barriers must exist before anything signals them
+  if constexpr (kPair || kSplit) cluster_sync_all();     // the peers' barriers must exist before anything signals them
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
@@ -114,17 +124,22 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   };
 
   // Tiles t = unit, + units, ... in the order of the groups; g only ever moves forward.
-  struct Tile { int m0, n0, begin, count, steps; };
+  struct Tile { int m0, n0, begin, count, first, steps; };      // steps first .. steps - 1 are this CTA's
   auto tile_at = [&](int t, int& g) {
     while (t >= s_first[g + 1]) ++g;
     Tile c;
     c.begin = s_begin[g];
     c.count = s_count[g];
     int m, n;
-    ragged_tile(t - s_first[g], kForm == kGradW ? m_tiles_w : (c.count + kTileRows - 1) / kTileRows, n_tiles, p.band, m, n);
-    c.m0 = m * kTileRows;
-    c.n0 = n * kBN;
+    ragged_tile(t - s_first[g], kForm == kGradW ? m_tiles_w : (c.count + kTile - 1) / kTile, n_tiles, p.band, m, n);
+    c.m0 = m * kTile;
+    c.n0 = n * kTile;
+    c.first = 0;
     c.steps = ((kForm == kGradW ? c.count : p.k_total) + kStepK - 1) / kStepK;
+    if constexpr (kSplit) {
+      c.first = c.steps * part / split;
+      c.steps = c.steps * (part + 1) / split;
+    }
     return c;
   };
 
@@ -134,7 +149,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     bool ok = true;
     for (int t = unit, g = 0; t < total && ok; t += units) {
       const Tile c = tile_at(t, g);
-      for (int kb = 0; kb < c.steps; ++kb, ++it) {
+      for (int kb = c.first; kb < c.steps; ++kb, ++it) {
         const int s = it % kStages;
         ok = mbar_wait_warp(&empty_bar[s], ((it / kStages) & 1u) ^ 1u, abort_ptr);
         if (!ok) { give_up(kStatusRaggedProducer); break; }
@@ -146,13 +161,13 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
           uint64_t* own = tail ? &tail_bar[s] : &full_bar[s];
           if (tail || rank == 0) mbar_arrive_expect_tx(own, tail ? kStageBytes : kCtas * kStageBytes);
           const uint32_t bar = kPair ? mapa_shared(smem_u32(own), tail ? rank : 0) : smem_u32(own);
-          const int m0 = c.m0 + rank * kTileM, n0 = c.n0 + rank * kCols;
+          const int m0 = c.m0 + rank * kTileM, n0 = c.n0 + rank * kTileM;
           if constexpr (kForm == kGradW) {
 #pragma unroll
             for (int i = 0; i < kTileM / 64; ++i)
               load_2d<kPair>(a + i * kMnBoxBytes, &p.map_a, bar, m0 + i * 64, c.begin + kb * kStepK);
 #pragma unroll
-            for (int i = 0; i < kCols / 64; ++i)
+            for (int i = 0; i < kTileM / 64; ++i)
               load_2d<kPair>(b + i * kMnBoxBytes, &p.map_b, bar, n0 + i * 64, c.begin + kb * kStepK);
           } else {
             load_2d<kPair>(a, &p.map_a, bar, kb * kStepK, c.begin + m0);
@@ -160,7 +175,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
               load_3d<kPair>(b, &p.map_b, bar, kb * kStepK, n0, g);
             } else {
 #pragma unroll
-              for (int i = 0; i < kCols / 64; ++i)
+              for (int i = 0; i < kTileM / 64; ++i)
                 load_3d<kPair>(b + i * kMnBoxBytes, &p.map_b, bar, n0 + i * 64, kb * kStepK, g);
             }
           }
@@ -175,14 +190,14 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     bool ok = true;
     for (int t = unit, g = 0; t < total && ok && rank == 0; t += units) {
       const Tile c = tile_at(t, g);
-      if (c.steps == 0) continue;
+      if (c.steps == c.first) continue;
       const uint32_t as = acc & 1u;
       ok = mbar_wait_warp(&tmem_empty_bar[as], ((acc >> 1) & 1u) ^ 1u, abort_ptr);
       if (!ok) { give_up(kStatusRaggedMma); break; }
       ++acc;
       tc_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + as * kBN;
-      for (int kb = 0; kb < c.steps; ++kb, ++it) {
+      const uint32_t d_tmem = tmem_base + as * kTile;
+      for (int kb = c.first; kb < c.steps; ++kb, ++it) {
         const int s = it % kStages;
         ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u, abort_ptr);
         if (!ok) { give_up(kStatusRaggedMma); break; }
@@ -203,8 +218,8 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
           constexpr uint32_t kAdvA = kForm == kGradW ? 128 : 2, kAdvB = kForm == kForward ? 2 : 128;
 #pragma unroll
           for (int k = 0; k < kStepK / 16; ++k) {
-            if constexpr (kPair) umma_ss_pair<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
-            else umma_ss<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, (kb | k) != 0 ? 1u : 0u);
+            if constexpr (kPair) umma_ss_pair<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, kb != c.first || k != 0 ? 1u : 0u);
+            else umma_ss<false>(d_tmem, a_desc + k * kAdvA, b_desc + k * kAdvB, p.idesc, kb != c.first || k != 0 ? 1u : 0u);
           }
           commit<kPair>(&empty_bar[s]);
         }
@@ -226,14 +241,14 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     uint32_t it = 0, tails = 0;                     // bit s: parity of tail_bar[s]
     for (int t = unit, g = 0; t < total; t += units) {
       const Tile c = tile_at(t, g);
-      it += c.steps;
+      it += c.steps - c.first;
       const int valid = c.count - (c.steps - 1) * kStepK;
-      if (c.steps == 0 || valid == kStepK) continue;
+      if (c.steps == c.first || valid >= kStepK) continue;
       const int s = (it - 1) % kStages;
       if (!mbar_wait_warp(&tail_bar[s], (tails >> s) & 1u, abort_ptr)) { give_up(kStatusRaggedMma); break; }
       tails ^= 1u << s;
       uint8_t* a = smem + s * kStageBytes;
-      for (int box = 0; box < (kTileM + kCols) / 64; ++box)
+      for (int box = 0; box < 2 * kTileM / 64; ++box)
         for (int o = valid * 128 + lane * 16; o < kMnBoxBytes; o += 512)
           *reinterpret_cast<uint4*>(a + box * kMnBoxBytes + o) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
@@ -247,13 +262,60 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint8_t* store = smem + kStages * kStageBytes + (warp - 2) * kStoreTileBytes;
-    constexpr int kChunks = kBN / 64;               // chunks of 32 columns of this warp's half
-    uint32_t acc = 0;
+    uint8_t* store = smem + Shape::kStores + (warp - 2) * kStoreTileBytes;
+    // 32 rows from row0 on (inside the group; d W: inside dw[g]) of 32 columns of the output: lane l has row l
+    auto emit = [&](const Tile& c, int g, int row0, int col, const uint32_t (&v)[32]) {
+      const int rows_here = (kForm == kGradW ? p.m_total : c.count) - row0;
+      if (rows_here <= 0 || col >= p.n_total) return;
+      const int sides = kForm == kGradW && p.out_fp32 ? 2 : 1;        // 32 columns of fp32 are two store tiles
+      for (int side = 0; side < sides; ++side) {
+        if (lane == 0) bulk_wait_read_all();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4 piece;
+          if (sides == 2) {
+            // (selected by a loop-invariant condition: v stays in registers)
+            piece = side == 0 ? make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3])
+                              : make_uint4(v[16 + 4 * q], v[17 + 4 * q], v[18 + 4 * q], v[19 + 4 * q]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float lo = __uint_as_float(v[8 * q + 2 * j]), hi = __uint_as_float(v[8 * q + 2 * j + 1]);
+              w[j] = p.fp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+            }
+            piece = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          *reinterpret_cast<uint4*>(store + store_piece(lane, q)) = piece;
+        }
+        const int x = col + side * 16;
+        if (rows_here >= 32 || kForm == kGradW) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kForm == kGradW) tma_store_3d(&p.map_out, store, x, row0, g);
+            else tma_store_2d(&p.map_out, store, x, c.begin + row0);
+            bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = k * 8 + (lane >> 2), piece = lane & 3;
+            if (row < rows_here && x + piece * 8 < p.n_total)
+              *reinterpret_cast<uint4*>(p.out + static_cast<long long>(c.begin + row0 + row) * p.ld_out + 2 * (x + piece * 8)) =
+                  *reinterpret_cast<const uint4*>(store + store_piece(row, piece));
+          }
+        }
+      }
+    };
+    constexpr int kChunks = kTile / 64;             // chunks of 32 columns of this warp's half
+    uint32_t acc = 0, parts_phase = 0;
     for (int t = unit, g = 0; t < total; t += units) {
       const Tile c = tile_at(t, g);
       uint32_t r[kChunks][32];
-      if (c.steps == 0) {
+      if (c.steps == c.first) {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
 #pragma unroll
@@ -265,7 +327,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
         tc_fence_after_sync();
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
-          tmem_ld_32x32b_x32(lane_base + as * kBN + half * (kBN / 2) + i * 32, r[i]);
+          tmem_ld_32x32b_x32(lane_base + as * kTile + half * (kTile / 2) + i * 32, r[i]);
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -274,56 +336,67 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
           else mbar_arrive(&tmem_empty_bar[as]);
         }
       }
-      const int row0 = c.m0 + rank * kTileM + quarter * 32;         // inside the group (d W: inside dw[g])
-      const int rows_here = (kForm == kGradW ? p.m_total : c.count) - row0;
-      const bool whole = rows_here >= 32;
+      if constexpr (kSplit) {
+        // Every CTA lays out its sums, four columns of one row after another: [row / 32][column / 4][row % 32][4].  Then each
+        // of the 8 x split warps adds up 64 / split columns of 32 rows in the order of the parts, and stores them.
+        const int w = warp - 2;
+        uint8_t* mine = smem + Shape::kParts + lane * 16;
+        if (!mbar_wait_warp(&parts_empty_bar, parts_phase ^ 1u, abort_ptr)) { give_up(kStatusRaggedEpilogue); break; }
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int col = c.n0 + half * (kBN / 2) + i * 32;
-        if (rows_here <= 0 || col >= p.n_total) continue;
-        const int parts = kForm == kGradW && p.out_fp32 ? 2 : 1;      // 32 columns of fp32 are two store tiles
-        for (int part = 0; part < parts; ++part) {
-          if (lane == 0) bulk_wait_read_all();
-          __syncwarp();
+        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 v;
-            if (parts == 2) {
-              // (selected by a loop-invariant condition: r stays in registers)
-              v = part == 0 ? make_uint4(r[i][4 * q], r[i][4 * q + 1], r[i][4 * q + 2], r[i][4 * q + 3])
-                            : make_uint4(r[i][16 + 4 * q], r[i][17 + 4 * q], r[i][18 + 4 * q], r[i][19 + 4 * q]);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(mine + ((quarter * 32 + half * 16 + i * 8 + j) << 9)) =
+                make_uint4(r[i][4 * j], r[i][4 * j + 1], r[i][4 * j + 2], r[i][4 * j + 3]);
+        __syncwarp();
+        if (lane < split) mbar_arrive_cluster(mapa_shared(smem_u32(&parts_full_bar), lane));
+        if (!mbar_wait_warp(&parts_full_bar, parts_phase, abort_ptr)) { give_up(kStatusRaggedEpilogue); break; }
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        parts_phase ^= 1u;
+        const int share = (w * split + part) * 16 / split;       // first of its 16 / split quadruples
+        const int row0 = c.m0 + (share >> 5) * 32, col = c.n0 + (share & 31) * 4;
+        auto finish = [&](auto parts) {
+          constexpr int kFrom = decltype(parts)::value, kQuads = 16 / kFrom;
+          float4 v[kFrom][kQuads];
+#pragma unroll
+          for (int from = 0; from < kFrom; ++from) {
+            const uint32_t at = mapa_shared(smem_u32(mine + (share << 9)), from);
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j) v[from][j] = ld_cluster_f4(at + (j << 9));
+          }
+#pragma unroll
+          for (int from = 1; from < kFrom; ++from)
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j) {
+              v[0][j].x += v[from][j].x; v[0][j].y += v[from][j].y; v[0][j].z += v[from][j].z; v[0][j].w += v[from][j].w;
+            }
+          if (row0 + lane >= (kForm == kGradW ? p.m_total : c.count)) return;
+          uint8_t* row = p.out + (kForm == kGradW ? g * p.out_group + static_cast<long long>(row0 + lane) * p.ld_out
+                                                  : static_cast<long long>(c.begin + row0 + lane) * p.ld_out);
+#pragma unroll
+          for (int j = 0; j < kQuads; j += 2) {
+            if (col + 4 * j >= p.n_total) break;
+            if (kForm == kGradW && p.out_fp32) {
+              float4* to = reinterpret_cast<float4*>(row + 4 * (col + 4 * j));
+              to[0] = v[0][j];
+              to[1] = v[0][j + 1];
             } else {
-              uint32_t w[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float lo = __uint_as_float(r[i][8 * q + 2 * j]), hi = __uint_as_float(r[i][8 * q + 2 * j + 1]);
-                w[j] = p.fp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
-              }
-              v = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            *reinterpret_cast<uint4*>(store + store_piece(lane, q)) = v;
-          }
-          const int x = col + part * 16;
-          if (whole || kForm == kGradW) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (kForm == kGradW) tma_store_3d(&p.map_out, store, x, row0, g);
-              else tma_store_2d(&p.map_out, store, x, c.begin + row0);
-              bulk_commit_group();
-            }
-          } else {
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = k * 8 + (lane >> 2), piece = lane & 3;
-              if (row < rows_here && x + piece * 8 < p.n_total)
-                *reinterpret_cast<uint4*>(p.out + static_cast<long long>(c.begin + row0 + row) * p.ld_out +
-                                          2 * (x + piece * 8)) =
-                    *reinterpret_cast<const uint4*>(store + store_piece(row, piece));
+              const float4 a = v[0][j], b = v[0][j + 1];
+              *reinterpret_cast<uint4*>(row + 2 * (col + 4 * j)) =
+                  p.fp16 ? make_uint4(pack_f16x2(a.x, a.y), pack_f16x2(a.z, a.w), pack_f16x2(b.x, b.y), pack_f16x2(b.z, b.w))
+                         : make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
             }
           }
-        }
+        };
+        if (split == 8) finish(std::integral_constant<int, 8>{});
+        else if (split == 4) finish(std::integral_constant<int, 4>{});
+        else finish(std::integral_constant<int, 2>{});
+        __syncwarp();
+        if (lane < split) mbar_arrive_cluster(mapa_shared(smem_u32(&parts_empty_bar), lane));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+          emit(c, g, c.m0 + rank * kTileM + quarter * 32, c.n0 + half * (kTile / 2) + i * 32, r[i]);
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -339,7 +412,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     while (clock64() - t0 < 2000000LL) __nanosleep(1000);     // copies in flight may still land in shared memory
   }
   tc_fence_before_sync();
-  if constexpr (kPair) cluster_sync_all();      // neither CTA leaves while the other may still signal it or use its TMEM
+  if constexpr (kPair || kSplit) cluster_sync_all();      // no CTA leaves while another may still signal it or read from it
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
@@ -348,24 +421,72 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   }
 }
 
-template <int kForm, int kBN, int kCtas>
-static int launch_gmm(const GmmParams& p, int sms, cudaStream_t stream) {
-  return launch_ragged<grouped_matmul_kernel<kForm, kBN, kCtas>, kCtas>(
-      p, kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, GmmShape<kBN, kCtas>::kTables, sms, stream);
-}
-
-template <int kForm>
-static int launch_gmm_ctas(int ctas, const GmmParams& p, int sms, cudaStream_t stream) {
-  return ctas == 2 ? launch_gmm<kForm, 256, 2>(p, sms, stream) : launch_gmm<kForm, 128, 1>(p, sms, stream);
-}
-
 // SM pairs with 256 x 256 tiles where the groups have the rows for them, 128 x 128 tiles of single CTAs below.  Measured (us,
 // pair / single): forward at 512 rows a group 76 / 98, 256: 56 / 58, 64: 42 / 39; dx 119 / 169 (4096 rows), 50 / 44 (64);
 // dw, whose contraction is the group's rows, 100 / 173 (4096 rows), 112 / 120 (256), 92 / 80 (64).  Tiles of 64 columns, and
 // pairs with 128, were never the fastest.
-static int pick_ctas(int64_t rows, int64_t groups, int64_t pair_from) {
+//
+// Where even the 128 x 128 tiles leave half of the SMs without one and the contraction is long, clusters of 2, 4 or 8 CTAs
+// share each tile's contraction and add their sums up through shared memory, in the order of the parts.  The exchange takes
+// 3 us, a step of 64 0.3 us, so it is worth it from 24 steps on.  Measured (us, whole / shared): y at 100 rows, 2 groups,
+// 8192 -> 256: 37.9 / 13.7; 2048 -> 512: 13.5 / 10.8; 1024 -> 256: 9.4 / 9.8; 4 groups, 4096 -> 2048, 64 rows: 23.6 / 18.0;
+// dw 512 x 512 of 8000 rows: 41.7 / 18.3.  All clusters have to be on the device at once (of 8 CTAs it holds 15): a
+// second wave takes as long as the first, 24 instead of 14 us for 16 tiles of 64 steps.
+constexpr int kSplitSteps = 24, kSplitMin = 4;
+struct GmmPlan { int ctas, split, tiles; };
+
+// Clusters of `size` CTAs of the splitting kernel that the current device holds at once.
+static int resident_clusters(int size) {
+  static thread_local int known = -1, held[9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev != known) {
+    constexpr size_t kBytes = GmmShape<1, true>::kTables + ragged_tables(kRaggedMaxGroups) + 1024;
+    const auto kernel = grouped_matmul_kernel<kGradW, 1, true>;
+    if (allow_shared_memory<grouped_matmul_kernel<kGradW, 1, true>>(kBytes) != COMFY_MOE_OK) return 0;
+    for (int s = 2; s <= 8; s *= 2) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cfg.gridDim = dim3(s);
+      cfg.blockDim = dim3(kRaggedTailThreads);
+      cfg.dynamicSmemBytes = kBytes;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = s;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&held[s], kernel, &cfg) != cudaSuccess) { cudaGetLastError(); held[s] = 0; }
+    }
+    known = dev;
+  }
+  return held[size];
+}
+
+static GmmPlan plan_gmm(int64_t rows, int64_t groups, int64_t pair_from, int64_t tiles, int64_t steps, int sms) {
   const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
-  return rows >= pair_from * busy ? 2 : 1;
+  GmmPlan plan = {rows >= pair_from * busy ? 2 : 1, 1, 0};
+  for (int s = 8; s > 1; s /= 2)
+    if (steps >= kSplitSteps && steps >= kSplitMin * s && tiles * s <= sms && tiles <= resident_clusters(s)) {
+      plan.ctas = 1; plan.split = s; plan.tiles = static_cast<int>(tiles);
+      break;
+    }
+  return plan;
+}
+
+static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
+
+template <int kForm, int kCtas, bool kSplit>
+static int launch_gmm(const GmmParams& p, int cluster, int ctas, cudaStream_t stream) {
+  return launch_ragged<grouped_matmul_kernel<kForm, kCtas, kSplit>>(
+      p, kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, GmmShape<kCtas, kSplit>::kTables, cluster, ctas, stream);
+}
+
+template <int kForm>
+static int launch_gmm_plan(const GmmPlan& plan, GmmParams& p, int sms, cudaStream_t stream) {
+  p.split = plan.split;
+  if (plan.split > 1) return launch_gmm<kForm, 1, true>(p, plan.split, plan.tiles * plan.split, stream);
+  return plan.ctas == 2 ? launch_gmm<kForm, 2, false>(p, 2, sms / 2 * 2, stream) : launch_gmm<kForm, 1, false>(p, 1, sms, stream);
 }
 
 static bool rows_ok(const void* p, int64_t ld, int64_t cols, int elem_bytes) {
@@ -420,7 +541,10 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int ctas = pick_ctas(rows, groups, 128);
+  // (no more row tiles than these, however the rows are dealt)
+  const int64_t tiles = (rows / kTileM + (groups < rows ? groups : rows)) * up_to(cols, kTileM);
+  const GmmPlan plan = plan_gmm(rows, groups, 128, tiles, up_to(in, kStepK), sms);
+  const int ctas = plan.ctas;
   if ((rc = ragged_map(&p.map_a, t, 2, a, in, rows, 0, ld_a, 0, 64, kTileM)) != COMFY_MOE_OK) return rc;
   if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? kTileM : kStepK)) != COMFY_MOE_OK)
     return rc;
@@ -436,7 +560,7 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   p.zero_unused = zero_unused;
   p.fp16 = dtype == COMFY_MOE_FP16;
   p.idesc = gmm_idesc(dtype, form, ctas);
-  return form == kForward ? launch_gmm_ctas<kForward>(ctas, p, sms, s) : launch_gmm_ctas<kGradX>(ctas, p, sms, s);
+  return form == kForward ? launch_gmm_plan<kForward>(plan, p, sms, s) : launch_gmm_plan<kGradX>(plan, p, sms, s);
 }
 
 extern "C" int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride,
@@ -473,7 +597,8 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int ctas = pick_ctas(rows, n_groups, 192);
+  const int64_t tiles = n_groups * up_to(n, kTileM) * up_to(k, kTileM);
+  const GmmPlan plan = plan_gmm(rows, n_groups, 192, tiles, rows / n_groups / kStepK, sms);
   if (rows > 0) {
     if ((rc = ragged_map(&p.map_a, t, 2, dy, n, rows, 0, ld_dy, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
     if ((rc = ragged_map(&p.map_b, t, 2, x, k, rows, 0, ld_x, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
@@ -482,13 +607,13 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
                        dw_group_stride, fp32 ? 16 : 32, 32)) != COMFY_MOE_OK)
     return rc;
   p.offsets = offsets; p.counts = counts;
-  p.out = static_cast<uint8_t*>(dw); p.ld_out = ld_dw * out_bytes;
+  p.out = static_cast<uint8_t*>(dw); p.ld_out = ld_dw * out_bytes; p.out_group = dw_group_stride * out_bytes;
   p.status = status;
   p.groups = n_groups; p.rows = rows;
   p.m_total = n; p.n_total = k;
   p.band = 16;
   p.fp16 = dtype == COMFY_MOE_FP16;
   p.out_fp32 = fp32;
-  p.idesc = gmm_idesc(dtype, kGradW, ctas);
-  return launch_gmm_ctas<kGradW>(ctas, p, sms, static_cast<cudaStream_t>(stream));
+  p.idesc = gmm_idesc(dtype, kGradW, plan.ctas);
+  return launch_gmm_plan<kGradW>(plan, p, sms, static_cast<cudaStream_t>(stream));
 }

@@ -182,20 +182,20 @@ int allow_shared_memory(size_t bytes) {
 
 constexpr size_t ragged_tables(int groups) { return (3 * static_cast<size_t>(groups) + 1) * sizeof(int); }
 
-// One persistent CTA (or CTA pair) per SM (pair); `fixed` bytes of shared memory besides the groups' tables.
-template <auto kKernel, int kCtas, typename Params>
-int launch_ragged(const Params& p, int threads, size_t fixed, int sms, cudaStream_t stream) {
+// Persistent CTAs, one per SM, in clusters of `cluster`; `fixed` bytes of shared memory besides the groups' tables.
+template <auto kKernel, typename Params>
+int launch_ragged(const Params& p, int threads, size_t fixed, int cluster, int ctas, cudaStream_t stream) {
   const int rc = allow_shared_memory<kKernel>(fixed + ragged_tables(kRaggedMaxGroups) + 1024);
   if (rc != COMFY_MOE_OK) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(sms / kCtas * kCtas));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = fixed + ragged_tables(p.groups) + 1024;      // (1024: the stages start on a multiple of it)
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kCtas;
+  attr.val.clusterDim.x = cluster;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;

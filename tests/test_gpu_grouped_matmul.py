@@ -361,3 +361,38 @@ def test_few_rows(cuda_device, counts, gap, k, n, dtype):
     for (lo, _), c in zip(ranges, counts):
         assert torch.equal(half[lo:lo + c // 2], y[lo:lo + c // 2]) and (half[lo + c // 2:lo + c] == 0).all()
     assert torch.equal(M.grouped_matmul(x, w, offsets), y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("counts,k,n", [
+    ([17], 4096, 136), ([0, 40, 100], 2056, 264), ([300, 0, 129], 1096, 1000),      # along k: the result
+    ([17], 136, 4096), ([129, 0, 3, 40], 264, 1544),                                          # along n: the gradient of x
+    ([4003], 520, 264), ([1500, 0, 1700], 264, 136), ([3000, 100, 0, 1], 72, 520), ([515, 509], 1000, 1032),   # the rows
+], ids=str)
+def test_few_tiles_and_a_long_contraction(cuda_device, counts, k, n, dtype):
+    check_all(cuda_device, counts, k, n, dtype)
+
+
+def test_few_tiles_run_alike_and_replay(cuda_device):
+    from comfyui_b200 import moe_ops as M
+
+    x, w, dy, offsets = make(cuda_device, [2000, 0, 1203], 4096, 136, torch.bfloat16)
+    first = [M.grouped_matmul_dgrad(dy, w, offsets), M.grouped_matmul_wgrad(dy, x, offsets)]
+    y = M.grouped_matmul(x[:90].contiguous(), w, offsets.clamp(max=90))
+    stream = torch.cuda.Stream()
+    small = x[:90].contiguous()
+    few = offsets.clamp(max=90)
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        M.grouped_matmul(small, w, few)
+    with torch.cuda.graph(graph, stream=stream):
+        out = M.grouped_matmul(small, w, few)
+        dw = M.grouped_matmul_wgrad(dy, x, offsets)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, y) and torch.equal(dw, first[1])
+    assert torch.equal(M.grouped_matmul_dgrad(dy, w, offsets), first[0])
+    M.check_all_status()
