@@ -47,6 +47,17 @@ template <int kCtas> struct FpShape {
   static_assert(kStages > kFpAcc, "a stage's barriers are never a whole turn ahead of an epilogue warp");
 };
 
+__device__ __forceinline__ void unpack_8(const uint4& raw, bool fp16, float (&f)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 v = fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                          : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+    f[2 * j] = v.x;
+    f[2 * j + 1] = v.y;
+  }
+}
+
 struct alignas(64) BlockParams {
   CUtensorMap map_a, map_b, map_out;
   const int32_t* offsets;
@@ -61,35 +72,41 @@ struct alignas(64) BlockParams {
   long long ws_group;                            // scales per group
   int ws_n, ws_k;                                // strides over column blocks and contraction blocks
   int groups, rows, n_total, k_total, band, zero_unused, fp16;
+  int split;                                     // CTAs that share a tile's contraction (kSplit)
   uint32_t idesc;
 };
 
-template <bool kTransposed, int kCtas>
+template <bool kTransposed, int kCtas, bool kSplit>
 __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __grid_constant__ BlockParams p) {
   using Shape = FpShape<kCtas>;
   constexpr bool kPair = kCtas == 2;
+  static_assert(!kPair || !kSplit, "a contraction is split among single CTAs");
   constexpr int kStages = Shape::kStages, kStageBytes = Shape::kStageBytes, kTileRows = Shape::kTileRows;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
-  __shared__ __align__(8) uint64_t scale_full_bar[kScaleSlots], scale_empty_bar[kScaleSlots], drain_bar;
+  __shared__ __align__(8) uint64_t scale_full_bar[kScaleSlots], scale_empty_bar[kScaleSlots], drain_bar, parts_bar;
   __shared__ int4 tile_ring[kScaleSlots];          // of the slot's tile: first row and column, rows and first row of its group
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;      // 0 = leader of the pair
-  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
+  const int split = kSplit ? p.split : 1, part = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / (kCtas * split), units = gridDim.x / (kCtas * split);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
   int* s_count = s_begin + p.groups;
   int* s_first = s_count + p.groups;
   const int n_tiles = (p.n_total + kFpTile - 1) / kFpTile;
-  const int steps = (p.k_total + kBlk - 1) / kBlk;      // blocks of the contraction
+  const int blocks = (p.k_total + kBlk - 1) / kBlk, turns = (blocks + kFpUnit - 1) / kFpUnit;
+  const int first = kSplit ? turns * part / split * kFpUnit : 0;      // blocks first .. steps - 1 are this CTA's
+  const int steps = kSplit ? min(turns * (part + 1) / split * kFpUnit, blocks) : blocks;
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1 + kRaggedEpilogueWarps * kCtas); mbar_init(&empty_bar[s], 1); }
       for (int s = 0; s < kScaleSlots; ++s) { mbar_init(&scale_full_bar[s], kScaleWarps); mbar_init(&scale_empty_bar[s], kRaggedEpilogueWarps); }
       mbar_init(&drain_bar, 1);
+      mbar_init(&parts_bar, kRaggedEpilogueWarps * split);
       fence_mbar_init();
       abort_flag = 0;
     }
@@ -101,12 +118,12 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
   }
   __syncwarp();
   tc_fence_before_sync();
-  if constexpr (kPair) cluster_sync_all();     // the peer's barriers must exist before anything signals them
+  if constexpr (kPair || kSplit) cluster_sync_all();     // the peers' barriers must exist before anything signals them
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort_ptr = &abort_flag;
-  const int total = s_first[p.groups];
+  const int total = kSplit ? min(s_first[p.groups], unit + 1) : s_first[p.groups];      // (clusters: one tile each)
   auto give_up = [&](int code) {
     if (lane == 0) { atomicCAS(p.status, 0, code); abort_flag = 1; }
   };
@@ -136,7 +153,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
       bool ok = true;
       for (int t = unit, g = 0; t < total && ok; t += units) {
         const Tile c = tile_at(t, g);
-        for (int kb = 0; kb < steps; kb += kFpUnit) {
+        for (int kb = first; kb < steps; kb += kFpUnit) {
           ok = mbar_wait_warp(&empty_bar[s], phase, abort_ptr);
           if (!ok) { give_up(kStatusRaggedProducer); break; }
           uint8_t* a = smem + s * kStageBytes;
@@ -167,7 +184,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
                                            : umma_desc_k_sw128(b_addr);
       bool ok = true;
       for (int t = unit; t < total && ok && rank == 0; t += units) {
-        for (int kb = 0; kb < steps; kb += kFpUnit) {
+        for (int kb = first; kb < steps; kb += kFpUnit) {
           ok = mbar_wait_warp(&full_bar[s], phase, abort_ptr);
           if (!ok) { give_up(kStatusRaggedMma); break; }
           tc_fence_after_sync();
@@ -210,7 +227,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
       for (int t = unit, g = 0; t < total && ok; t += units) {
         const Tile c = tile_at(t, g);
         const float* ws = p.ws + g * p.ws_group + static_cast<long long>(c.n0 / kBlk) * p.ws_n;
-        for (int kb = 0; kb < steps; kb += kScaleSteps, ++slot) {
+        for (int kb = first; kb < steps; kb += kScaleSteps, ++slot) {
           const int q = slot % kScaleSlots;
           ok = mbar_wait_warp(&scale_empty_bar[q], ((slot / kScaleSlots) & 1u) ^ 1u, abort_ptr);
           if (!ok) { give_up(kStatusRaggedEpilogue); break; }
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0.f;
       int4 tile = make_int4(0, 0, 0, 0);
-      for (int kb = 0; kb < steps && ok; kb += kScaleSteps) {
+      for (int kb = first; kb < steps && ok; kb += kScaleSteps) {
         ok = mbar_wait_warp(&scale_full_bar[slot], slot_phase, abort_ptr);
         if (!ok) { give_up(kStatusRaggedEpilogue); break; }
         const float* scales = scale_ring + slot * kScaleSteps * kFpTile + quarter * 32 + lane;
@@ -297,6 +314,25 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
         slot_phase ^= slot == 0;
       }
       if (!ok) break;
+      if constexpr (kSplit) {
+        ok = join_parts(
+            smem, &parts_bar, warp - kFpFirst, quarter, half, split, part, abort_ptr,
+            [&](int j) { return make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]); },
+            [&](int row, int col, float4 a, float4 b) {
+              row += tile.x;
+              col += tile.y;
+              if (row >= tile.z || col >= p.n_total) return;
+              if (p.bias != nullptr) {
+                float f[8];
+                unpack_8(__ldg(reinterpret_cast<const uint4*>(p.bias) + col / 8), p.fp16, f);
+                a.x += f[0]; a.y += f[1]; a.z += f[2]; a.w += f[3];
+                b.x += f[4]; b.y += f[5]; b.z += f[6]; b.w += f[7];
+              }
+              *reinterpret_cast<uint4*>(p.out + (tile.w + row) * p.ld_out + 2 * col) = pack_8(a, b, p.fp16);
+            });
+        if (!ok) { give_up(kStatusRaggedEpilogue); break; }
+        continue;
+      }
       const int row0 = tile.x + rank * kFpTile + quarter * 32, rows_here = tile.z - row0;
       if (rows_here <= 0) continue;
       const int col0 = tile.y + half * 64;
@@ -304,15 +340,10 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           if (col0 + q * 8 >= p.n_total) break;
-          const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.bias) + col0 / 8 + q);
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+          float f[8];
+          unpack_8(__ldg(reinterpret_cast<const uint4*>(p.bias) + col0 / 8 + q), p.fp16, f);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
-                                    : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-            sum[q * 8 + 2 * j] += f.x;
-            sum[q * 8 + 2 * j + 1] += f.y;
-          }
+          for (int j = 0; j < 8; ++j) sum[q * 8 + j] += f[j];
         }
       }
       uint32_t packed[32];
@@ -368,7 +399,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
     while (clock64() - t0 < 2000000LL) __nanosleep(1000);     // copies in flight may still land in shared memory
   }
   tc_fence_before_sync();
-  if constexpr (kPair) cluster_sync_all();      // neither CTA leaves while the other may still signal it or use its TMEM
+  if constexpr (kPair || kSplit) cluster_sync_all();      // no CTA leaves while another may still signal it or read from it
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
@@ -377,17 +408,28 @@ __global__ void __launch_bounds__(kFpThreads, 1) block_matmul_kernel(const __gri
   }
 }
 
-template <bool kTransposed, int kCtas>
-static int launch_block(const BlockParams& p, int sms, cudaStream_t stream) {
+template <bool kTransposed, int kCtas, bool kSplit>
+static int launch_block(const BlockParams& p, int cluster, int ctas, cudaStream_t stream) {
   // the warpgroups' register shares have to be there at launch, or the larger ones would wait for good
   static const int regs = [] {
     cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, block_matmul_kernel<kTransposed, kCtas>) == cudaSuccess ? a.numRegs : 0;
+    return cudaFuncGetAttributes(&a, block_matmul_kernel<kTransposed, kCtas, kSplit>) == cudaSuccess ? a.numRegs : 0;
   }();
   if (regs < kFpLaunchRegs) return COMFY_MOE_EUNSUPPORTED;
-  return launch_ragged<block_matmul_kernel<kTransposed, kCtas>>(p, kFpThreads, FpShape<kCtas>::kTables, kCtas,
-                                                                sms / kCtas * kCtas, stream);
+  return launch_ragged<block_matmul_kernel<kTransposed, kCtas, kSplit>>(p, kFpThreads, FpShape<kCtas>::kTables, cluster, ctas,
+                                                                        stream);
 }
+
+template <bool kTransposed>
+static int launch_block_plan(const BlockParams& p, int ctas, int tiles, int sms, cudaStream_t stream) {
+  if (p.split > 1) return launch_block<kTransposed, 1, true>(p, p.split, tiles * p.split, stream);
+  return ctas == 2 ? launch_block<kTransposed, 2, false>(p, 2, sms / 2 * 2, stream)
+                   : launch_block<kTransposed, 1, false>(p, 1, sms, stream);
+}
+
+// Blocks from which on the contraction of few tiles is shared by clusters (pick_split).  Measured (us, whole / shared): 100
+// rows, 8192 -> 256: 22.8 / 12.9; 64 rows, 6912 -> 2560: 20.6 / 14.2; with 20 blocks, 2560 -> 2560: 12.7 / 12.0.
+constexpr int kSplitBlocks = 20;
 
 static int64_t scale_offset(int64_t rows, int64_t cols) { return (rows * cols + 255) / 256 * 256; }
 
@@ -424,7 +466,6 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   }
   if (!w || !w_scale || !aligned16(w) || ld_w < k || ld_w % 16 || (n_groups > 1 && (w_group_stride <= 0 || w_group_stride % 16)))
     return COMFY_MOE_EINVAL;
-  const int ctas = rows >= 128 * (n_groups < rows ? n_groups : rows) ? 2 : 1;     // pairs where groups have the rows for them
   const int sms = sm100_count();
   if (sms < 0) return -sms;
   const int nb = (n + kBlk - 1) / kBlk, kb = (k + kBlk - 1) / kBlk;
@@ -446,6 +487,11 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
     f.groups = n_groups; f.rows = rows; f.n = n; f.k = k; f.zero_unused = zero_unused;
     return launch_few_rows_block(f, dtype == COMFY_MOE_FP16, s);
   }
+  const int64_t tiles = most_row_tiles(rows, n_groups, kFpTile) * ((cols + kFpTile - 1) / kFpTile);
+  const int split = pick_split<block_matmul_kernel<false, 1, true>>(tiles, (in + kBlk - 1) / kBlk, kSplitBlocks, kFpThreads,
+                                                                    FpShape<1>::kTables);
+  // pairs where groups have the rows for them
+  const int ctas = split == 1 && rows >= 128 * (n_groups < rows ? n_groups : rows) ? 2 : 1;
   BlockParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -468,6 +514,7 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   const int64_t band = (32ll << 20) / (static_cast<int64_t>(kFpTile * ctas) * in);   // 32 MB of rows stay in L2
   p.band = static_cast<int>(band < 8 ? 8 : (band > 64 ? 64 : band));
   p.idesc = umma_idesc<true>(kFpTile * ctas, kFpTile) | (transpose_w ? 1u << 16 : 0u);
-  if (ctas == 2) return transpose_w ? launch_block<true, 2>(p, sms, s) : launch_block<false, 2>(p, sms, s);
-  return transpose_w ? launch_block<true, 1>(p, sms, s) : launch_block<false, 1>(p, sms, s);
+  p.split = split;
+  return transpose_w ? launch_block_plan<true>(p, ctas, static_cast<int>(tiles), sms, s)
+                     : launch_block_plan<false>(p, ctas, static_cast<int>(tiles), sms, s);
 }

@@ -22,8 +22,6 @@
 // the leader's `peer` barrier.  (An arrival of the other CTA at every step, so that one barrier would do, halved the rate:
 // 762 us against 412 with single CTAs at 16384 rows, 8 groups, 2048 x 8192.  Zeros by the MMA warp itself held up every
 // tile of a short group: 111 us against 108 at 2048 rows.)
-#include <type_traits>
-
 #include "few_rows.cuh"
 #include "ragged.cuh"
 
@@ -37,16 +35,8 @@ constexpr int kABytes = kTileM * 128;
 constexpr int kMnBoxBytes = kStepK * 128;      // one box of an MN-major operand: 64 steps x 64 elements
 
 constexpr int kStageBytes = 2 * kABytes;        // 128 rows of A, 128 columns of B
-constexpr int kPartBytes = 128 * 128 * 4;      // one CTA's sums of a tile (kSplit)
-
-template <int kCtas, bool kSplit> struct GmmShape {
-  static constexpr int kTile = kTileM * kCtas;   // rows and columns
-  static constexpr int kStages = kSplit ? 4 : 6;
-  static constexpr int kTmemCols = 2 * kTile;  // two accumulators: the epilogue of one tile overlaps the next one's MMAs
-  static constexpr int kParts = kStages * kStageBytes;
-  static constexpr int kStores = kParts + (kSplit ? kPartBytes : 0);
-  static constexpr int kTables = kStores + kRaggedEpilogueWarps * kStoreTileBytes;
-};
+constexpr int kStages = 6;
+constexpr int kGmmTables = kStages * kStageBytes + kRaggedEpilogueWarps * kStoreTileBytes;
 
 struct alignas(64) GmmParams {
   CUtensorMap map_a, map_b, map_out;
@@ -69,16 +59,15 @@ struct alignas(64) GmmParams {
 template <int kForm, int kCtas, bool kSplit>
 __global__ void __launch_bounds__(kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, 1)
 grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
-  using Shape = GmmShape<kCtas, kSplit>;
-  constexpr int kStages = Shape::kStages;
-  constexpr int kTile = Shape::kTile;
+  constexpr int kTile = kTileM * kCtas;          // rows and columns
+  constexpr int kTmemCols = 2 * kTile;           // two accumulators: the epilogue of one tile overlaps the next one's MMAs
   constexpr bool kPair = kCtas == 2;
   static_assert(!kPair || !kSplit, "a contraction is split among single CTAs");
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ __align__(8) uint64_t tmem_full_bar[2], tmem_empty_bar[2], drain_bar;
   __shared__ __align__(8) uint64_t tail_bar[kStages], peer_bar[kStages];
-  __shared__ __align__(8) uint64_t parts_full_bar, parts_empty_bar;
+  __shared__ __align__(8) uint64_t parts_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
@@ -87,7 +76,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   const int split = kSplit ? p.split : 1, part = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / (kCtas * split), units = gridDim.x / (kCtas * split);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* s_begin = reinterpret_cast<int*>(smem + Shape::kTables);
+  int* s_begin = reinterpret_cast<int*>(smem + kGmmTables);
   int* s_count = s_begin + p.groups;
   int* s_first = s_count + p.groups;
 
@@ -99,8 +88,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
       for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full_bar[s], 1); mbar_init(&tmem_empty_bar[s], kRaggedEpilogueWarps * kCtas); }
       mbar_init(&drain_bar, 1);
       for (int s = 0; s < kStages; ++s) { mbar_init(&tail_bar[s], 1); mbar_init(&peer_bar[s], 1); }
-      mbar_init(&parts_full_bar, kRaggedEpilogueWarps * split);
-      mbar_init(&parts_empty_bar, kRaggedEpilogueWarps * split);
+      mbar_init(&parts_bar, kRaggedEpilogueWarps * split);
       fence_mbar_init();
       abort_flag = 0;
     }
@@ -108,8 +96,8 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     ragged_ranges(p.offsets, p.counts, p.groups, p.rows, kForm == kGradW ? 0 : kTile,
                   kForm == kGradW ? m_tiles_w * n_tiles : n_tiles, s_begin, s_count, s_first);
   } else if (warp == 1) {
-    if constexpr (kPair) { tmem_alloc_pair(&tmem_slot, Shape::kTmemCols); tmem_relinquish_pair(); }
-    else { tmem_alloc(&tmem_slot, Shape::kTmemCols); tmem_relinquish(); }
+    if constexpr (kPair) { tmem_alloc_pair(&tmem_slot, kTmemCols); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_slot, kTmemCols); tmem_relinquish(); }
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -118,7 +106,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort_ptr = &abort_flag;
-  const int total = s_first[p.groups];
+  const int total = kSplit ? min(s_first[p.groups], unit + 1) : s_first[p.groups];      // (clusters: one tile each)
   auto give_up = [&](int code) {
     if (lane == 0) { atomicCAS(p.status, 0, code); abort_flag = 1; }
   };
@@ -262,7 +250,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint8_t* store = smem + Shape::kStores + (warp - 2) * kStoreTileBytes;
+    uint8_t* store = smem + kStages * kStageBytes + (warp - 2) * kStoreTileBytes;
     // 32 rows from row0 on (inside the group; d W: inside dw[g]) of 32 columns of the output: lane l has row l
     auto emit = [&](const Tile& c, int g, int row0, int col, const uint32_t (&v)[32]) {
       const int rows_here = (kForm == kGradW ? p.m_total : c.count) - row0;
@@ -311,7 +299,7 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
       }
     };
     constexpr int kChunks = kTile / 64;             // chunks of 32 columns of this warp's half
-    uint32_t acc = 0, parts_phase = 0;
+    uint32_t acc = 0;
     for (int t = unit, g = 0; t < total; t += units) {
       const Tile c = tile_at(t, g);
       uint32_t r[kChunks][32];
@@ -337,62 +325,25 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
         }
       }
       if constexpr (kSplit) {
-        // Every CTA lays out its sums, four columns of one row after another: [row / 32][column / 4][row % 32][4].  Then each
-        // of the 8 x split warps adds up 64 / split columns of 32 rows in the order of the parts, and stores them.
-        const int w = warp - 2;
-        uint8_t* mine = smem + Shape::kParts + lane * 16;
-        if (!mbar_wait_warp(&parts_empty_bar, parts_phase ^ 1u, abort_ptr)) { give_up(kStatusRaggedEpilogue); break; }
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(mine + ((quarter * 32 + half * 16 + i * 8 + j) << 9)) =
-                make_uint4(r[i][4 * j], r[i][4 * j + 1], r[i][4 * j + 2], r[i][4 * j + 3]);
-        __syncwarp();
-        if (lane < split) mbar_arrive_cluster(mapa_shared(smem_u32(&parts_full_bar), lane));
-        if (!mbar_wait_warp(&parts_full_bar, parts_phase, abort_ptr)) { give_up(kStatusRaggedEpilogue); break; }
-        asm volatile("fence.acq_rel.cluster;" ::: "memory");
-        parts_phase ^= 1u;
-        const int share = (w * split + part) * 16 / split;       // first of its 16 / split quadruples
-        const int row0 = c.m0 + (share >> 5) * 32, col = c.n0 + (share & 31) * 4;
-        auto finish = [&](auto parts) {
-          constexpr int kFrom = decltype(parts)::value, kQuads = 16 / kFrom;
-          float4 v[kFrom][kQuads];
-#pragma unroll
-          for (int from = 0; from < kFrom; ++from) {
-            const uint32_t at = mapa_shared(smem_u32(mine + (share << 9)), from);
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j) v[from][j] = ld_cluster_f4(at + (j << 9));
-          }
-#pragma unroll
-          for (int from = 1; from < kFrom; ++from)
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j) {
-              v[0][j].x += v[from][j].x; v[0][j].y += v[from][j].y; v[0][j].z += v[from][j].z; v[0][j].w += v[from][j].w;
-            }
-          if (row0 + lane >= (kForm == kGradW ? p.m_total : c.count)) return;
-          uint8_t* row = p.out + (kForm == kGradW ? g * p.out_group + static_cast<long long>(row0 + lane) * p.ld_out
-                                                  : static_cast<long long>(c.begin + row0 + lane) * p.ld_out);
-#pragma unroll
-          for (int j = 0; j < kQuads; j += 2) {
-            if (col + 4 * j >= p.n_total) break;
-            if (kForm == kGradW && p.out_fp32) {
-              float4* to = reinterpret_cast<float4*>(row + 4 * (col + 4 * j));
-              to[0] = v[0][j];
-              to[1] = v[0][j + 1];
-            } else {
-              const float4 a = v[0][j], b = v[0][j + 1];
-              *reinterpret_cast<uint4*>(row + 2 * (col + 4 * j)) =
-                  p.fp16 ? make_uint4(pack_f16x2(a.x, a.y), pack_f16x2(a.z, a.w), pack_f16x2(b.x, b.y), pack_f16x2(b.z, b.w))
-                         : make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
-            }
-          }
-        };
-        if (split == 8) finish(std::integral_constant<int, 8>{});
-        else if (split == 4) finish(std::integral_constant<int, 4>{});
-        else finish(std::integral_constant<int, 2>{});
-        __syncwarp();
-        if (lane < split) mbar_arrive_cluster(mapa_shared(smem_u32(&parts_empty_bar), lane));
+        const bool ok = join_parts(
+            smem, &parts_bar, warp - 2, quarter, half, split, part, abort_ptr,
+            [&](int j) {
+              const uint32_t* q = &r[j >> 3][(j & 7) * 4];
+              return make_float4(__uint_as_float(q[0]), __uint_as_float(q[1]), __uint_as_float(q[2]), __uint_as_float(q[3]));
+            },
+            [&](int row, int col, float4 a, float4 b) {
+              row += c.m0;
+              col += c.n0;
+              if (row >= (kForm == kGradW ? p.m_total : c.count) || col >= p.n_total) return;
+              uint8_t* to = p.out + (kForm == kGradW ? g * p.out_group + row * p.ld_out : (c.begin + row) * p.ld_out);
+              if (kForm == kGradW && p.out_fp32) {
+                reinterpret_cast<float4*>(to + 4 * col)[0] = a;
+                reinterpret_cast<float4*>(to + 4 * col)[1] = b;
+              } else {
+                *reinterpret_cast<uint4*>(to + 2 * col) = pack_8(a, b, p.fp16);
+              }
+            });
+        if (!ok) { give_up(kStatusRaggedEpilogue); break; }
       } else {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
@@ -416,8 +367,8 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    if constexpr (kPair) tmem_dealloc_pair(tmem_base, Shape::kTmemCols);
-    else tmem_dealloc(tmem_base, Shape::kTmemCols);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, kTmemCols);
+    else tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
@@ -426,52 +377,17 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
 // dw, whose contraction is the group's rows, 100 / 173 (4096 rows), 112 / 120 (256), 92 / 80 (64).  Tiles of 64 columns, and
 // pairs with 128, were never the fastest.
 //
-// Where even the 128 x 128 tiles leave half of the SMs without one and the contraction is long, clusters of 2, 4 or 8 CTAs
-// share each tile's contraction and add their sums up through shared memory, in the order of the parts.  The exchange takes
-// 3 us, a step of 64 0.3 us, so it is worth it from 24 steps on.  Measured (us, whole / shared): y at 100 rows, 2 groups,
-// 8192 -> 256: 37.9 / 13.7; 2048 -> 512: 13.5 / 10.8; 1024 -> 256: 9.4 / 9.8; 4 groups, 4096 -> 2048, 64 rows: 23.6 / 18.0;
-// dw 512 x 512 of 8000 rows: 41.7 / 18.3.  All clusters have to be on the device at once (of 8 CTAs it holds 15): a
-// second wave takes as long as the first, 24 instead of 14 us for 16 tiles of 64 steps.
-constexpr int kSplitSteps = 24, kSplitMin = 4;
+//
+// Few tiles with a long contraction are shared by clusters (pick_split).  Measured (us, whole / shared): y at 100 rows,
+// 2 groups, 8192 -> 256: 37.6 / 13.5; 2048 -> 512: 13.4 / 10.4; with 16 steps, 1024 -> 256: 9.4 / 9.8; 4 groups,
+// 4096 -> 2048, 64 rows: 23.0 / 17.9; dw 512 x 512 of 8000 rows: 41.9 / 18.0.
 struct GmmPlan { int ctas, split, tiles; };
 
-// Clusters of `size` CTAs of the splitting kernel that the current device holds at once.
-static int resident_clusters(int size) {
-  static thread_local int known = -1, held[9];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (dev != known) {
-    constexpr size_t kBytes = GmmShape<1, true>::kTables + ragged_tables(kRaggedMaxGroups) + 1024;
-    const auto kernel = grouped_matmul_kernel<kGradW, 1, true>;
-    if (allow_shared_memory<grouped_matmul_kernel<kGradW, 1, true>>(kBytes) != COMFY_MOE_OK) return 0;
-    for (int s = 2; s <= 8; s *= 2) {
-      cudaLaunchConfig_t cfg;
-      memset(&cfg, 0, sizeof(cfg));
-      cfg.gridDim = dim3(s);
-      cfg.blockDim = dim3(kRaggedTailThreads);
-      cfg.dynamicSmemBytes = kBytes;
-      cudaLaunchAttribute attr;
-      attr.id = cudaLaunchAttributeClusterDimension;
-      attr.val.clusterDim.x = s;
-      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&held[s], kernel, &cfg) != cudaSuccess) { cudaGetLastError(); held[s] = 0; }
-    }
-    known = dev;
-  }
-  return held[size];
-}
-
-static GmmPlan plan_gmm(int64_t rows, int64_t groups, int64_t pair_from, int64_t tiles, int64_t steps, int sms) {
+static GmmPlan plan_gmm(int64_t rows, int64_t groups, int64_t pair_from, int64_t tiles, int64_t steps) {
   const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
-  GmmPlan plan = {rows >= pair_from * busy ? 2 : 1, 1, 0};
-  for (int s = 8; s > 1; s /= 2)
-    if (steps >= kSplitSteps && steps >= kSplitMin * s && tiles * s <= sms && tiles <= resident_clusters(s)) {
-      plan.ctas = 1; plan.split = s; plan.tiles = static_cast<int>(tiles);
-      break;
-    }
-  return plan;
+  const int split = pick_split<grouped_matmul_kernel<kGradW, 1, true>>(tiles, steps, 24, kRaggedTailThreads, kGmmTables);
+  if (split > 1) return {1, split, static_cast<int>(tiles)};
+  return {rows >= pair_from * busy ? 2 : 1, 1, 0};
 }
 
 static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
@@ -479,7 +395,7 @@ static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
 template <int kForm, int kCtas, bool kSplit>
 static int launch_gmm(const GmmParams& p, int cluster, int ctas, cudaStream_t stream) {
   return launch_ragged<grouped_matmul_kernel<kForm, kCtas, kSplit>>(
-      p, kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, GmmShape<kCtas, kSplit>::kTables, cluster, ctas, stream);
+      p, kForm == kGradW ? kRaggedTailThreads : kRaggedThreads, kGmmTables, cluster, ctas, stream);
 }
 
 template <int kForm>
@@ -541,9 +457,7 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  // (no more row tiles than these, however the rows are dealt)
-  const int64_t tiles = (rows / kTileM + (groups < rows ? groups : rows)) * up_to(cols, kTileM);
-  const GmmPlan plan = plan_gmm(rows, groups, 128, tiles, up_to(in, kStepK), sms);
+  const GmmPlan plan = plan_gmm(rows, groups, 128, most_row_tiles(rows, groups, kTileM) * up_to(cols, kTileM), up_to(in, kStepK));
   const int ctas = plan.ctas;
   if ((rc = ragged_map(&p.map_a, t, 2, a, in, rows, 0, ld_a, 0, 64, kTileM)) != COMFY_MOE_OK) return rc;
   if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? kTileM : kStepK)) != COMFY_MOE_OK)
@@ -598,7 +512,7 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int64_t tiles = n_groups * up_to(n, kTileM) * up_to(k, kTileM);
-  const GmmPlan plan = plan_gmm(rows, n_groups, 192, tiles, rows / n_groups / kStepK, sms);
+  const GmmPlan plan = plan_gmm(rows, n_groups, 192, tiles, rows / n_groups / kStepK);
   if (rows > 0) {
     if ((rc = ragged_map(&p.map_a, t, 2, dy, n, rows, 0, ld_dy, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
     if ((rc = ragged_map(&p.map_b, t, 2, x, k, rows, 0, ld_x, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;

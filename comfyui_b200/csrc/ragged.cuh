@@ -1,6 +1,7 @@
 // What the products over ragged groups of rows share: the rows of each group, the order of the tiles, tensor maps.
 #pragma once
 #include <cstring>
+#include <type_traits>
 #include <cuda.h>
 
 #include "moe_common.cuh"
@@ -102,6 +103,47 @@ __device__ __forceinline__ uint32_t store_piece(int row, int piece) {
   return row * kStoreRowBytes + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 
+// The sums of a 128 x 128 tile whose contraction the `split` CTAs of a cluster have shared.  A warp of each CTA's eight holds
+// rows quarter * 32 + lane and 16 quadruples of columns, quad(j) = columns half * 64 + 4 j .. + 3.  Every CTA lays its sums
+// out as [row / 32][column / 4][row % 32][4]; then each of the cluster's warps adds up 64 / split columns of 32 rows, in the
+// order of the parts, and hands over eight columns at a time: store(row, column, four, four).  One call per launch: `parts`
+// (64 KB) may be what the operands stood in, and `bar` (8 x split arrivals) completes once.
+template <typename Quad, typename Store>
+__device__ __forceinline__ bool join_parts(uint8_t* parts, uint64_t* bar, int warp, int quarter, int half, int split,
+                                           int part, volatile int* abort_ptr, Quad quad, Store store) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* mine = parts + lane * 16;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(mine + ((quarter * 32 + half * 16 + j) << 9)) = quad(j);
+  __syncwarp();
+  if (lane < split) mbar_arrive_cluster(mapa_shared(smem_u32(bar), lane));
+  if (!mbar_wait_warp(bar, 0, abort_ptr)) return false;
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  const int share = warp * 16 + part * 16 / split;         // the first of 16 / split quadruples
+  auto finish = [&](auto parts_of) {
+    constexpr int kFrom = decltype(parts_of)::value, kQuads = 16 / kFrom;
+    float4 v[kFrom][kQuads];
+#pragma unroll
+    for (int from = 0; from < kFrom; ++from) {
+      const uint32_t at = mapa_shared(smem_u32(mine + (share << 9)), from);
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) v[from][j] = ld_cluster_f4(at + (j << 9));
+    }
+#pragma unroll
+    for (int from = 1; from < kFrom; ++from)
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) {
+        v[0][j].x += v[from][j].x; v[0][j].y += v[from][j].y; v[0][j].z += v[from][j].z; v[0][j].w += v[from][j].w;
+      }
+#pragma unroll
+    for (int j = 0; j < kQuads; j += 2) store((share >> 5) * 32 + lane, (share & 31) * 4 + 4 * j, v[0][j], v[0][j + 1]);
+  };
+  if (split == 8) finish(std::integral_constant<int, 8>{});
+  else if (split == 4) finish(std::integral_constant<int, 4>{});
+  else finish(std::integral_constant<int, 2>{});
+  return true;
+}
+
 // Zeros in the rows that belong to no group, dealt to all epilogue warps of the grid.
 __device__ __forceinline__ void zero_rows_between(const int* begin, const int* count, int groups, int rows, uint8_t* out,
                                                   long long ld_bytes, int row_bytes, int worker, int workers) {
@@ -200,6 +242,50 @@ int launch_ragged(const Params& p, int threads, size_t fixed, int cluster, int c
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kKernel, p) == cudaSuccess ? check_launch() : COMFY_MOE_ECUDA;
+}
+
+// Clusters of `size` CTAs of a kernel that the current device holds at once.
+template <auto kKernel>
+int resident_clusters(int size, int threads, size_t fixed) {
+  static thread_local int known = -1, held[9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev != known) {
+    const size_t bytes = fixed + ragged_tables(kRaggedMaxGroups) + 1024;
+    if (allow_shared_memory<kKernel>(bytes) != COMFY_MOE_OK) return 0;
+    for (int s = 2; s <= 8; s *= 2) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cfg.gridDim = dim3(s);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = bytes;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = s;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&held[s], kKernel, &cfg) != cudaSuccess) { cudaGetLastError(); held[s] = 0; }
+    }
+    known = dev;
+  }
+  return held[size];
+}
+
+// How many CTAs of a cluster share the contraction of each of (at most) `tiles` 128 x 128 tiles; 1: none.  The exchange takes
+// 3 us, so a contraction of fewer than `worth` steps is not shared, and no CTA takes fewer than 4.  All clusters have to be
+// on the device at once (of 8 CTAs it holds 15): a second wave takes as long as the first.
+template <auto kKernel>
+int pick_split(int64_t tiles, int64_t steps, int64_t worth, int threads, size_t fixed) {
+  if (steps >= worth)
+    for (int s = 8; s > 1; s /= 2)
+      if (steps >= 4 * s && tiles <= resident_clusters<kKernel>(s, threads, fixed)) return s;
+  return 1;
+}
+
+// No more row tiles than these, however the rows are dealt to the groups.
+inline int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t tile) {
+  return rows / tile + (groups < rows ? groups : rows);
 }
 
 }  // namespace comfy_b200

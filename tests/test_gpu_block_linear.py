@@ -446,3 +446,31 @@ def test_registered_operators(cuda_device):
     got = torch.autograd.grad(ops.grouped_matmul(x, w, off).sum(), (x, w))
     want = torch.autograd.grad(M.grouped_matmul(x, w, off).sum(), (x, w))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("counts", [[17], [130], [0, 40, 100], [128, 1, 0, 60]], ids=str)
+@pytest.mark.parametrize("n,k", [(144, 2688), (272, 4112), (16, 8192), (2064, 4112)])
+def test_few_tiles_and_a_long_contraction(cuda_device, counts, n, k, dtype):
+    from comfyui_b200 import moe_ops as M
+
+    dev = cuda_device
+    gen = torch.Generator(device=dev).manual_seed(n + k)
+    rows, g = sum(counts) + 5, len(counts)
+    x = torch.randn((rows, k), generator=gen, device=dev).to(dtype)
+    w, ws = M.quantize_weight_blocks_e4m3(0.05 * torch.randn((g, n, k), generator=gen, device=dev))
+    ws *= torch.rand(ws.shape, generator=gen, device=dev) + 0.5
+    wt, wts = w.transpose(1, 2).contiguous(), ws.transpose(1, 2).contiguous()
+    ends = [5 + sum(counts[:i]) for i in range(g + 1)]
+    offsets = torch.tensor(ends, dtype=torch.int32, device=dev)
+    bias = torch.randn((n,), generator=gen, device=dev).to(dtype)
+    y, dx = M.grouped_block_linear(x, w, ws, offsets), M.grouped_block_linear_dgrad(x, wt, wts, offsets)
+    for i, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        want = product(x[lo:hi], w[i], ws[i], None, dtype)
+        close(y[lo:hi], *want, k, f"y of group {i}")
+        close(dx[lo:hi], *want, k, f"dx of group {i}")
+    assert (y[:5] == 0).all() and (dx[:5] == 0).all()
+    close(M.block_linear(x, w[0], ws[0], bias), *product(x, w[0], ws[0], bias, dtype), k, "with a bias")
+    again = [M.grouped_block_linear(x, w, ws, offsets) for _ in range(3)]
+    assert all(torch.equal(a, y) for a in again)
+    M.check_all_status()
