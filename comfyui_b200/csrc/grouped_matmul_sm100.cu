@@ -372,25 +372,36 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
   }
 }
 
-// SM pairs with 256 x 256 tiles where the groups have the rows for them, 128 x 128 tiles of single CTAs below.  Measured (us,
-// pair / single): forward at 512 rows a group 76 / 98, 256: 56 / 58, 64: 42 / 39; dx 119 / 169 (4096 rows), 50 / 44 (64);
-// dw, whose contraction is the group's rows, 100 / 173 (4096 rows), 112 / 120 (256), 92 / 80 (64).  Tiles of 64 columns, and
-// pairs with 128, were never the fastest.
-//
-//
+// 256 x 256 tiles of SM pairs or 128 x 128 tiles of single CTAs.  A step of either takes the same time (the single CTA's is
+// bound by shared memory: 32 KB written and 64 KB read for 128 x 128 x 64 products), so what counts for y and d x is how
+// many rounds of tiles the SMs go through; as many of either: single CTAs, whose prologue and last tile are shorter.
+// Measured (us, pair / single): 4 groups, 2560 -> 6912: 100 rows each, 2 rounds of either, 37.0 / 34.7; 150, 2 and 3:
+// 37.9 / 43.5; 500, 4 and 7: 64.3 / 91.4; 6912 -> 2560: 150, 1 and 1: 43.1 / 39.2; 200, 1 and 2: 43.3 / 67.5; 8 groups,
+// 2048 -> 2048, 100 rows, 1 and 2: 19.0 / 26.1.  d W, whose contraction is the rows, writes more than it multiplies below
+// 256 rows a group: at 200 57.1 / 51.9, 28.9 / 25.7; 300 63.6 / 65.8, 34.4 / 36.3; 900 110.7 / 148.3.  Tiles of 64 columns,
+// and pairs with 128, were never the fastest.
+static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
+
+static bool pairs_take_fewer_rounds(int64_t rows, int64_t groups, int64_t cols, int sms) {
+  const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
+  auto rounds = [&](int64_t tile) {
+    const int64_t some = rows / tile + busy / 2;               // a group's last tile is half full, more or less
+    const int64_t row_tiles = groups == 1 ? up_to(rows, tile) : (some > busy ? some : busy);
+    return up_to(row_tiles * up_to(cols, tile) * (tile / kTileM), sms);
+  };
+  return rounds(2 * kTileM) < rounds(kTileM);
+}
+
 // Few tiles with a long contraction are shared by clusters (pick_split).  Measured (us, whole / shared): y at 100 rows,
 // 2 groups, 8192 -> 256: 37.6 / 13.5; 2048 -> 512: 13.4 / 10.4; with 16 steps, 1024 -> 256: 9.4 / 9.8; 4 groups,
 // 4096 -> 2048, 64 rows: 23.0 / 17.9; dw 512 x 512 of 8000 rows: 41.9 / 18.0.
 struct GmmPlan { int ctas, split, tiles; };
 
-static GmmPlan plan_gmm(int64_t rows, int64_t groups, int64_t pair_from, int64_t tiles, int64_t steps) {
-  const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
+static GmmPlan plan_gmm(bool pairs, int64_t tiles, int64_t steps) {
   const int split = pick_split<grouped_matmul_kernel<kGradW, 1, true>>(tiles, steps, 24, kRaggedTailThreads, kGmmTables);
   if (split > 1) return {1, split, static_cast<int>(tiles)};
-  return {rows >= pair_from * busy ? 2 : 1, 1, 0};
+  return {pairs ? 2 : 1, 1, 0};
 }
-
-static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
 
 template <int kForm, int kCtas, bool kSplit>
 static int launch_gmm(const GmmParams& p, int cluster, int ctas, cudaStream_t stream) {
@@ -457,7 +468,8 @@ static int rows_by_group(int form, const void* a, int64_t ld_a, const void* w, i
   GmmParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const GmmPlan plan = plan_gmm(rows, groups, 128, most_row_tiles(rows, groups, kTileM) * up_to(cols, kTileM), up_to(in, kStepK));
+  const GmmPlan plan = plan_gmm(pairs_take_fewer_rounds(rows, groups, cols, sms),
+                                most_row_tiles(rows, groups, kTileM) * up_to(cols, kTileM), up_to(in, kStepK));
   const int ctas = plan.ctas;
   if ((rc = ragged_map(&p.map_a, t, 2, a, in, rows, 0, ld_a, 0, 64, kTileM)) != COMFY_MOE_OK) return rc;
   if ((rc = ragged_map(&p.map_b, t, 2, w, k, n, groups, ld_w, w_group_stride, 64, form == kForward ? kTileM : kStepK)) != COMFY_MOE_OK)
@@ -512,7 +524,7 @@ extern "C" int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, con
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int64_t tiles = n_groups * up_to(n, kTileM) * up_to(k, kTileM);
-  const GmmPlan plan = plan_gmm(rows, n_groups, 192, tiles, rows / n_groups / kStepK);
+  const GmmPlan plan = plan_gmm(rows >= 256ll * n_groups, tiles, rows / n_groups / kStepK);
   if (rows > 0) {
     if ((rc = ragged_map(&p.map_a, t, 2, dy, n, rows, 0, ld_dy, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
     if ((rc = ragged_map(&p.map_b, t, 2, x, k, rows, 0, ld_x, 0, 64, kStepK)) != COMFY_MOE_OK) return rc;
