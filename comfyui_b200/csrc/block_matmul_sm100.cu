@@ -487,11 +487,15 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
     f.groups = n_groups; f.rows = rows; f.n = n; f.k = k; f.zero_unused = zero_unused;
     return launch_few_rows_block(f, dtype == COMFY_MOE_FP16, s);
   }
-  const int64_t tiles = most_row_tiles(rows, n_groups, kFpTile) * ((cols + kFpTile - 1) / kFpTile);
+  const int64_t col_tiles = up_to(cols, kFpTile), tiles = most_row_tiles(rows, n_groups, kFpTile) * col_tiles;
   const int split = pick_split<block_matmul_kernel<false, 1, true>>(tiles, (in + kBlk - 1) / kBlk, kSplitBlocks, kFpThreads,
                                                                     FpShape<1>::kTables);
-  // pairs where groups have the rows for them
-  const int ctas = split == 1 && rows >= 128 * (n_groups < rows ? n_groups : rows) ? 2 : 1;
+  // A step of a pair's 256 x 128 tile takes 6 % less than one of a single CTA's 128 x 128, but half-empty row tiles may add
+  // rounds (us, pair / single): one group, 2560 -> 6912: 1999 rows 47.8 / 50.6; 4 groups: 500 rows each, 8 and 7 rounds,
+  // 61.9 / 58.2; 1400, 18 and 17, 123.7 / 131.8; 8 groups, 1008 -> 2064, the gradient at 200 rows, 2 and 1: 25.0 / 18.5.
+  const bool pairs = 16 * tile_rounds(rows, n_groups, 2 * kFpTile, col_tiles, 2, sms) <=
+                     17 * tile_rounds(rows, n_groups, kFpTile, col_tiles, 1, sms);
+  const int ctas = split == 1 && pairs ? 2 : 1;
   BlockParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType t = dtype == COMFY_MOE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

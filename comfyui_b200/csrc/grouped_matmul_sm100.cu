@@ -380,16 +380,9 @@ grouped_matmul_kernel(const __grid_constant__ GmmParams p) {
 // 2048 -> 2048, 100 rows, 1 and 2: 19.0 / 26.1.  d W, whose contraction is the rows, writes more than it multiplies below
 // 256 rows a group: at 200 57.1 / 51.9, 28.9 / 25.7; 300 63.6 / 65.8, 34.4 / 36.3; 900 110.7 / 148.3.  Tiles of 64 columns,
 // and pairs with 128, were never the fastest.
-static int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
-
 static bool pairs_take_fewer_rounds(int64_t rows, int64_t groups, int64_t cols, int sms) {
-  const int64_t busy = groups < rows ? groups : rows;          // no more groups than rows have any
-  auto rounds = [&](int64_t tile) {
-    const int64_t some = rows / tile + busy / 2;               // a group's last tile is half full, more or less
-    const int64_t row_tiles = groups == 1 ? up_to(rows, tile) : (some > busy ? some : busy);
-    return up_to(row_tiles * up_to(cols, tile) * (tile / kTileM), sms);
-  };
-  return rounds(2 * kTileM) < rounds(kTileM);
+  return tile_rounds(rows, groups, 2 * kTileM, up_to(cols, 2 * kTileM), 2, sms) <
+         tile_rounds(rows, groups, kTileM, up_to(cols, kTileM), 1, sms);
 }
 
 // Few tiles with a long contraction are shared by clusters (pick_split).  Measured (us, whole / shared): y at 100 rows,

@@ -283,6 +283,16 @@ int pick_split(int64_t tiles, int64_t steps, int64_t worth, int threads, size_t 
   return 1;
 }
 
+inline int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step; }
+
+// Rounds of tiles of `tile` rows that the SMs go through, `ctas` of them to a tile, by how many row tiles are to be expected:
+// a group's last one is half full, more or less, and no more groups than rows have any.
+inline int64_t tile_rounds(int64_t rows, int64_t groups, int64_t tile, int64_t col_tiles, int ctas, int sms) {
+  const int64_t busy = groups < rows ? groups : rows, some = rows / tile + busy / 2;
+  const int64_t row_tiles = groups == 1 ? up_to(rows, tile) : (some > busy ? some : busy);
+  return up_to(row_tiles * col_tiles * ctas, sms);
+}
+
 // No more row tiles than these, however the rows are dealt to the groups.
 inline int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t tile) {
   return rows / tile + (groups < rows ? groups : rows);
