@@ -474,3 +474,26 @@ def test_few_tiles_and_a_long_contraction(cuda_device, counts, n, k, dtype):
     again = [M.grouped_block_linear(x, w, ws, offsets) for _ in range(3)]
     assert all(torch.equal(a, y) for a in again)
     M.check_all_status()
+
+
+def test_few_tiles_with_strides_padding_and_given_results(cuda_device):
+    from comfyui_b200 import moe_ops as M
+
+    dev, n, k = cuda_device, 272, 4112
+    gen = torch.Generator(device=dev).manual_seed(9)
+    offsets = torch.tensor([3, 60, 60, 110], dtype=torch.int32, device=dev)
+    counts = torch.tensor([50, 1, 41], dtype=torch.int32, device=dev)
+    x = torch.randn((120, k + 24), generator=gen, device=dev).bfloat16()[:, 8:8 + k]
+    keep = torch.zeros(120, dtype=torch.bool, device=dev)
+    for lo, hi in ((3, 53), (60, 101)):
+        keep[lo:hi] = True
+    x[~keep] = float("nan")
+    w, ws = M.quantize_weight_blocks_e4m3(0.05 * torch.randn((3, n, k), generator=gen, device=dev))
+    y = torch.full((120, n + 8), 7.0, dtype=torch.bfloat16, device=dev)
+    M.grouped_block_linear(x, w, ws, offsets, counts, out=y[:, :n])
+    for g, lo, hi in ((0, 3, 53), (2, 60, 101)):
+        close(y[lo:hi, :n], *product(x[lo:hi], w[g], ws[g], None, x.dtype), k, f"y of group {g}")
+    assert (y[~keep] == 7).all() and (y[:, n:] == 7).all()
+    z = M.grouped_block_linear(x, w, ws, offsets, counts)
+    assert torch.equal(z[keep], y[keep, :n]) and (z[~keep] == 0).all()
+    M.check_all_status()

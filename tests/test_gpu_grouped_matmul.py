@@ -396,3 +396,60 @@ def test_few_tiles_run_alike_and_replay(cuda_device):
     assert torch.equal(out, y) and torch.equal(dw, first[1])
     assert torch.equal(M.grouped_matmul_dgrad(dy, w, offsets), first[0])
     M.check_all_status()
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_few_tiles_with_strides_padding_and_given_results(cuda_device, out_dtype):
+    """Rows 16 apart in wider buffers, values that are not finite behind the groups, results in the middle of others."""
+    from comfyui_b200 import moe_ops as M
+
+    dev, k, n = cuda_device, 2056, 264
+    gen = torch.Generator(device=dev).manual_seed(9)
+    offsets = torch.tensor([2, 2900, 2900, 5900], dtype=torch.int32, device=dev)
+    counts = torch.tensor([2801, 9, 2777], dtype=torch.int32, device=dev)
+    ranges = [(2, 2803), (2900, 2900), (2900, 5677)]
+    used = torch.zeros(6000, dtype=torch.bool, device=dev)
+    for lo, hi in ranges:
+        used[lo:hi] = True
+    x = torch.randn((6000, 160), generator=gen, device=dev).bfloat16()[:, 8:144]
+    dy = torch.randn((6000, n + 16), generator=gen, device=dev).bfloat16()[:, 8:8 + n]
+    x[~used], dy[~used] = float("nan"), float("inf")
+    dw = torch.full((3, n + 1, 144), 7.0, dtype=out_dtype, device=dev)
+    M.grouped_matmul_wgrad(dy, x, offsets, counts, out=dw[:, :n, :136], out_dtype=out_dtype)
+    for g, (lo, hi) in enumerate(ranges):
+        a, b = dy[lo:hi].double(), x[lo:hi].double()
+        close(dw[g, :n, :136], a.t() @ b, a.abs().t() @ b.abs(), max(hi - lo, 1), f"dw[{g}]")
+    assert (dw[:, n] == 7).all() and (dw[:, :, 136:] == 7).all()
+    few, most = torch.tensor([3, 60, 60, 110], dtype=torch.int32, device=dev), torch.tensor([50, 1, 41], dtype=torch.int32, device=dev)
+    ranges = [(3, 53), (60, 60), (60, 101)]
+    small = torch.randn((120, k + 24), generator=gen, device=dev).bfloat16()[:, 8:8 + k]
+    w = (0.05 * torch.randn((3, n, k), generator=gen, device=dev)).bfloat16()
+    keep = torch.zeros(120, dtype=torch.bool, device=dev)
+    for lo, hi in ranges:
+        keep[lo:hi] = True
+    small[~keep] = float("nan")
+    y = torch.full((120, n + 8), 7.0, dtype=torch.bfloat16, device=dev)
+    M.grouped_matmul(small, w, few, most, out=y[:, :n])
+    ref, mag = by_group(small, w, ranges, 120, n, lambda a, b: a @ b.t())
+    close(y[keep, :n], ref[keep], mag[keep], k, "y")
+    assert (y[~keep] == 7).all() and (y[:, n:] == 7).all()
+    z = M.grouped_matmul(small, w, few, most)
+    assert torch.equal(z[keep], y[keep, :n]) and (z[~keep] == 0).all()
+    M.check_all_status()
+
+
+def test_few_tiles_on_two_streams_at_once(cuda_device):
+    from comfyui_b200 import moe_ops as M
+
+    x, w, dy, offsets = make(cuda_device, [2000, 0, 1203], 4096, 136, torch.bfloat16)
+    want = M.grouped_matmul_wgrad(dy, x, offsets)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for i in range(12):
+        stream = streams[i % 3]
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got.append(M.grouped_matmul_wgrad(dy, x, offsets))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    M.check_all_status()
