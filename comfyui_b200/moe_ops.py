@@ -841,13 +841,20 @@ def _group_stride(what: str, t: torch.Tensor, unit: int) -> int:
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
-    """A gradient as autograd hands it over (possibly expanded or transposed), as rows that the kernels can read."""
+    """A tensor as autograd hands it over (a gradient, possibly expanded or transposed; a saved tensor, in whatever layout a
+    saved-tensor hook gives back), as rows that the kernels can read."""
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t
     unit = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0)) and \
-        t.data_ptr() % 16 == 0
+    rows, cols = t.size(-2), t.size(-1)
+    ok = t.stride(-1) == 1 and (rows <= 1 or (t.stride(-2) >= cols and t.stride(-2) % unit == 0)) and \
+        (t.dim() == 2 or t.size(0) <= 1 or (t.stride(0) > 0 and t.stride(0) % unit == 0)) and t.data_ptr() % 16 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Saved offsets, counts or scales, which the kernels read without strides."""
+    return None if t is None else t.contiguous()
 
 
 def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups: int) -> None:
@@ -957,27 +964,18 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, counts):
         ctx.save_for_backward(x, w, offsets, counts)
-        ctx.sizes = sizes = _grouped_sizes(x, w, offsets, counts, 2)
+        sizes = _grouped_sizes(x, w, offsets, counts, 2)
         return _rows_by_group("comfy_moe_grouped_matmul", sizes, x, w, offsets, counts, None, sizes[4])
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_matmul")
+        # a saved-tensor hook (offloading, compression) may give back tensors of other strides, so all are measured again
         x, w, offsets, counts = ctx.saved_tensors
-        index, code, r, g, n, k, ld_x, ld_w, step = ctx.sizes      # checked by the forward pass; dy has the result's shape
+        offsets, counts, dy = _vector(offsets), _vector(counts), _readable(dy)
         need_x, need_w = ctx.needs_input_grad[:2]
-        dy = _readable(dy)
-        ld_dy = n if r <= 1 else dy.stride(0)
-        dx = dw = None
-        if need_x:
-            sizes = (index, code, r, g, n, k, ld_dy, ld_w, step)
-            dx = _rows_by_group("comfy_moe_grouped_matmul_dgrad", sizes, dy, w, offsets, counts, None, k)
-        if need_w:
-            dw = x.new_empty((g, n, k))
-            if g:
-                _call("comfy_moe_grouped_matmul_wgrad", index, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, r, g, n, k,
-                      offsets.data_ptr(), _address(counts), code, dw.data_ptr(), k, n * k,
-                      device_status(x.device).data_ptr())
+        dx = grouped_matmul_dgrad(dy, _readable(w), offsets, counts) if need_x else None
+        dw = grouped_matmul_wgrad(dy, _readable(x), offsets, counts) if need_w else None
         return dx, dw, None, None
 
 
@@ -1127,25 +1125,18 @@ def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch
     return _block_product(sizes, dy, w, w_scale, offsets, counts, None, out, True)
 
 
-def _block_backward(ctx, dy: torch.Tensor, w, w_scale, offsets, counts) -> torch.Tensor:
-    index, code, r, groups, n, k, _, ld_w, step = ctx.sizes        # checked by the forward pass; dy has the result's shape
-    sizes = (index, code, r, groups, n, k, n if r <= 1 else dy.stride(0), ld_w, step)
-    return _block_product(sizes, dy, w, w_scale, offsets, counts, None, None, True)
-
-
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, bias):
         ctx.save_for_backward(w, w_scale)
-        ctx.sizes = sizes = _block_sizes(x, w, w_scale, None, None, bias, False)
-        return _block_product(sizes, x, w, w_scale, None, None, bias, None, False)
+        return _block_product(_block_sizes(x, w, w_scale, None, None, bias, False), x, w, w_scale, None, None, bias, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("block_linear")
-        w, w_scale = ctx.saved_tensors
+        w, w_scale = ctx.saved_tensors                  # (of any strides: a saved-tensor hook may have copied them)
         dy = _readable(dy)
-        dx = _block_backward(ctx, dy, w, w_scale, None, None) if ctx.needs_input_grad[0] else None
+        dx = block_linear_dgrad(dy, _readable(w), _vector(w_scale)) if ctx.needs_input_grad[0] else None
         db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, db
 
@@ -1154,10 +1145,12 @@ class _GroupedBlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, offsets, counts):
         ctx.save_for_backward(w, w_scale, offsets, counts)
-        ctx.sizes = sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
+        sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
         return _block_product(sizes, x, w, w_scale, offsets, counts, None, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_block_linear")
-        return _block_backward(ctx, _readable(dy), *ctx.saved_tensors), None, None, None, None
+        w, w_scale, offsets, counts = ctx.saved_tensors
+        dx = grouped_block_linear_dgrad(_readable(dy), _readable(w), _vector(w_scale), _vector(offsets), _vector(counts))
+        return dx, None, None, None, None

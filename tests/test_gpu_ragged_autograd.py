@@ -1,0 +1,45 @@
+"""Autograd around the products by expert and the block-scaled products: saved-tensor hooks, derivatives that are refused,
+what a backward pass keeps.  Needs a B200."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def strided(t, before, behind):
+    """The values of t as a slice of wider rows (and, for weights, of more rows), with NaN around them."""
+    pad = (before, behind) if t.dim() == 2 else (before, behind, 0, 3)
+    wide = torch.nn.functional.pad(t.float(), pad, value=float("nan")).to(t.dtype)
+    return wide[..., :t.shape[-2], before:before + t.shape[-1]]
+
+
+@pytest.mark.parametrize("pin", [False, True], ids=["pageable", "pinned"])
+def test_strided_operands_saved_on_the_host(cuda_device, pin):
+    """save_on_cpu hands back dense copies of strided operands: the gradients are those of the direct calls."""
+    from comfyui_b200 import moe_ops as M
+
+    dev, k, n = cuda_device, 136, 80
+    gen = torch.Generator(device=dev).manual_seed(4)
+    x = strided(torch.randn((201, k), generator=gen, device=dev).bfloat16(), 8, 512)
+    w = strided(torch.randn((2, n, k), generator=gen, device=dev).bfloat16(), 8, 256)
+    dy = torch.randn((201, n), generator=gen, device=dev).bfloat16()
+    off = torch.tensor([0, 70, 201], dtype=torch.int32, device=dev)
+    want = M.grouped_matmul_dgrad(dy, w, off), M.grouped_matmul_wgrad(dy, x, off)
+    xg, wg = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+        y = M.grouped_matmul(xg, wg, off)
+    got = torch.autograd.grad(y, (xg, wg), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    k = 272
+    x = torch.randn((201, k), generator=gen, device=dev).bfloat16()
+    wq, ws = M.quantize_weight_blocks_e4m3(torch.randn((2, n, k), generator=gen, device=dev))
+    wide = strided(wq, 16, 240)
+    assert not wide.is_contiguous()
+    want = M.grouped_block_linear_dgrad(dy, wq, ws, off), M.block_linear_dgrad(dy, wq[1], ws[1])
+    x.requires_grad_(True)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+        ys = M.grouped_block_linear(x, wide, ws, off), M.block_linear(x, wide[1], ws[1])
+    for y, expected in zip(ys, want):
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], expected)
+    M.check_all_status()

@@ -1,0 +1,95 @@
+"""Autograd around the products by expert, what needs no GPU: a recorder stands in for the C entry points."""
+import pytest
+import torch
+
+
+class Recorder:
+    """Calls of the C entry points as {name: arguments}; nothing is launched and no result is written."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __call__(self, name, index, *args):
+        self.calls[name] = args
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    from comfyui_b200 import moe_ops as M
+
+    rec = Recorder()
+    monkeypatch.setattr(M, "_call", rec)
+    monkeypatch.setattr(M, "_place", lambda first, *others: 0)
+    monkeypatch.setattr(M, "device_status", lambda device: torch.zeros(4, dtype=torch.int32))
+    return rec
+
+
+def dense_copies():
+    """What an offloading hook does: a dense copy when a tensor is saved, handed back in the backward pass."""
+    kept = []
+
+    def pack(t):
+        kept.append(torch.empty(t.size(), dtype=t.dtype).copy_(t))
+        return kept[-1]
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), kept
+
+
+def test_gradients_read_the_strides_of_what_a_hook_hands_back(recorder):
+    from comfyui_b200 import moe_ops as M
+
+    k, n = 64, 80
+    x = torch.zeros((11, 1024), dtype=torch.bfloat16)[:, :k].requires_grad_(True)
+    w = torch.zeros((2, 96, 1024), dtype=torch.bfloat16)[:, :n, :k].requires_grad_(True)
+    off = torch.tensor([0, 5, 11], dtype=torch.int32)
+    dy = torch.zeros((11, n), dtype=torch.bfloat16)
+    hooks, kept = dense_copies()
+    with hooks:
+        y = M.grouped_matmul(x, w, off)
+    torch.autograd.grad(y, (x, w), dy)
+    kx, kw = [t for t in kept if t.shape == x.shape][0], [t for t in kept if t.shape == w.shape][0]
+    args = recorder.calls["comfy_moe_grouped_matmul_wgrad"]
+    assert args[2:4] == (kx.data_ptr(), k)                                     # x and its row stride
+    args = recorder.calls["comfy_moe_grouped_matmul_dgrad"]
+    assert args[2:5] == (kw.data_ptr(), k, n * k)                              # w, its row and its group stride
+
+
+def test_block_gradients_read_the_strides_of_what_a_hook_hands_back(recorder):
+    from comfyui_b200 import moe_ops as M
+
+    k, n = 64, 80
+    x = torch.zeros((11, k), dtype=torch.bfloat16, requires_grad=True)
+    w = torch.zeros((2, 96, 1024), dtype=torch.uint8).view(torch.float8_e4m3fn)[:, :n, :k]
+    ws = torch.ones((2, 1, 1))
+    off = torch.tensor([0, 5, 11], dtype=torch.int32)
+    dy = torch.zeros((11, n), dtype=torch.bfloat16)
+    for call, shape, step in ((lambda: M.grouped_block_linear(x, w, ws, off), w.shape, n * k),
+                              (lambda: M.block_linear(x, w[1], ws[1]), w[1].shape, 1)):
+        hooks, kept = dense_copies()
+        with hooks:
+            y = call()
+        torch.autograd.grad(y, x, dy)
+        kw = [t for t in kept if t.shape == shape][0]
+        assert recorder.calls["comfy_moe_block_matmul"][4:7] == (kw.data_ptr(), k, step)
+
+
+def test_what_a_hook_hands_back_unreadable_is_copied(recorder):
+    """Transposed memory and odd addresses."""
+    from comfyui_b200 import moe_ops as M
+
+    k, n = 64, 80
+    x = torch.zeros((11, k), dtype=torch.bfloat16, requires_grad=True)
+    w = torch.zeros((2, n, k), dtype=torch.bfloat16, requires_grad=True)
+    off = torch.tensor([0, 5, 11], dtype=torch.int32)
+
+    def other_layout(t):
+        if t.dim() == 3:
+            return t.transpose(1, 2).contiguous().transpose(1, 2)
+        buf = torch.zeros((t.numel() + 1,), dtype=t.dtype)[1:].view(t.shape)
+        return buf.copy_(t)
+
+    with torch.autograd.graph.saved_tensors_hooks(other_layout, lambda t: t):
+        y = M.grouped_matmul(x, w, off)
+    torch.autograd.grad(y, (x, w), torch.zeros((11, n), dtype=torch.bfloat16))
+    for name, at, ld in (("comfy_moe_grouped_matmul_dgrad", 2, k), ("comfy_moe_grouped_matmul_wgrad", 2, k)):
+        assert recorder.calls[name][at] % 16 == 0 and recorder.calls[name][at + 1] == ld
