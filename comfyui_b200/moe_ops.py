@@ -879,6 +879,20 @@ def _once(what: str) -> None:
         raise RuntimeError(f"{what} is differentiable once: its gradient has no gradient")
 
 
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of them is a dual tensor of a forward-mode derivative that is being taken."""
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+               for t in tensors)
+
+
+def _no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Dual tensors ask for a derivative without requires_grad; a result without a tangent would say that it is zero."""
+    if has_tangent(*tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _grouped_sizes(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, counts: Optional[torch.Tensor],
                    width: int) -> tuple:
     """What the C entry points want to know of checked rows and weights: (device index, dtype code, rows, groups, N, K,
@@ -914,7 +928,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
     where ``counts`` is given (the routing plan's expert_offsets and expert_counts).  x [R, K], w [G, N, K], both bf16 or
     both fp16, K and N multiples of 8, y [R, N]; offsets int32 [G + 1], counts int32 [G], on the device and never read by
     the host.  Rows of no group are zero in a result that this function makes, and stay as they were in ``out``.
-    Differentiable in x and w (once); a group without rows has the gradient 0."""
+    Differentiable in x and w (once, in reverse mode); a group without rows has the gradient 0."""
+    _no_tangents("grouped_matmul", x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         if out is not None:
             raise ValueError("grouped_matmul: out cannot be given where a gradient is asked for")
@@ -1087,8 +1102,9 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
     """``x @ (w * scales).T + bias`` in e4m3: x [.., K] (bf16 or fp16) is quantised by blocks of 128 on the way
     (quantize_blocks_e4m3), w is e4m3 [N, K] with w_scale [ceil(N / 128), ceil(K / 128)] (quantize_weight_blocks_e4m3),
     bias [N] in x's dtype; K a multiple of 16, N of 8 (of 16 where a gradient is asked for); sums in fp32, result [.., N]
-    in x's dtype.  Differentiable (once) in x, whose gradient is the same product with the gradient of the result
-    quantised and the weight transposed, and in bias; w is frozen."""
+    in x's dtype.  Differentiable (once, in reverse mode) in x, whose gradient is the same product with the gradient of the
+    result quantised and the weight transposed, and in bias; w is frozen."""
+    _no_tangents("block_linear", x, w, w_scale, bias)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if _asks_for_gradient(x, w, w_scale, bias, out):
         y = _BlockLinear.apply(rows, w, w_scale, bias)
@@ -1112,6 +1128,7 @@ def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor
     """block_linear by expert: ``y[r] = x[r] @ (w[g] * scales[g]).T`` for the rows r of group g.  x [R, K], w e4m3
     [G, N, K], w_scale [G, ceil(N / 128), ceil(K / 128)]; offsets, counts, out and rows of no group as for grouped_matmul,
     the quantised rows and the gradient (x only) as for block_linear."""
+    _no_tangents("grouped_block_linear", x, w, w_scale)
     if _asks_for_gradient(x, w, w_scale, None, out):
         return _GroupedBlockLinear.apply(x, w, w_scale, offsets, counts)
     sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)

@@ -683,7 +683,7 @@ def swiglu_ffn_forward(ffn, x: torch.Tensor) -> Optional[torch.Tensor]:
 def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
     """A Linear of ``block_scaled_fp8_ops`` on the block-scaled product, or None when this call is not eligible: bf16 or
     fp16 input on a B200 with the weight and its scales beside it, no patch closures, in_features a multiple of 16,
-    out_features of 8 (of 16 where a gradient is asked for)."""
+    out_features of 8 (of 16 where a gradient is asked for), no forward-mode derivative."""
     w, s, b = lin.weight, lin.scale_weight, lin.bias
     if not ENABLE_SM100_KERNELS or lin.weight_function or lin.bias_function or not x.is_cuda or \
             x.dtype not in (torch.bfloat16, torch.float16) or not model_management.is_sm100(x.device):
@@ -694,6 +694,10 @@ def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
     grad = torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad))
     if grad and w.shape[0] % 16:
         return None
+    from . import moe_ops
+
+    if moe_ops.has_tangent(x, b):
+        return None
     if b is not None:
         b = model_management.cast_to(b, dtype=x.dtype, device=x.device)
         if b.data_ptr() % 16:
@@ -701,8 +705,6 @@ def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
     rows = x.reshape(-1, x.shape[-1])
     if rows.stride(-1) != 1 or rows.data_ptr() % 16 or (rows.shape[0] > 1 and (rows.stride(0) % 8 or rows.stride(0) < rows.shape[1])):
         rows = rows.clone(memory_format=torch.contiguous_format)
-    from . import moe_ops
-
     with _Range("comfyui_b200::block_linear"):
         return moe_ops.block_linear(rows, w, s, b).view(x.shape[:-1] + (w.shape[0],))
 

@@ -43,3 +43,27 @@ def test_strided_operands_saved_on_the_host(cuda_device, pin):
     for y, expected in zip(ys, want):
         assert torch.equal(torch.autograd.grad(y, x, dy)[0], expected)
     M.check_all_status()
+
+
+def test_forward_mode_of_a_linear(cuda_device):
+    """The tensor-level calls refuse a dual tensor; a Linear of the namespace composes, so its tangent is that of the weight."""
+    from torch.autograd import forward_ad
+
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import ops
+
+    dev, n, k = cuda_device, 48, 64
+    gen = torch.Generator(device=dev).manual_seed(3)
+    lin = ops.block_scaled_fp8_ops().Linear(k, n, device=dev, dtype=torch.bfloat16)
+    w, ws = M.quantize_weight_blocks_e4m3(torch.randn((n, k), generator=gen, device=dev))
+    lin.load_state_dict({"weight": w, "scale_weight": ws, "bias": torch.zeros(n, device=dev).bfloat16()}, strict=True)
+    x = torch.randn((9, k), generator=gen, device=dev).bfloat16()
+    along = torch.zeros_like(x)
+    along[:, 5] = 1                                          # the tangent is then one column of the weight, rounded once
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, along)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            M.block_linear(dual, w, ws)
+        got = forward_ad.unpack_dual(lin(dual)).tangent
+    want = w.double()[:, 5] * ws.double()[0, 0]
+    assert got is not None and ((got.double() - want).abs() <= 2.0 ** -7 * want.abs()).all()

@@ -93,3 +93,27 @@ def test_what_a_hook_hands_back_unreadable_is_copied(recorder):
     torch.autograd.grad(y, (x, w), torch.zeros((11, n), dtype=torch.bfloat16))
     for name, at, ld in (("comfy_moe_grouped_matmul_dgrad", 2, k), ("comfy_moe_grouped_matmul_wgrad", 2, k)):
         assert recorder.calls[name][at] % 16 == 0 and recorder.calls[name][at + 1] == ld
+
+
+def test_forward_mode_derivatives_are_refused(recorder):
+    """A result without a tangent would read as a derivative of zero."""
+    from torch.autograd import forward_ad
+
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import torch_ops  # noqa: F401
+
+    x, w = torch.zeros((11, 64), dtype=torch.bfloat16), torch.zeros((2, 48, 64), dtype=torch.bfloat16)
+    off = torch.tensor([0, 5, 11], dtype=torch.int32)
+    wq, ws, bias = w.to(torch.float8_e4m3fn), torch.ones((2, 1, 1)), torch.zeros(48, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))                          # noqa: E731
+        for call in (lambda: M.grouped_matmul(dual(x), w, off), lambda: M.grouped_matmul(x, dual(w), off),
+                     lambda: M.block_linear(dual(x), wq[0], ws[0]), lambda: M.block_linear(x, wq[0], ws[0], dual(bias)),
+                     lambda: M.block_linear(x, wq[0], dual(ws[0])), lambda: M.grouped_block_linear(dual(x), wq, ws, off),
+                     lambda: torch.ops.comfyui_b200.grouped_matmul(dual(x), w, off)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert M.grouped_matmul(x, w, off).shape == (11, 48)                                 # no operand has a tangent
+        assert M.block_linear(x, wq[0], ws[0], bias).shape == (11, 48)
