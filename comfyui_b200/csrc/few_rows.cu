@@ -259,9 +259,12 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewPa
   few_store<T, 1>(p, part, sum, begin, count, n0);
 }
 
+// Whether there may be rows of no group to zero: without offsets the one group has all rows, unless counts say fewer.
+static bool few_zeroes(const FewParams& p) { return p.zero_unused && (p.offsets || p.counts); }
+
 template <auto kKernel>
 static int launch_few(const FewParams& p, size_t smem, size_t most, cudaStream_t stream) {
-  const dim3 grid((p.n + kFewCols - 1) / kFewCols, p.groups + (p.zero_unused && p.offsets ? 1 : 0));
+  const dim3 grid((p.n + kFewCols - 1) / kFewCols, p.groups + (few_zeroes(p) ? 1 : 0));
   if (smem > 32 * 1024) {                      // beyond what a kernel may have unasked, beside its static part
     const int rc = allow_shared_memory<kKernel>(most);
     if (rc != COMFY_MOE_OK) return rc;
@@ -270,9 +273,7 @@ static int launch_few(const FewParams& p, size_t smem, size_t most, cudaStream_t
   return check_launch();
 }
 
-static size_t few_tables(const FewParams& p) {
-  return p.zero_unused && p.offsets ? ragged_tables(p.groups) : 0;
-}
+static size_t few_tables(const FewParams& p) { return few_zeroes(p) ? ragged_tables(p.groups) : 0; }
 
 int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
   if (p.rows <= 8)
