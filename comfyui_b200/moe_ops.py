@@ -1092,8 +1092,8 @@ def _asks_for_gradient(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, 
         return False
     if out is not None:
         raise ValueError("out cannot be given where a gradient is asked for")
-    if w.shape[-2] % 16:
-        raise ValueError(f"out_features must be a multiple of 16 for a gradient, got {w.shape[-2]}")
+    if x.requires_grad and w.shape[-2] % 16:
+        raise ValueError(f"out_features must be a multiple of 16 for a gradient of the rows, got {w.shape[-2]}")
     return True
 
 
@@ -1101,9 +1101,9 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ (w * scales).T + bias`` in e4m3: x [.., K] (bf16 or fp16) is quantised by blocks of 128 on the way
     (quantize_blocks_e4m3), w is e4m3 [N, K] with w_scale [ceil(N / 128), ceil(K / 128)] (quantize_weight_blocks_e4m3),
-    bias [N] in x's dtype; K a multiple of 16, N of 8 (of 16 where a gradient is asked for); sums in fp32, result [.., N]
-    in x's dtype.  Differentiable (once, in reverse mode) in x, whose gradient is the same product with the gradient of the
-    result quantised and the weight transposed, and in bias; w is frozen."""
+    bias [N] in x's dtype; K a multiple of 16, N of 8 (of 16 where a gradient of x is asked for); sums in fp32, result
+    [.., N] in x's dtype.  Differentiable (once, in reverse mode) in x, whose gradient is the same product with the gradient
+    of the result quantised and the weight transposed, and in bias; w is frozen."""
     _no_tangents("block_linear", x, w, w_scale, bias)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if _asks_for_gradient(x, w, w_scale, bias, out):

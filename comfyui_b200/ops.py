@@ -683,7 +683,7 @@ def swiglu_ffn_forward(ffn, x: torch.Tensor) -> Optional[torch.Tensor]:
 def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
     """A Linear of ``block_scaled_fp8_ops`` on the block-scaled product, or None when this call is not eligible: bf16 or
     fp16 input on a B200 with the weight and its scales beside it, no patch closures, in_features a multiple of 16,
-    out_features of 8 (of 16 where a gradient is asked for), no forward-mode derivative."""
+    out_features of 8 (of 16 where a gradient of x is asked for), no forward-mode derivative."""
     w, s, b = lin.weight, lin.scale_weight, lin.bias
     if not ENABLE_SM100_KERNELS or lin.weight_function or lin.bias_function or not x.is_cuda or \
             x.dtype not in (torch.bfloat16, torch.float16) or not model_management.is_sm100(x.device):
@@ -691,8 +691,7 @@ def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
     if w.dtype != FP8 or w.device != x.device or s.device != x.device or s.dtype != torch.float32 or \
             w.shape[1] % 16 or w.shape[0] % 8 or not w.is_contiguous() or w.data_ptr() % 16 or not s.is_contiguous():
         return None
-    grad = torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad))
-    if grad and w.shape[0] % 16:
+    if torch.is_grad_enabled() and x.requires_grad and w.shape[0] % 16:
         return None
     from . import moe_ops
 

@@ -67,3 +67,23 @@ def test_forward_mode_of_a_linear(cuda_device):
         got = forward_ad.unpack_dual(lin(dual)).tangent
     want = w.double()[:, 5] * ws.double()[0, 0]
     assert got is not None and ((got.double() - want).abs() <= 2.0 ** -7 * want.abs()).all()
+
+
+def test_the_gradient_of_a_bias_alone(cuda_device):
+    """out_features of 8 stay on the kernel where only the bias asks for a gradient, in the call and in a Linear."""
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import ops
+
+    dev, n, k = cuda_device, 72, 272
+    gen = torch.Generator(device=dev).manual_seed(8)
+    x = torch.randn((50, k), generator=gen, device=dev).bfloat16()
+    w, ws = M.quantize_weight_blocks_e4m3(torch.randn((n, k), generator=gen, device=dev))
+    bias = torch.randn((n,), generator=gen, device=dev).bfloat16()
+    dy = torch.randint(-3, 4, (50, n), generator=gen, device=dev).bfloat16()          # sums of whole numbers are exact
+    want = M.block_linear(x, w, ws, bias)
+    lin = ops.block_scaled_fp8_ops().Linear(k, n, device=dev, dtype=torch.bfloat16)
+    lin.load_state_dict({"weight": w, "scale_weight": ws, "bias": bias}, strict=True)
+    leaf = bias.clone().requires_grad_(True)
+    for y, b in ((M.block_linear(x, w, ws, leaf), leaf), (lin(x), lin.bias)):
+        assert torch.equal(y, want)
+        assert torch.equal(torch.autograd.grad(y, b, dy)[0], dy.float().sum(0).bfloat16())

@@ -117,3 +117,18 @@ def test_forward_mode_derivatives_are_refused(recorder):
                 call()
         assert M.grouped_matmul(x, w, off).shape == (11, 48)                                 # no operand has a tangent
         assert M.block_linear(x, wq[0], ws[0], bias).shape == (11, 48)
+
+
+def test_the_gradient_of_a_bias_alone_needs_no_product(recorder):
+    """out_features of 8: the gradient of x would contract over them in steps of 16, that of the bias only adds up."""
+    from comfyui_b200 import moe_ops as M
+
+    x, bias = torch.zeros((11, 64), dtype=torch.bfloat16), torch.zeros(72, dtype=torch.bfloat16, requires_grad=True)
+    w, ws = torch.zeros((72, 64), dtype=torch.bfloat16).to(torch.float8_e4m3fn), torch.ones((1, 1))
+    dy = torch.arange(11.0)[:, None].expand(11, 72).bfloat16()
+    y = M.block_linear(x, w, ws, bias)
+    recorder.calls.clear()
+    db, = torch.autograd.grad(y, bias, dy)
+    assert (db == 55).all() and not recorder.calls
+    with pytest.raises(ValueError, match="multiple of 16 for a gradient"):
+        M.block_linear(x.clone().requires_grad_(True), w, ws, bias)
