@@ -301,16 +301,22 @@ def block_scaled_fp8_ops(fp8_matrix_mult=True):
                 weight, bias = cast_bias_weight(self, input)
                 return F.linear(input, self.convert_weight(weight), bias)
 
+            # The scales stay in fp32, as the kernel applies them: in fp16 those below 6e-5 would lose digits and those
+            # below 3e-8 would be 0, in bf16 each would shift its whole block by up to 2^-8.
+            def _wide(self, weight):
+                """The weight and a scale for each of its elements, in fp32 or more."""
+                wide = torch.float64 if weight.dtype == torch.float64 else torch.float32
+                scale = self.scale_weight.to(device=weight.device, dtype=wide)
+                return weight.to(wide), _spread_block_scales(scale, *weight.shape)
+
             def convert_weight(self, weight, inplace=False, **kwargs):
-                scale = _spread_block_scales(self.scale_weight, *weight.shape).to(device=weight.device, dtype=weight.dtype)
-                if inplace:
-                    weight *= scale
-                    return weight
-                return weight * scale
+                wide, scale = self._wide(weight)
+                scaled = wide * scale
+                return weight.copy_(scaled) if inplace else scaled.to(weight.dtype)
 
             def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
-                scaled = weight / _spread_block_scales(self.scale_weight, *weight.shape).to(device=weight.device,
-                                                                                           dtype=weight.dtype)
+                wide, scale = self._wide(weight)
+                scaled = wide / scale
                 q = stochastic_rounding(scaled, self.weight.dtype, seed=seed)
                 if return_weight:
                     return q
