@@ -285,6 +285,8 @@ def block_scaled_fp8_ops(fp8_matrix_mult=True):
 
     class block_scaled_fp8_op(manual_cast):
         class Linear(manual_cast.Linear):
+            block_scales = True
+
             def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
                 super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
                 self.weight = torch.nn.Parameter(torch.empty((out_features, in_features), device=device, dtype=FP8),
@@ -481,9 +483,15 @@ def _patched_weight(lin, device):
     return out
 
 
+def _has_block_scales(lin) -> bool:
+    """Whether the weight is one of ``block_scaled_fp8_ops``.  It means nothing without its scales, also where the module has
+    been cast to bf16, so no kernel that takes a bf16 weight, or one with a scale per tensor, may take it."""
+    return getattr(lin, "block_scales", False)
+
+
 def _linear_state(lin, device):
     """(weight, scale_weight, scale_input) if this Linear can feed the kernels as it is now, else None."""
-    if lin.bias_function or lin.bias is not None:
+    if lin.bias_function or lin.bias is not None or _has_block_scales(lin):
         return None
     w = lin.weight
     if lin.weight_function:
@@ -717,7 +725,7 @@ def block_linear_forward(lin, x: torch.Tensor) -> Optional[torch.Tensor]:
 # ---- q / k / v glue of the HiDream attention processor ----------------------------------------------------------
 def _bias_linear_state(lin, device, in_features):
     """(weight, bias or None) if this bf16 Linear can feed the grouped GEMM as it is now, else None."""
-    if lin.weight_function or lin.bias_function:
+    if lin.weight_function or lin.bias_function or _has_block_scales(lin):
         return None
     w, b = lin.weight, lin.bias
     if w.device != device or w.dtype != torch.bfloat16 or w.dim() != 2 or w.stride(1) != 1 or w.shape[1] != in_features:
@@ -873,7 +881,7 @@ def hidream_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
 # ---- Hunyuan3D-2.1 MoE block (GELU feed-forwards with biases) ------------------------------------------------
 def _biased_linear_state(lin, device):
     """(weight, bias or None) if this Linear can feed the GELU-MLP kernels as it is now, else None."""
-    if lin.weight_function or lin.bias_function:
+    if lin.weight_function or lin.bias_function or _has_block_scales(lin):
         return None
     w, b = lin.weight, lin.bias
     if w.device != device or w.dtype != torch.bfloat16 or w.dim() != 2 or w.stride(1) != 1:

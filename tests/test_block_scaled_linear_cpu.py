@@ -59,3 +59,22 @@ def test_a_weight_is_set_through_scales_of_any_size(dtype):
     # smallest fp16 number over the scale, 2^-25 / 7.1e-5 = 0.22 x 2^-9; stochastic rounding then ends on it or next to it
     assert torch.isfinite(got).all()
     assert ((got - want).abs() <= torch.clamp(2.0 ** -3 * want.abs(), min=2.0 ** -9) * (1 + 2.0 ** -6)).all()
+
+
+def test_no_fused_path_takes_the_weights_without_their_scales():
+    """A module cast to bf16 as a whole holds e4m3 numbers in bf16: still nothing without the block scales."""
+    from comfyui_b200 import ops
+
+    cpu = torch.device("cpu")
+    lin, exact = linear([0.5, 0.0078125])
+    assert ops._linear_state(lin, cpu) is None
+    lin.to(torch.bfloat16)
+    assert lin.weight.dtype == torch.bfloat16
+    for state in (ops._linear_state(lin, cpu), ops._biased_linear_state(lin, cpu)):
+        assert state is None
+    wide = ops.block_scaled_fp8_ops().Linear(256, 256, dtype=torch.bfloat16).to(torch.bfloat16)      # a shape for the projections
+    assert ops._bias_linear_state(wide, cpu, 256) is None
+    plain = ops.disable_weight_init.Linear(256, 256, dtype=torch.bfloat16)
+    assert ops._bias_linear_state(plain, cpu, 256) is not None
+    x = torch.eye(K, dtype=torch.bfloat16)
+    assert torch.equal(lin(x).t().double(), exact)                           # powers of two: no rounding at all
