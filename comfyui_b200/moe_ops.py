@@ -978,7 +978,8 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, counts):
-        ctx.save_for_backward(x, w, offsets, counts)
+        need_x, need_w = ctx.needs_input_grad[:2]         # each gradient reads the other operand: keep no more than that
+        ctx.save_for_backward(x if need_w else None, w if need_x else None, offsets, counts)
         sizes = _grouped_sizes(x, w, offsets, counts, 2)
         return _rows_by_group("comfy_moe_grouped_matmul", sizes, x, w, offsets, counts, None, sizes[4])
 
@@ -1145,15 +1146,17 @@ def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, bias):
-        ctx.save_for_backward(w, w_scale)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(w, w_scale)
         return _block_product(_block_sizes(x, w, w_scale, None, None, bias, False), x, w, w_scale, None, None, bias, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("block_linear")
-        w, w_scale = ctx.saved_tensors                  # (of any strides: a saved-tensor hook may have copied them)
-        dy = _readable(dy)
-        dx = block_linear_dgrad(dy, _readable(w), _vector(w_scale)) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            w, w_scale = ctx.saved_tensors                # (of any strides: a saved-tensor hook may have copied them)
+            dx = block_linear_dgrad(_readable(dy), _readable(w), _vector(w_scale))
         db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, db
 

@@ -243,7 +243,9 @@ def _(dy, x, offsets, counts=None):
 
 
 def _grouped_setup(ctx, inputs, output):
-    ctx.save_for_backward(*inputs)
+    x, w, offsets, counts = inputs
+    need_x, need_w = ctx.needs_input_grad[:2]             # each gradient reads the other operand
+    ctx.save_for_backward(x if need_w else None, w if need_x else None, offsets, counts)
 
 
 def _grouped_backward(ctx, dy):

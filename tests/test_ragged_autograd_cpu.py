@@ -132,3 +132,29 @@ def test_the_gradient_of_a_bias_alone_needs_no_product(recorder):
     assert (db == 55).all() and not recorder.calls
     with pytest.raises(ValueError, match="multiple of 16 for a gradient"):
         M.block_linear(x.clone().requires_grad_(True), w, ws, bias)
+
+
+def test_a_frozen_operand_keeps_nothing_of_the_other(recorder):
+    """The gradient of x reads w only, that of w x only: what is not read is not kept, and may be overwritten."""
+    from comfyui_b200 import moe_ops as M
+    from comfyui_b200 import torch_ops  # noqa: F401
+
+    off, dy = torch.tensor([0, 5, 11], dtype=torch.int32), torch.zeros((11, 80), dtype=torch.bfloat16)
+    leaf = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, requires_grad=True)        # noqa: E731
+    for call in (M.grouped_matmul, torch.ops.comfyui_b200.grouped_matmul):
+        for frozen in (0, 1):
+            operands = [leaf(11, 64), leaf(2, 80, 64)]
+            operands[frozen] = operands[frozen].detach()
+            used = [t * 1 for t in operands]
+            kept = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.shape) or t, lambda t: t):
+                y = call(*used, off)
+            assert used[1 - frozen].shape not in kept and used[frozen].shape in kept
+            with torch.no_grad():
+                used[1 - frozen].add_(1)
+            torch.autograd.grad(y, operands[1 - frozen], dy)
+    w, ws, bias = torch.zeros((80, 64), dtype=torch.bfloat16).to(torch.float8_e4m3fn), torch.ones((1, 1)), leaf(80)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.shape) or t, lambda t: t):
+        y = M.block_linear(torch.zeros((11, 64), dtype=torch.bfloat16), w, ws, bias)
+    assert not kept and (torch.autograd.grad(y, bias, dy + 1)[0] == 11).all()
