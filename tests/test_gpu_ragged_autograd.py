@@ -42,7 +42,7 @@ def test_strided_operands_saved_on_the_host(cuda_device, pin):
         ys = M.grouped_block_linear(x, wide, ws, off), M.block_linear(x, wide[1], ws[1])
     for y, expected in zip(ys, want):
         assert torch.equal(torch.autograd.grad(y, x, dy)[0], expected)
-    M.check_all_status()
+    M.read_status(M.device_status(dev))
 
 
 def test_forward_mode_of_a_linear(cuda_device):

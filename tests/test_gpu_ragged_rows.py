@@ -25,4 +25,4 @@ def test_counts_of_a_single_group_without_offsets(cuda_device, rows, zero):
                 1, n, k, None, counts.data_ptr(), None, zero, out.data_ptr(), n, M.device_status(dev).data_ptr())
         used = min(used, rows)
         assert torch.equal(out[:used], want[:used]) and (out[used:] == (0 if zero else 7)).all()
-    M.check_all_status()
+    M.read_status(M.device_status(dev))
