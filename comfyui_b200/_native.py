@@ -22,7 +22,9 @@ STATIC_MAX_TOKENS = 131072
 STATUS_WORDS = 4         # [0] sticky device status, [1] near-ties of the last gate call, [2] e4m3 overflows, [3] reserved
 SCALE_BLOCK = 128            # COMFY_MOE_SCALE_BLOCK: elements along a row that share a scale
 FEW_ROWS_BLOCK, FEW_ROWS_BLOCK_MAX_K = 2, 65536      # COMFY_MOE_FEW_ROWS_BLOCK*: calls that need no workspace
+MAX_SCALE_BLOCKS = 65535     # COMFY_MOE_MAX_SCALE_BLOCKS: blocks along a row that is quantised
 RAGGED_MAX_GROUPS = 768      # COMFY_MOE_RAGGED_MAX_GROUPS: groups of one call over ragged rows
+RAGGED_MAX_ROWS, RAGGED_MAX_FEATURES = 2147482624, 268435456      # COMFY_MOE_RAGGED_MAX_ROWS, _FEATURES
 LINEAR_MAX_MAPS = 22     # COMFY_MOE_LINEAR_MAX_MAPS: distinct operands of one comfy_moe_grouped_linear call
 MAX_RANKS = 8
 EP_ARRIVED, EP_DONE = 0, 1

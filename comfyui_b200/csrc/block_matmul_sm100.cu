@@ -451,7 +451,7 @@ extern "C" int comfy_moe_block_matmul(const void* x, int64_t ld_x, int dtype, vo
   if (rows < 0 || n_groups < 0 || n <= 0 || k <= 0 || !status) return COMFY_MOE_EINVAL;
   if (dtype != COMFY_MOE_BF16 && dtype != COMFY_MOE_FP16) return COMFY_MOE_EUNSUPPORTED;
   const int in = transpose_w ? n : k, cols = transpose_w ? k : n;
-  if (n_groups > kRaggedMaxGroups || k % 16 || in % 16 || cols % 8) return COMFY_MOE_EUNSUPPORTED;
+  if (n_groups > kRaggedMaxGroups || k % 16 || in % 16 || cols % 8 || !ragged_sizes_fit(rows, n, k)) return COMFY_MOE_EUNSUPPORTED;
   if (n_groups != 1 && !offsets) return COMFY_MOE_EINVAL;
   if (rows == 0) return COMFY_MOE_OK;
   const bool quantise_inside = !transpose_w && rows <= kFewRowsQuantise && k <= kFewQuantiseMaxK;

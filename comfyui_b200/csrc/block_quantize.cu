@@ -124,15 +124,14 @@ using namespace comfy_b200;
 extern "C" int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
                                         float* scale, int64_t ld_scale, void* stream) {
   const int bytes = elem_bytes(dtype);
-  if (!bytes || cols % 16) return COMFY_MOE_EUNSUPPORTED;
+  if (!bytes || cols % 16 || rows > COMFY_MOE_RAGGED_MAX_ROWS || cols > COMFY_MOE_MAX_SCALE_BLOCKS * kQuantBlock)
+    return COMFY_MOE_EUNSUPPORTED;
   if (rows < 0 || cols <= 0) return COMFY_MOE_EINVAL;
   if (rows == 0) return COMFY_MOE_OK;
   if (!x || !out || !scale || !aligned16(x) || !aligned16(out) || ld_x < cols || ld_x * bytes % 16 || ld_out < cols ||
       ld_out % 16 || ld_scale < rows)
     return COMFY_MOE_EINVAL;
-  const int blocks = (cols + kQuantBlock - 1) / kQuantBlock;
-  if (blocks > 65535) return COMFY_MOE_EUNSUPPORTED;
-  const dim3 grid((rows + 31) / 32, blocks);
+  const dim3 grid((rows + 31) / 32, (cols + kQuantBlock - 1) / kQuantBlock);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* q = static_cast<uint8_t*>(out);
   if (dtype == COMFY_MOE_BF16)
@@ -147,14 +146,14 @@ extern "C" int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, 
 extern "C" int comfy_moe_block_quantize_weight(const void* w, int64_t ld_w, int64_t w_group_stride, int dtype, int n_groups,
                                                int out_features, int in_features, void* out, float* scale, void* stream) {
   const int bytes = elem_bytes(dtype), n = out_features, k = in_features;
-  if (!bytes || k % 16) return COMFY_MOE_EUNSUPPORTED;
+  constexpr int kMost = COMFY_MOE_MAX_SCALE_BLOCKS * kQuantBlock;
+  if (!bytes || k % 16 || k > kMost || n > kMost || n_groups > COMFY_MOE_MAX_SCALE_BLOCKS) return COMFY_MOE_EUNSUPPORTED;
   if (n_groups < 0 || n <= 0 || k <= 0) return COMFY_MOE_EINVAL;
   if (n_groups == 0) return COMFY_MOE_OK;
   if (!w || !out || !scale || !aligned16(w) || !aligned16(out) || ld_w < k || ld_w * bytes % 16 ||
       (n_groups > 1 && w_group_stride * bytes % 16))
     return COMFY_MOE_EINVAL;
   const dim3 grid((k + kQuantBlock - 1) / kQuantBlock, (n + kQuantBlock - 1) / kQuantBlock, n_groups);
-  if (grid.y > 65535 || grid.z > 65535) return COMFY_MOE_EUNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* q = static_cast<uint8_t*>(out);
   if (dtype == COMFY_MOE_BF16)

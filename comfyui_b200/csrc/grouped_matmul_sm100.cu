@@ -416,7 +416,7 @@ static bool rows_ok(const void* p, int64_t ld, int64_t cols, int elem_bytes) {
 static int check_gmm(int dtype, int rows, int groups, int n, int k, const int32_t* offsets, const int32_t* status) {
   if (rows < 0 || groups < 0 || n <= 0 || k <= 0 || !status) return COMFY_MOE_EINVAL;
   if (dtype != COMFY_MOE_BF16 && dtype != COMFY_MOE_FP16) return COMFY_MOE_EUNSUPPORTED;
-  if (groups > kRaggedMaxGroups || n % 8 || k % 8) return COMFY_MOE_EUNSUPPORTED;
+  if (groups > kRaggedMaxGroups || n % 8 || k % 8 || !ragged_sizes_fit(rows, n, k)) return COMFY_MOE_EUNSUPPORTED;
   if (groups > 0 && !offsets) return COMFY_MOE_EINVAL;
   return COMFY_MOE_OK;
 }

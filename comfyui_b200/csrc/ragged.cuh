@@ -222,6 +222,11 @@ int allow_shared_memory(size_t bytes) {
   return COMFY_MOE_OK;
 }
 
+// Sizes whose tiles, row numbers and bytes of a row the kernels count in int32.
+inline bool ragged_sizes_fit(int rows, int n, int k) {
+  return rows <= COMFY_MOE_RAGGED_MAX_ROWS && n <= COMFY_MOE_RAGGED_MAX_FEATURES && k <= COMFY_MOE_RAGGED_MAX_FEATURES;
+}
+
 constexpr size_t ragged_tables(int groups) { return (3 * static_cast<size_t>(groups) + 1) * sizeof(int); }
 
 // Persistent CTAs, one per SM, in clusters of `cluster`; `fixed` bytes of shared memory besides the groups' tables.

@@ -857,6 +857,17 @@ def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.contiguous()
 
 
+def _check_sizes(rows: int, *features: int) -> None:
+    """Sizes that the C entry points take as int32, before ctypes cuts them to it."""
+    if rows > N.RAGGED_MAX_ROWS or min(features) == 0 or max(features) > N.RAGGED_MAX_FEATURES:
+        raise ValueError(f"at most {N.RAGGED_MAX_ROWS} rows and 1 to {N.RAGGED_MAX_FEATURES} features, got {rows} and {features}")
+
+
+def _check_blocks(*sizes: int) -> None:
+    if max(sizes) > N.MAX_SCALE_BLOCKS * N.SCALE_BLOCK:
+        raise ValueError(f"at most {N.MAX_SCALE_BLOCKS} blocks of {N.SCALE_BLOCK} along a dimension, got {sizes} elements")
+
+
 def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups: int) -> None:
     if groups > N.RAGGED_MAX_GROUPS:
         raise ValueError(f"at most {N.RAGGED_MAX_GROUPS} groups, got {groups}")
@@ -904,6 +915,7 @@ def _grouped_sizes(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
     if code is None or w.dtype != a.dtype:
         raise ValueError(f"rows and weights must both be bf16 or both fp16, got {a.dtype} and {w.dtype}")
     g, n, k = w.shape
+    _check_sizes(a.size(0), n, k)
     _check_ragged(offsets, counts, g)
     return (index, code, a.size(0), g, n, k, _row_stride("rows", a, 8), _row_stride("weights", w, 8),
             _group_stride("weights", w, 8))
@@ -951,7 +963,10 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     x [R, K] -> [G, N, K] in ``out_dtype`` (x's dtype, or fp32), summed in fp32."""
     if dy.dim() != 2 or x.dim() != 2 or dy.size(0) != x.size(0):
         raise ValueError(f"need dy [R, N] and x [R, K], got {tuple(dy.shape)} and {tuple(x.shape)}")
+    if offsets.numel() == 0:
+        raise ValueError("offsets must have one element more than there are groups")
     g, (r, n), k = offsets.numel() - 1, dy.shape, x.size(1)
+    _check_sizes(r, n, k)
     index = _place(x, dy, offsets, counts, out)
     code = _HALF_CODES.get(x.dtype)
     if code is None or dy.dtype != x.dtype:
@@ -1011,6 +1026,8 @@ def quantize_blocks_e4m3(x: torch.Tensor):
     if x.dim() != 2 or x.dtype not in _QUANT_CODES or x.shape[1] == 0 or x.shape[1] % 16:
         raise ValueError("x must be [R, K] in bf16, fp16 or fp32 with K a multiple of 16")
     r, k = x.shape
+    _check_sizes(r, k)
+    _check_blocks(k)
     q = torch.empty((r, k), dtype=_FP8, device=x.device)
     scale = torch.empty((_blocks(k), r), dtype=torch.float32, device=x.device)
     _call("comfy_moe_block_quantize", index, x.data_ptr(), _row_stride("x", x, 16 // x.element_size()),
@@ -1026,6 +1043,7 @@ def quantize_weight_blocks_e4m3(w: torch.Tensor):
         raise ValueError("w must be [N, K] or [G, N, K] in bf16, fp16 or fp32 with K a multiple of 16")
     n, k = w.shape[-2:]
     groups = w.shape[0] if w.dim() == 3 else 1
+    _check_blocks(n, k, groups * N.SCALE_BLOCK)
     unit = 16 // w.element_size()
     q = torch.empty(w.shape, dtype=_FP8, device=w.device)
     scale = torch.empty(w.shape[:-2] + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
@@ -1049,6 +1067,8 @@ def _block_sizes(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offset
     n, k = w.size(-2), w.size(-1)
     if n % 8 or k % 16 or contraction % 16 or n == 0 or k == 0:
         raise ValueError(f"in_features must be a multiple of 16 and out_features of 8 (of 16 for a gradient), got {k} and {n}")
+    _check_sizes(r, n, k)
+    _check_blocks(contraction)
     nb, kb = _blocks(n), _blocks(k)
     if w_scale.dtype != torch.float32 or w_scale.shape != ((nb, kb) if offsets is None else (w.size(0), nb, kb)) or \
             not w_scale.is_contiguous():

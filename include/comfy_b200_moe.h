@@ -369,8 +369,11 @@ int comfy_moe_grouped_linear(int n_groups, const ComfyMoeLinearGroup* h_groups, 
  * dtype COMFY_MOE_BF16 or COMFY_MOE_FP16 for all operands (wgrad: out_dtype the same or COMFY_MOE_FP32); products are summed
  * in fp32 and rounded once.  Rows of `out` / `dx` that belong to no group are zeroed if zero_unused is set, else not
  * touched.  Leading dimensions and group strides in elements; every row and group starts on 16 bytes; in_features and
- * out_features are multiples of 8; n_groups <= COMFY_MOE_RAGGED_MAX_GROUPS.  status: a status block. */
+ * out_features are multiples of 8; n_groups <= COMFY_MOE_RAGGED_MAX_GROUPS; row numbers, and bytes of a row, stay within int32:
+ * rows <= COMFY_MOE_RAGGED_MAX_ROWS, features <= COMFY_MOE_RAGGED_MAX_FEATURES.  status: a status block. */
 #define COMFY_MOE_RAGGED_MAX_GROUPS 768
+#define COMFY_MOE_RAGGED_MAX_ROWS 2147482624
+#define COMFY_MOE_RAGGED_MAX_FEATURES 268435456
 int comfy_moe_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t w_group_stride, int dtype,
                              int rows, int n_groups, int out_features, int in_features, const int32_t* offsets,
                              const int32_t* counts, int zero_unused, void* out, int64_t ld_out, int32_t* status,
@@ -399,8 +402,11 @@ int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x,
  *                                    out[r, :] = x[r, :] . w[g]^T (+ bias);  transpose_w: out[r, :] = x[r, :] . w[g].
  * Groups of rows, zero_unused, status: as for comfy_moe_grouped_matmul; offsets NULL with n_groups = 1 means all rows.
  * Block products are summed in fp32 and folded, times both scales, into fp32 sums; out (and bias, contiguous) have x's
- * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes. */
+ * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes.  Rows and
+ * features as above; what is quantised has at most COMFY_MOE_MAX_SCALE_BLOCKS blocks along a row (weights: and along a column,
+ * and as many groups). */
 #define COMFY_MOE_SCALE_BLOCK 128
+#define COMFY_MOE_MAX_SCALE_BLOCKS 65535
 #define COMFY_MOE_FEW_ROWS_BLOCK 2
 #define COMFY_MOE_FEW_ROWS_BLOCK_MAX_K 65536
 int comfy_moe_block_quantize(const void* x, int64_t ld_x, int dtype, int rows, int cols, void* out, int64_t ld_out,
