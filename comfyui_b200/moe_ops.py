@@ -877,6 +877,33 @@ def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups:
         raise ValueError(f"counts must be a contiguous int32 vector of {groups} elements")
 
 
+def _extent(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte of t's elements, and the one behind the last."""
+    size = t.element_size()
+    return t.data_ptr(), t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _check_apart(out: torch.Tensor, *operands: Optional[torch.Tensor]) -> None:
+    """Tiles are written while others are still read: a result may stand between the columns of an operand's buffer, but
+    share no element with it."""
+    if out.numel() == 0:
+        return
+    first, last = _extent(out)
+    for t in operands:
+        if t is None or t.numel() == 0:
+            continue
+        begin, end = _extent(t)
+        if end <= first or last <= begin:
+            continue
+        if t.dim() == 2 and out.dim() == 2:                                # columns of the same rows?
+            pitch = {a.stride(0) * a.element_size() for a in (t, out) if a.size(0) > 1}
+            ld = pitch.pop() if len(pitch) == 1 else 0
+            shift = (first - begin) % ld if ld > 0 else 0
+            if shift >= t.size(1) * t.element_size() and shift + out.size(1) * out.element_size() <= ld:
+                continue
+        raise ValueError("out must not overlap an operand")
+
+
 def _result(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     if out is None:
         return like.new_empty((rows, cols))
@@ -929,6 +956,7 @@ def _rows_by_group(name: str, sizes: tuple, a: torch.Tensor, w: torch.Tensor, of
     else:
         res = _result(out, a, r, cols)
         ld = _row_stride("out", res, 8)
+        _check_apart(res, a, w, offsets, counts)
     _call(name, index, a.data_ptr(), ld_a, w.data_ptr(), ld_w, step, code, r, g, n, k, offsets.data_ptr(), _address(counts),
           out is None, res.data_ptr(), ld, device_status(a.device).data_ptr())
     return res
@@ -939,7 +967,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
     """``y[r] = x[r] @ w[g].T`` for the rows r of group g = rows offsets[g] .. offsets[g + 1], of which the first counts[g]
     where ``counts`` is given (the routing plan's expert_offsets and expert_counts).  x [R, K], w [G, N, K], both bf16 or
     both fp16, K and N multiples of 8, y [R, N]; offsets int32 [G + 1], counts int32 [G], on the device and never read by
-    the host.  Rows of no group are zero in a result that this function makes, and stay as they were in ``out``.
+    the host.  Rows of no group are zero in a result that this function makes, and stay as they were in ``out``, which
+    overlaps no operand.
     Differentiable in x and w (once, in reverse mode); a group without rows has the gradient 0."""
     _no_tangents("grouped_matmul", x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
@@ -984,6 +1013,8 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     ld, step = _row_stride("out", res, unit), _group_stride("out", res, unit)
     if g > 1 and step < n * ld:
         raise ValueError("out: groups must not overlap")
+    if out is not None:
+        _check_apart(out, dy, x, offsets, counts)
     _call("comfy_moe_grouped_matmul_wgrad", index, dy.data_ptr(), _row_stride("dy", dy, 8), x.data_ptr(),
           _row_stride("x", x, 8), code, r, g, n, k, offsets.data_ptr(), _address(counts),
           N.FP32 if dt == torch.float32 else code, res.data_ptr(), ld, step, device_status(x.device).data_ptr())
@@ -1094,6 +1125,7 @@ def _block_product(sizes: tuple, x: torch.Tensor, w: torch.Tensor, w_scale: torc
     else:
         res = _result(out, x, r, cols)
         ld = _row_stride("out", res, 8)
+        _check_apart(res, x, w, w_scale, offsets, counts, bias)
     work = None
     if transpose or r > N.FEW_ROWS_BLOCK or k > N.FEW_ROWS_BLOCK_MAX_K:      # the quantised rows and their scales
         work = x.new_empty((r * contraction + 255) // 256 * 256 + 4 * r * _blocks(contraction), dtype=torch.uint8)

@@ -83,3 +83,34 @@ def test_the_library_refuses_sizes_beyond_its_counters():
     assert lib.comfy_moe_block_quantize(GOOD, long, 0, 5, long, GOOD, long, GOOD, 5, None) == N.EUNSUPPORTED
     for groups, n, k in ((1, 32, long), (1, long, 32), (N.MAX_SCALE_BLOCKS + 1, 32, 32)):
         assert lib.comfy_moe_block_quantize_weight(GOOD, k, n * k, 0, groups, n, k, GOOD, GOOD, None) == N.EUNSUPPORTED
+
+
+def test_a_result_that_overlaps_an_operand_is_refused(calls):
+    """Tiles of it would be written while others are still to be read."""
+    from comfyui_b200 import moe_ops as M
+
+    off = torch.zeros(2, dtype=torch.int32)
+    x, w = torch.zeros((11, 64), dtype=torch.bfloat16), torch.zeros((1, 64, 64), dtype=torch.bfloat16)
+    wq, ws = w.to(torch.float8_e4m3fn), torch.ones((1, 1, 1))
+    rows = torch.zeros((40, 64), dtype=torch.bfloat16)
+    dw = torch.zeros((1, 64, 64), dtype=torch.bfloat16)
+    for call in (lambda: M.grouped_matmul(x, w, off, out=x), lambda: M.grouped_matmul_dgrad(x, w, off, out=x),
+                 lambda: M.grouped_matmul(rows[:11], w, off, out=rows[10:21]), lambda: M.grouped_matmul(x, w, off, out=w[0, 3:14]),
+                 lambda: M.grouped_matmul(rows.view(20, 128)[:5, :64], w, off, out=rows[:5]),
+                 lambda: M.block_linear(x, wq[0], ws[0], out=x), lambda: M.block_linear_dgrad(x, wq[0], ws[0], out=x),
+                 lambda: M.grouped_block_linear(x, wq, ws, off, out=x),
+                 lambda: M.grouped_matmul_wgrad(dw[0, :11], x, off, out=dw)):
+        with pytest.raises(ValueError, match="overlap an operand"):
+            call()
+    assert not calls
+    wide = torch.zeros((11, 136), dtype=torch.bfloat16)                       # columns of one buffer, before and behind
+    M.grouped_matmul(wide[:, :64], w, off, out=wide[:, 64:128])
+    M.grouped_matmul(wide[:, 72:], w, off, out=wide[:, 8:72])
+    M.grouped_matmul(rows[:11], w, off, out=rows[11:22])
+    M.block_linear(wide[:, :64], wq[0], ws[0], out=wide[:, 72:])
+    M.grouped_matmul(wide[3:4, 64:128], w, off, out=wide[3, :64][None])
+    M.block_linear(wide[:, :64], wq[0], ws[0, :, :], out=wide[:, 64:128])
+    M.grouped_matmul(wide[3, :64][None], w, off, out=wide[3:4, 64:128])
+    assert len(calls) == 7
+    with pytest.raises(ValueError, match="overlap an operand"):
+        M.grouped_matmul(wide[:, :64], w, off, out=wide[:, 56:120])
