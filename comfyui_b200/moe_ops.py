@@ -912,6 +912,16 @@ def _result(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: in
     return out
 
 
+def _rows_of(out: torch.Tensor, shape: Sequence[int]) -> torch.Tensor:
+    """A result of any dimensions as rows, in place."""
+    if out.shape != shape:
+        raise ValueError(f"out must be of shape {tuple(shape)}, or its rows of {shape[-1]}, got {tuple(out.shape)}")
+    try:
+        return out.view(-1, shape[-1])
+    except RuntimeError:
+        raise ValueError(f"out: rows must be equally far apart; got strides {out.stride()}") from None
+
+
 def _once(what: str) -> None:
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} is differentiable once: its gradient has no gradient")
@@ -1158,11 +1168,15 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
     [.., N] in x's dtype.  Differentiable (once, in reverse mode) in x, whose gradient is the same product with the gradient
     of the result quantised and the weight transposed, and in bias; w is frozen."""
     _no_tangents("block_linear", x, w, w_scale, bias)
-    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x.dim() == 0 or w.dim() != 2 or w.size(1) == 0 or x.size(-1) != w.size(1):
+        raise ValueError(f"need rows [.., K] and weights [N, K] that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+    rows = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
     if _asks_for_gradient(x, w, w_scale, bias, out):
         y = _BlockLinear.apply(rows, w, w_scale, bias)
     else:
-        flat = out if out is None or out.dim() == 2 else out.view(-1, out.shape[-1])
+        flat = out
+        if out is not None and out.dim() != 2:
+            flat = _rows_of(out, x.shape[:-1] + w.shape[:1])
         sizes = _block_sizes(rows, w, w_scale, None, None, bias, False)
         y = _block_product(sizes, rows, w, w_scale, None, None, bias, flat, False)
         if out is not None:

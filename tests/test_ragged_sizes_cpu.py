@@ -23,6 +23,10 @@ def meta(*shape, dtype=torch.bfloat16):
     return torch.empty(shape, dtype=dtype, device="meta")
 
 
+def host(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype)
+
+
 def test_sizes_beyond_int32_are_refused(calls):
     """The C entry points count in int32; ctypes would cut a row number down to it and compute a part."""
     from comfyui_b200 import moe_ops as M
@@ -114,3 +118,27 @@ def test_a_result_that_overlaps_an_operand_is_refused(calls):
     assert len(calls) == 7
     with pytest.raises(ValueError, match="overlap an operand"):
         M.grouped_matmul(wide[:, :64], w, off, out=wide[:, 56:120])
+
+
+def test_shapes_of_a_block_linear_are_checked(calls):
+    """Leading dimensions of a given result are those of the rows; what cannot be read or written as rows is refused."""
+    from comfyui_b200 import moe_ops as M
+
+    n, k = 48, 64
+    x, w, ws = host(2, 3, k), host(n, k, dtype=torch.float8_e4m3fn), host(1, 1, dtype=torch.float32)
+    for call, match in ((lambda: M.block_linear(x, w, ws, out=host(3, 2, n)), "out must be of shape"),
+                        (lambda: M.block_linear(x, w, ws, out=host(1, 6, n)), "out must be of shape"),
+                        (lambda: M.block_linear(x, w, ws, out=host(2, 3, n + 8)), "out must be of shape"),
+                        (lambda: M.block_linear(x[0, 0], w, ws, out=host(1, 1, n)), "out must be of shape"),
+                        (lambda: M.block_linear(x, w, ws, out=host(3, 2, n).transpose(0, 1)), "equally far apart"),
+                        (lambda: M.block_linear(host(), w, ws), "that fit"), (lambda: M.block_linear(x, w[0], ws), "that fit"),
+                        (lambda: M.block_linear(host(0, 0), host(n, 0, dtype=w.dtype), ws), "that fit"),
+                        (lambda: M.block_linear(x, w[None], ws), "that fit"), (lambda: M.block_linear(x[..., :48], w, ws), "that fit")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not calls
+    for rows, out in ((x, host(2, 3, n)), (x, host(6, n)), (x, host(2, 3, n + 8)[..., :n]), (x[0, 0], host(n)), (x[0, 0], host(1, n)),
+                      (x[0], host(3, n)), (x[:0], host(0, 3, n))):
+        assert M.block_linear(rows, w, ws, out=out) is out
+    assert M.block_linear(x, w, ws).shape == (2, 3, n) and M.block_linear(x[0, 0], w, ws).shape == (n,)
+    assert len(calls) == 9
