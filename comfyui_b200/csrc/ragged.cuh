@@ -21,10 +21,37 @@ constexpr int kStatusRaggedProducer = 10;
 constexpr int kStatusRaggedMma = 11;
 constexpr int kStatusRaggedEpilogue = 12;
 
-// The groups' rows, made by one warp of every block from what the caller left on the device:
+// The rows of 32 groups, one to a lane of a whole warp, from what the caller left on the device:
 //   begin[g] = max(offsets[0 .. g]) clipped to [0, rows],  end = the same up to g + 1,  count[g] = at most counts[g].
 // Offsets that do not rise therefore give empty groups, never rows outside the buffers or rows that two groups share.
-// first_tile[g] = tiles of the groups before g, for tiles of `tile_rows` rows (of one fixed number where tile_rows is 0).
+// `reach` carries the maximum from the 32 groups before these to the next ones; a lane behind the last group has no rows.
+__device__ __forceinline__ void ragged_chunk(const int32_t* offsets, const int32_t* counts, int groups, int rows, int g,
+                                             int& reach, int& begin, int& count) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = 0, most = 0;
+  if (g < groups) {
+    if (offsets) {
+      lo = min(max(offsets[g], 0), rows);
+      hi = min(max(offsets[g + 1], 0), rows);
+    } else {
+      hi = rows;                               // one group: all rows
+    }
+    most = counts ? max(counts[g], 0) : rows;
+  }
+  lo = max(lo, reach);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, max(lo, hi), d);
+    if (lane >= d) lo = max(lo, v);
+  }
+  hi = max(lo, hi);
+  begin = lo;
+  count = min(hi - lo, most);
+  reach = __shfl_sync(0xffffffffu, hi, 31);
+}
+
+// All groups' rows, made by one warp of every block.  first_tile[g] = tiles of the groups before g, for tiles of `tile_rows`
+// rows (of one fixed number where tile_rows is 0).
 __device__ __forceinline__ void ragged_ranges(const int32_t* offsets, const int32_t* counts, int groups, int rows,
                                               int tile_rows, int tiles_per_row_tile, int* begin, int* count,
                                               int* first_tile) {
@@ -32,24 +59,8 @@ __device__ __forceinline__ void ragged_ranges(const int32_t* offsets, const int3
   int reach = 0, tiles = 0;                    // carried from one chunk of 32 groups to the next
   for (int g0 = 0; g0 < groups; g0 += 32) {
     const int g = g0 + lane;
-    int lo = 0, hi = 0, most = 0;
-    if (g < groups) {
-      if (offsets) {
-        lo = min(max(offsets[g], 0), rows);
-        hi = min(max(offsets[g + 1], 0), rows);
-      } else {
-        hi = rows;                             // one group: all rows
-      }
-      most = counts ? max(counts[g], 0) : rows;
-    }
-    lo = max(lo, reach);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, max(lo, hi), d);
-      if (lane >= d) lo = max(lo, v);
-    }
-    hi = max(lo, hi);
-    const int n = min(hi - lo, most);
+    int lo, n;
+    ragged_chunk(offsets, counts, groups, rows, g, reach, lo, n);
     const int mine = g < groups ? (tile_rows ? (n + tile_rows - 1) / tile_rows : 1) * tiles_per_row_tile : 0;
     int upto = mine;
 #pragma unroll
@@ -62,7 +73,6 @@ __device__ __forceinline__ void ragged_ranges(const int32_t* offsets, const int3
       count[g] = n;
       first_tile[g] = tiles + upto - mine;
     }
-    reach = __shfl_sync(0xffffffffu, hi, 31);
     tiles += __shfl_sync(0xffffffffu, upto, 31);
   }
   if (lane == 0) first_tile[groups] = tiles;
