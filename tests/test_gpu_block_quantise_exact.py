@@ -111,3 +111,27 @@ def test_fp32_blocks_of_zeros_tiny_and_not_finite_values(cuda_device):
     assert torch.isnan(q[2, :128].float()).all() and torch.isnan(scale[2, 0]) and (byte[2, 128:] == 0).all()
     assert torch.isnan(q[3, 7].float()) and torch.isinf(scale[3, 0]) and byte[3, 8] == 128 and byte[3, 9] == 0
     assert q[4, 130].float() == 448 and byte[4, 131] == 0 and byte[4, 132] == 128 and torch.isfinite(scale[4]).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_every_ratio_of_bf16_significands(cuda_device, sign):
+    """x / m for all 128 significands of both, powers of two among them, over every power of two that e4m3 covers."""
+    from comfyui_b200 import moe_ops as M
+
+    dev = cuda_device
+    sig = torch.arange(128, 256, device=dev).double()
+    x = (sig[:, None] / 2.0 ** torch.arange(20, device=dev).double()).flatten()          # 255 down to 2^-12
+    x = sign * torch.nn.functional.pad(x, (0, -x.numel() % (BLOCK - 1)), value=1.0).view(-1, BLOCK - 1)
+    alternate = torch.where(torch.arange(BLOCK - 1, device=dev) % 2 == 0, 1.0, -1.0)
+    x = (x * alternate)[None].expand(128, -1, -1)
+    m = (2 * sig)[:, None, None].expand(128, x.shape[1], 1)                             # a place of its own in every block
+    rows = torch.cat([m, x], 2)
+    for s in sig.tolist():
+        assert (rows[0, :, 1:].abs() == s).any()
+    rows, tops = rows.reshape(128, -1).bfloat16(), m.expand(-1, -1, BLOCK).reshape(128, -1)
+    assert torch.equal(rows.view(128, -1, BLOCK).abs().amax(2).double(), m[:, :, 0])
+    q, scale = M.quantize_blocks_e4m3(rows)
+    assert torch.equal(q.view(torch.uint8), nearest(rows, tops))
+    assert torch.equal(scale, (m[:, :, 0] / 448.0).float())
+    q, scale = M.quantize_blocks_e4m3(rows.float())
+    assert torch.equal(q.view(torch.uint8), nearest(rows, tops))
