@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import weakref
 from dataclasses import dataclass, field
+from types import SimpleNamespace
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -51,12 +52,14 @@ _device_status = {}
 
 def device_status(device) -> torch.Tensor:
     """The status word shared by every call on `device` that brings no workspace of its own (dense feed-forwards)."""
-    key = str(device)
-    st = _device_status.get(key)
+    st = _device_status.get(device)                # (a device object finds it without being spelled out)
     if st is None:
-        st = torch.zeros((N.STATUS_WORDS,), dtype=torch.int32, device=device)
-        _device_status[key] = st
-        _status_words.add(st)
+        st = _device_status.get(str(device))
+        if st is None:
+            st = torch.zeros((N.STATUS_WORDS,), dtype=torch.int32, device=device)
+            _device_status[str(device)] = st
+            _status_words.add(st)
+        _device_status[device] = st
     return st
 
 
@@ -780,6 +783,8 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 # --------------------------------------------------------------------------------------- products over ragged rows
 # These calls last from a few microseconds on, so the way to the C entry points is kept short: plain integers instead of
 # ctypes objects, one pass of checks, no context manager where the tensors are on the current device.
+_MAX_ROWS, _MAX_FEATURES = N.RAGGED_MAX_ROWS, N.RAGGED_MAX_FEATURES      # what C takes as int32: ctypes would cut more down
+_MAX_BLOCKED = N.MAX_SCALE_BLOCKS * N.SCALE_BLOCK
 _HALF_CODES = {torch.bfloat16: N.BF16, torch.float16: N.FP16}
 
 
@@ -788,12 +793,13 @@ def _raw_stream(index: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)       # the same without a Stream object
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # without looking whether CUDA is up
 
 
 def _call(name: str, index: int, *args) -> None:
     """One C entry point on the current stream of the tensors' device, which need not be the current device."""
     fn = getattr(N.load(), name)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -822,9 +828,10 @@ def _place(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
 def _row_stride(what: str, t: torch.Tensor, unit: int) -> int:
     """Elements from one row of t [.., rows, cols] to the next, where the kernels can read and write it as it is: `unit`
     elements are 16 bytes."""
-    cols = t.size(-1)
-    ld = cols if t.size(-2) <= 1 else t.stride(-2)
-    if cols % unit or ld % unit or ld < cols or t.data_ptr() % 16 or (t.stride(-1) != 1 and cols > 1):
+    shape, strides = t.shape, t.stride()           # (as tuples: size(i) and stride(i) take twice as long each)
+    cols = shape[-1]
+    ld = cols if shape[-2] <= 1 else strides[-2]
+    if cols % unit or ld % unit or ld < cols or t.data_ptr() % 16 or (strides[-1] != 1 and cols > 1):
         raise ValueError(f"{what}: rows must be contiguous, of a multiple of {unit} elements, and start on 16 bytes; "
                          f"got shape {tuple(t.shape)}, strides {t.stride()}")
     return ld
@@ -832,9 +839,9 @@ def _row_stride(what: str, t: torch.Tensor, unit: int) -> int:
 
 def _group_stride(what: str, t: torch.Tensor, unit: int) -> int:
     """Elements from one group of t [G, rows, cols] to the next."""
-    if t.size(0) <= 1:
+    if t.shape[0] <= 1:
         return 0
-    step = t.stride(0)
+    step = t.stride()[0]
     if step <= 0 or step % unit:
         raise ValueError(f"{what}: groups must start on 16 bytes; got strides {t.stride()}")
     return step
@@ -845,11 +852,17 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     saved-tensor hook gives back), as rows that the kernels can read."""
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t
-    unit = 16 // t.element_size()
-    rows, cols = t.size(-2), t.size(-1)
-    ok = t.stride(-1) == 1 and (rows <= 1 or (t.stride(-2) >= cols and t.stride(-2) % unit == 0)) and \
-        (t.dim() == 2 or t.size(0) <= 1 or (t.stride(0) > 0 and t.stride(0) % unit == 0)) and t.data_ptr() % 16 == 0
+    unit, shape, strides = 16 // t.element_size(), t.shape, t.stride()
+    ok = strides[-1] == 1 and (shape[-2] <= 1 or (strides[-2] >= shape[-1] and strides[-2] % unit == 0)) and \
+        (len(shape) == 2 or shape[0] <= 1 or (strides[0] > 0 and strides[0] % unit == 0)) and t.data_ptr() % 16 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _unchanged(t: Optional[torch.Tensor], shape: tuple, strides: tuple, dtype: torch.dtype, index: int, unit: int = 1) -> bool:
+    """Whether a saved tensor came back with the strides that the forward pass measured (a dimension of one element, whose
+    stride it did not look at, says no: the checked calls then decide)."""
+    return t is None or (t.stride() == strides and t.shape == shape and t.dtype == dtype and t.get_device() == index and
+                         t.data_ptr() % unit == 0)
 
 
 def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -857,21 +870,18 @@ def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.contiguous()
 
 
-def _check_sizes(rows: int, *features: int) -> None:
-    """Sizes that the C entry points take as int32, before ctypes cuts them to it."""
-    if rows > N.RAGGED_MAX_ROWS or min(features) == 0 or max(features) > N.RAGGED_MAX_FEATURES:
-        raise ValueError(f"at most {N.RAGGED_MAX_ROWS} rows and 1 to {N.RAGGED_MAX_FEATURES} features, got {rows} and {features}")
+def _refuse_sizes(rows: int, *features: int) -> None:
+    raise ValueError(f"at most {N.RAGGED_MAX_ROWS} rows and 1 to {N.RAGGED_MAX_FEATURES} features, got {rows} and {features}")
 
 
-def _check_blocks(*sizes: int) -> None:
-    if max(sizes) > N.MAX_SCALE_BLOCKS * N.SCALE_BLOCK:
-        raise ValueError(f"at most {N.MAX_SCALE_BLOCKS} blocks of {N.SCALE_BLOCK} along a dimension, got {sizes} elements")
+def _refuse_blocks(*sizes: int) -> None:
+    raise ValueError(f"at most {N.MAX_SCALE_BLOCKS} blocks of {N.SCALE_BLOCK} along a dimension, got {sizes} elements")
 
 
 def _check_ragged(offsets: torch.Tensor, counts: Optional[torch.Tensor], groups: int) -> None:
     if groups > N.RAGGED_MAX_GROUPS:
         raise ValueError(f"at most {N.RAGGED_MAX_GROUPS} groups, got {groups}")
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.size(0) != groups + 1 or not offsets.is_contiguous():
+    if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_contiguous():
         raise ValueError(f"offsets must be a contiguous int32 vector of {groups + 1} elements")
     if counts is not None and (counts.dtype != torch.int32 or counts.shape != (groups,) or not counts.is_contiguous()):
         raise ValueError(f"counts must be a contiguous int32 vector of {groups} elements")
@@ -927,12 +937,16 @@ def _once(what: str) -> None:
         raise RuntimeError(f"{what} is differentiable once: its gradient has no gradient")
 
 
+# The level that is open, -1 for none (a torch without the name: every call looks at its tensors).
+_forward_ad = torch.autograd.forward_ad if hasattr(torch.autograd.forward_ad, "_current_level") else \
+    SimpleNamespace(_current_level=0)
+
+
 def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether one of them is a dual tensor of a forward-mode derivative that is being taken."""
-    if getattr(torch.autograd.forward_ad, "_current_level", 0) < 0:
-        return False
-    return any(t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
-               for t in tensors)
+    return _forward_ad._current_level >= 0 and any(
+        t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+        for t in tensors)
 
 
 def _no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -945,16 +959,18 @@ def _grouped_sizes(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
                    width: int) -> tuple:
     """What the C entry points want to know of checked rows and weights: (device index, dtype code, rows, groups, N, K,
     row stride of a, row and group stride of w)."""
-    if a.dim() != 2 or w.dim() != 3 or a.size(1) != w.size(width):
-        raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(a.shape)} and {tuple(w.shape)}")
+    shape, weights = a.shape, w.shape
+    if len(shape) != 2 or len(weights) != 3 or shape[1] != weights[width]:
+        raise ValueError(f"need rows [R, K] and weights [G, N, K] that fit, got {tuple(shape)} and {tuple(weights)}")
     index = _place(a, w, offsets, counts)
     code = _HALF_CODES.get(a.dtype)
     if code is None or w.dtype != a.dtype:
         raise ValueError(f"rows and weights must both be bf16 or both fp16, got {a.dtype} and {w.dtype}")
-    g, n, k = w.shape
-    _check_sizes(a.size(0), n, k)
+    r, (g, n, k) = shape[0], weights
+    if not (r <= _MAX_ROWS and 0 < n <= _MAX_FEATURES and 0 < k <= _MAX_FEATURES):
+        _refuse_sizes(r, n, k)
     _check_ragged(offsets, counts, g)
-    return (index, code, a.size(0), g, n, k, _row_stride("rows", a, 8), _row_stride("weights", w, 8),
+    return (index, code, r, g, n, k, _row_stride("rows", a, 8), _row_stride("weights", w, 8),
             _group_stride("weights", w, 8))
 
 
@@ -980,7 +996,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, coun
     the host.  Rows of no group are zero in a result that this function makes, and stay as they were in ``out``, which
     overlaps no operand.
     Differentiable in x and w (once, in reverse mode); a group without rows has the gradient 0."""
-    _no_tangents("grouped_matmul", x, w)
+    if _forward_ad._current_level >= 0:
+        _no_tangents("grouped_matmul", x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         if out is not None:
             raise ValueError("grouped_matmul: out cannot be given where a gradient is asked for")
@@ -1005,7 +1022,8 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     if offsets.numel() == 0:
         raise ValueError("offsets must have one element more than there are groups")
     g, (r, n), k = offsets.numel() - 1, dy.shape, x.size(1)
-    _check_sizes(r, n, k)
+    if not (r <= _MAX_ROWS and 0 < n <= _MAX_FEATURES and 0 < k <= _MAX_FEATURES):
+        _refuse_sizes(r, n, k)
     index = _place(x, dy, offsets, counts, out)
     code = _HALF_CODES.get(x.dtype)
     if code is None or dy.dtype != x.dtype:
@@ -1036,18 +1054,33 @@ class _GroupedMatmul(torch.autograd.Function):
     def forward(ctx, x, w, offsets, counts):
         need_x, need_w = ctx.needs_input_grad[:2]         # each gradient reads the other operand: keep no more than that
         ctx.save_for_backward(x if need_w else None, w if need_x else None, offsets, counts)
-        sizes = _grouped_sizes(x, w, offsets, counts, 2)
+        ctx.sizes = sizes = _grouped_sizes(x, w, offsets, counts, 2)
         return _rows_by_group("comfy_moe_grouped_matmul", sizes, x, w, offsets, counts, None, sizes[4])
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_matmul")
-        # a saved-tensor hook (offloading, compression) may give back tensors of other strides, so all are measured again
         x, w, offsets, counts = ctx.saved_tensors
-        offsets, counts, dy = _vector(offsets), _vector(counts), _readable(dy)
+        index, code, r, g, n, k, ld_x, ld_w, step = ctx.sizes
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx = grouped_matmul_dgrad(dy, _readable(w), offsets, counts) if need_x else None
-        dw = grouped_matmul_wgrad(dy, _readable(x), offsets, counts) if need_w else None
+        dy, dtype, vec = _readable(dy), dy.dtype, torch.int32
+        if not (_unchanged(x, (r, k), (ld_x, 1), dtype, index, 16) and _unchanged(offsets, (g + 1,), (1,), vec, index) and
+                _unchanged(w, (g, n, k), (step, ld_w, 1), dtype, index, 16) and _unchanged(counts, (g,), (1,), vec, index)):
+            # a saved-tensor hook (offloading, compression) gave back something else: the checked calls look at it anew
+            offsets, counts = _vector(offsets), _vector(counts)
+            return (grouped_matmul_dgrad(dy, _readable(w), offsets, counts) if need_x else None,
+                    grouped_matmul_wgrad(dy, _readable(x), offsets, counts) if need_w else None, None, None)
+        ld_dy = n if r <= 1 else dy.stride()[0]
+        dx = dw = None
+        if need_x:
+            sizes = (index, code, r, g, n, k, ld_dy, ld_w, step)
+            dx = _rows_by_group("comfy_moe_grouped_matmul_dgrad", sizes, dy, w, offsets, counts, None, k)
+        if need_w:
+            dw = x.new_empty((g, n, k))
+            if g:
+                _call("comfy_moe_grouped_matmul_wgrad", index, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, r, g, n, k,
+                      offsets.data_ptr(), _address(counts), code, dw.data_ptr(), k, n * k,
+                      device_status(x.device).data_ptr())
         return dx, dw, None, None
 
 
@@ -1067,8 +1100,8 @@ def quantize_blocks_e4m3(x: torch.Tensor):
     if x.dim() != 2 or x.dtype not in _QUANT_CODES or x.shape[1] == 0 or x.shape[1] % 16:
         raise ValueError("x must be [R, K] in bf16, fp16 or fp32 with K a multiple of 16")
     r, k = x.shape
-    _check_sizes(r, k)
-    _check_blocks(k)
+    if r > _MAX_ROWS or k > _MAX_BLOCKED:
+        _refuse_sizes(r, k) if r > _MAX_ROWS else _refuse_blocks(k)
     q = torch.empty((r, k), dtype=_FP8, device=x.device)
     scale = torch.empty((_blocks(k), r), dtype=torch.float32, device=x.device)
     _call("comfy_moe_block_quantize", index, x.data_ptr(), _row_stride("x", x, 16 // x.element_size()),
@@ -1084,7 +1117,8 @@ def quantize_weight_blocks_e4m3(w: torch.Tensor):
         raise ValueError("w must be [N, K] or [G, N, K] in bf16, fp16 or fp32 with K a multiple of 16")
     n, k = w.shape[-2:]
     groups = w.shape[0] if w.dim() == 3 else 1
-    _check_blocks(n, k, groups * N.SCALE_BLOCK)
+    if max(n, k, groups * N.SCALE_BLOCK) > _MAX_BLOCKED:
+        _refuse_blocks(n, k, groups * N.SCALE_BLOCK)
     unit = 16 // w.element_size()
     q = torch.empty(w.shape, dtype=_FP8, device=w.device)
     scale = torch.empty(w.shape[:-2] + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
@@ -1098,28 +1132,30 @@ def _block_sizes(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offset
                  counts: Optional[torch.Tensor], bias: Optional[torch.Tensor], transpose: bool) -> tuple:
     """What the C entry point wants to know of checked operands: (device index, dtype code, rows, groups, N, K, row stride
     of x, row and group stride of w).  offsets None: one group, w [N, K]; transpose: x is a gradient [R, N]."""
-    if w.dim() != (2 if offsets is None else 3) or x.dim() != 2 or x.size(1) != w.size(-2 if transpose else -1):
-        raise ValueError(f"need rows and weights that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+    shape, weights = x.shape, w.shape
+    if len(weights) != (2 if offsets is None else 3) or len(shape) != 2 or shape[1] != weights[-2 if transpose else -1]:
+        raise ValueError(f"need rows and weights that fit, got {tuple(shape)} and {tuple(weights)}")
     index = _place(x, w, w_scale, offsets, counts, bias)
     code = _HALF_CODES.get(x.dtype)
     if code is None or w.dtype != _FP8:
         raise ValueError(f"rows must be bf16 or fp16 and weights e4m3, got {x.dtype} and {w.dtype}")
-    r, contraction = x.shape
-    n, k = w.size(-2), w.size(-1)
+    (r, contraction), (n, k) = shape, weights[-2:]
     if n % 8 or k % 16 or contraction % 16 or n == 0 or k == 0:
         raise ValueError(f"in_features must be a multiple of 16 and out_features of 8 (of 16 for a gradient), got {k} and {n}")
-    _check_sizes(r, n, k)
-    _check_blocks(contraction)
+    if r > _MAX_ROWS or n > _MAX_FEATURES or k > _MAX_FEATURES:
+        _refuse_sizes(r, n, k)
+    if contraction > _MAX_BLOCKED:
+        _refuse_blocks(contraction)
     nb, kb = _blocks(n), _blocks(k)
-    if w_scale.dtype != torch.float32 or w_scale.shape != ((nb, kb) if offsets is None else (w.size(0), nb, kb)) or \
+    if w_scale.dtype != torch.float32 or w_scale.shape != ((nb, kb) if offsets is None else (weights[0], nb, kb)) or \
             not w_scale.is_contiguous():
         raise ValueError(f"the scales must be a contiguous fp32 tensor [.., {nb}, {kb}] for each group")
     groups = step = 1
     if offsets is not None:
-        groups = w.size(0)
+        groups = weights[0]
         _check_ragged(offsets, counts, groups)
         step = _group_stride("weights", w, 16)
-    if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.size(0) != n or not bias.is_contiguous() or
+    if bias is not None and (bias.dtype != x.dtype or bias.shape != (n,) or not bias.is_contiguous() or
                              bias.data_ptr() % 16):
         raise ValueError("bias must be a contiguous vector over the output features in the rows' dtype")
     return index, code, r, groups, n, k, _row_stride("rows", x, 8), _row_stride("weights", w, 16), step
@@ -1155,8 +1191,8 @@ def _asks_for_gradient(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, 
         return False
     if out is not None:
         raise ValueError("out cannot be given where a gradient is asked for")
-    if x.requires_grad and w.shape[-2] % 16:
-        raise ValueError(f"out_features must be a multiple of 16 for a gradient of the rows, got {w.shape[-2]}")
+    if x.requires_grad and w.dim() > 1 and w.size(-2) % 16:
+        raise ValueError(f"out_features must be a multiple of 16 for a gradient of the rows, got {w.size(-2)}")
     return True
 
 
@@ -1167,10 +1203,13 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
     bias [N] in x's dtype; K a multiple of 16, N of 8 (of 16 where a gradient of x is asked for); sums in fp32, result
     [.., N] in x's dtype.  Differentiable (once, in reverse mode) in x, whose gradient is the same product with the gradient
     of the result quantised and the weight transposed, and in bias; w is frozen."""
-    _no_tangents("block_linear", x, w, w_scale, bias)
-    if x.dim() == 0 or w.dim() != 2 or w.size(1) == 0 or x.size(-1) != w.size(1):
-        raise ValueError(f"need rows [.., K] and weights [N, K] that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
-    rows = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
+    if _forward_ad._current_level >= 0:
+        _no_tangents("block_linear", x, w, w_scale, bias)
+    rows = x
+    if x.dim() != 2 or x.size(1) == 0:
+        if x.dim() == 0 or x.size(-1) == 0:
+            raise ValueError(f"need rows [.., K] and weights [N, K] that fit, got {tuple(x.shape)} and {tuple(w.shape)}")
+        rows = x.reshape(-1, x.size(-1))
     if _asks_for_gradient(x, w, w_scale, bias, out):
         y = _BlockLinear.apply(rows, w, w_scale, bias)
     else:
@@ -1195,7 +1234,8 @@ def grouped_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor
     """block_linear by expert: ``y[r] = x[r] @ (w[g] * scales[g]).T`` for the rows r of group g.  x [R, K], w e4m3
     [G, N, K], w_scale [G, ceil(N / 128), ceil(K / 128)]; offsets, counts, out and rows of no group as for grouped_matmul,
     the quantised rows and the gradient (x only) as for block_linear."""
-    _no_tangents("grouped_block_linear", x, w, w_scale)
+    if _forward_ad._current_level >= 0:
+        _no_tangents("grouped_block_linear", x, w, w_scale)
     if _asks_for_gradient(x, w, w_scale, None, out):
         return _GroupedBlockLinear.apply(x, w, w_scale, offsets, counts)
     sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
@@ -1209,20 +1249,36 @@ def grouped_block_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, w_scale: torch
     return _block_product(sizes, dy, w, w_scale, offsets, counts, None, out, True)
 
 
+def _block_backward(ctx, dy: torch.Tensor, w, w_scale, offsets, counts) -> torch.Tensor:
+    index, code, r, g, n, k, _, ld_w, step = ctx.sizes
+    scales, vec = (-(-n // N.SCALE_BLOCK), -(-k // N.SCALE_BLOCK)), torch.int32
+    if offsets is None:
+        shape, strides = (n, k), (ld_w, 1)
+    else:
+        shape, strides, scales = (g, n, k), (step, ld_w, 1), (g, *scales)
+    dy = _readable(dy)
+    if _unchanged(w, shape, strides, _FP8, index, 16) and _unchanged(offsets, (g + 1,), (1,), vec, index) and \
+            _unchanged(counts, (g,), (1,), vec, index) and w_scale.is_contiguous() and w_scale.shape == scales and \
+            w_scale.dtype == torch.float32 and w_scale.get_device() == index:
+        sizes = (index, code, r, g, n, k, n if r <= 1 else dy.stride()[0], ld_w, step)
+    else:                                         # a saved-tensor hook gave back something else
+        w, w_scale, offsets, counts = _readable(w), _vector(w_scale), _vector(offsets), _vector(counts)
+        sizes = _block_sizes(dy, w, w_scale, offsets, counts, None, True)
+    return _block_product(sizes, dy, w, w_scale, offsets, counts, None, None, True)
+
+
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, bias):
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(w, w_scale)
-        return _block_product(_block_sizes(x, w, w_scale, None, None, bias, False), x, w, w_scale, None, None, bias, None, False)
+        ctx.sizes = sizes = _block_sizes(x, w, w_scale, None, None, bias, False)
+        return _block_product(sizes, x, w, w_scale, None, None, bias, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("block_linear")
-        dx = None
-        if ctx.needs_input_grad[0]:
-            w, w_scale = ctx.saved_tensors                # (of any strides: a saved-tensor hook may have copied them)
-            dx = block_linear_dgrad(_readable(dy), _readable(w), _vector(w_scale))
+        dx = _block_backward(ctx, dy, *ctx.saved_tensors, None, None) if ctx.needs_input_grad[0] else None
         db = dy.sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, db
 
@@ -1231,12 +1287,10 @@ class _GroupedBlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_scale, offsets, counts):
         ctx.save_for_backward(w, w_scale, offsets, counts)
-        sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
+        ctx.sizes = sizes = _block_sizes(x, w, w_scale, offsets, counts, None, False)
         return _block_product(sizes, x, w, w_scale, offsets, counts, None, None, False)
 
     @staticmethod
     def backward(ctx, dy):
         _once("grouped_block_linear")
-        w, w_scale, offsets, counts = ctx.saved_tensors
-        dx = grouped_block_linear_dgrad(_readable(dy), _readable(w), _vector(w_scale), _vector(offsets), _vector(counts))
-        return dx, None, None, None, None
+        return _block_backward(ctx, dy, *ctx.saved_tensors), None, None, None, None
