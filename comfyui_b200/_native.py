@@ -11,7 +11,7 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int6
 
 from . import build as _build
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 OK, EINVAL, EUNSUPPORTED, ECUDA, ETIMEOUT, EDEVICE, ETOOLARGE = range(7)
 BF16, FP32, FP8_E4M3, FP16 = 0, 1, 2, 3
@@ -54,6 +54,7 @@ EXPORTS = (
     "comfy_moe_combine_block",
     "comfy_moe_ffn_block",
     "comfy_moe_read_status",
+    "comfy_moe_relax_capture",
     "comfy_moe_quantize_e4m3",
     "comfy_moe_stochastic_round_e4m3",
     "comfy_moe_quantize_weight_e4m3",
@@ -293,6 +294,7 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
     lib.comfy_moe_ffn_block.argtypes = [POINTER(Layer), POINTER(Workspace), c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_int64, c_int, c_int, c_float, c_void_p, c_void_p]
     lib.comfy_moe_read_status.argtypes = [c_void_p, c_void_p, POINTER(c_int32)]
+    lib.comfy_moe_relax_capture.argtypes = [POINTER(c_int)]
     lib.comfy_moe_ep_dispatch.argtypes = [
         POINTER(PeerPlan), c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

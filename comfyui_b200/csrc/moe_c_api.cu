@@ -33,6 +33,14 @@ extern "C" int comfy_moe_read_status(int32_t* status, void* stream, int32_t* h_s
   return COMFY_MOE_ETIMEOUT;
 }
 
+extern "C" int comfy_moe_relax_capture(int* relaxed) {
+  if (!relaxed) return COMFY_MOE_EINVAL;
+  cudaStreamCaptureMode mode = *relaxed ? cudaStreamCaptureModeRelaxed : cudaStreamCaptureModeGlobal;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return COMFY_MOE_ECUDA;
+  *relaxed = mode == cudaStreamCaptureModeRelaxed;
+  return COMFY_MOE_OK;
+}
+
 // Block epilogue requested by comfy_moe_ffn_block: gate * (.) + residual folded into the combine.
 struct BlockEpilogue {
   const void* gate;

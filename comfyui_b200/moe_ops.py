@@ -50,13 +50,31 @@ _status_words = weakref.WeakSet()
 _device_status = {}
 
 
+def _lasting_zeros(device) -> torch.Tensor:
+    """A zeroed status block outside every CUDA graph: what a capture allocates belongs to the graph's memory pool, where the
+    temporaries of other graphs may lie over it, and its zeroing would be repeated by every replay."""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            return torch.zeros((N.STATUS_WORDS,), dtype=torch.int32, device=device)
+        relaxed, lib = ctypes.c_int(1), N.load()
+        N.check("comfy_moe_relax_capture", lib.comfy_moe_relax_capture(relaxed))
+        try:
+            side = torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                block = torch.zeros((N.STATUS_WORDS,), dtype=torch.int32, device=device)
+            side.synchronize()
+        finally:
+            N.check("comfy_moe_relax_capture", lib.comfy_moe_relax_capture(relaxed))
+        return block
+
+
 def device_status(device) -> torch.Tensor:
     """The status word shared by every call on `device` that brings no workspace of its own (dense feed-forwards)."""
     st = _device_status.get(device)                # (a device object finds it without being spelled out)
     if st is None:
         st = _device_status.get(str(device))
         if st is None:
-            st = torch.zeros((N.STATUS_WORDS,), dtype=torch.int32, device=device)
+            st = _lasting_zeros(device)
             _device_status[str(device)] = st
             _status_words.add(st)
         _device_status[device] = st

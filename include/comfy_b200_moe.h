@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define COMFY_MOE_ABI_VERSION 10
+#define COMFY_MOE_ABI_VERSION 11
 
 /* Return codes. */
 #define COMFY_MOE_OK 0
@@ -582,6 +582,10 @@ int comfy_moe_ffn_block(const ComfyMoeLayer* h_layer, const ComfyMoeWorkspace* h
  * COMFY_MOE_ETIMEOUT for any other code; a non-zero word is cleared once it has
  * been reported. */
 int comfy_moe_read_status(int32_t* status, void* stream, int32_t* h_status);
+
+/* While *relaxed is not 0, calls of this thread that have nothing to do with a capture under way (an allocation, a
+ * synchronisation of another stream) are allowed beside it.  Swaps the state with *relaxed, so a second call puts it back. */
+int comfy_moe_relax_capture(int* relaxed);
 
 #ifdef __cplusplus
 }
