@@ -12,7 +12,7 @@
 // off; s = fl(p + e) lies on the quotient's side of every border that it is not equal to (a border is an fp32 number), and
 // what is left, t, tells the side where it is equal: |t| is above 2^-30 of s then, and below 2^-45 where the quotient is the
 // border.  So s moves by one unit towards t if t counts and s is even, as borders are: onto no border and over none.
-// (8192 x 2560: 21.4 us; ((x * 7 / 16) / m) * 1024, whose product and quotient both round, took 18.4 and missed by a step
+// (8192 x 2560: 22.4 us; ((x * 7 / 16) / m) * 1024, whose product and quotient both round, took 19.4 and missed by a step
 // next to borders.)
 // The floor 2^-100 keeps the scales and their products out of the subnormal range; a block of zeros has zeros.  The maximum is
 // taken on the bit patterns, so a NaN or an infinity wins it and reaches every result the block takes part in: its scale

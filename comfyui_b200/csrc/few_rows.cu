@@ -1,16 +1,17 @@
 // Products of a few rows with weights that are read once: the single-token form of the grouped products and of the
 // block-scaled ones.  At up to 16 rows the weights are all there is to move (2 flops per byte and row), so the work is cut
 // for HBM: a block takes 16 output columns of one group over the whole contraction, its eight warps the chunks of it in
-// turns, and every lane keeps up to ten 16-byte loads of weights in flight.  The arithmetic is one mma.sync tile per eight
-// rows: 16 output columns x 8 rows, A = weights, B = rows, both operands in the registers that the loads filled: the
+// turns, and every lane asks for ten 16-byte pieces of weights before it uses the first.  The arithmetic is one mma.sync tile
+// per eight rows: 16 output columns x 8 rows, A = weights, B = rows, both operands in the registers that the loads filled: the
 // tile's steps of the contraction may come in any order as long as both sides agree, so a lane's 16 contiguous bytes serve
 // two MMAs without a shuffle or shared memory.  (tcgen05 would need both operands in shared memory and 128 rows of one of
 // them.)  The warps' partial sums are joined in a fixed order: the result is the same every time.
-// Measured (device time, us, cold weights, against the tcgen05 kernels): bf16 2560 -> 6912, one group, 1 row 9.9 / 18.5, 16
-// rows 12.7 / 17.7 (HBM: 5.4); four groups, 8 rows 23.5 / 43.2 (all of them busy: 21.6); eight groups 2048 -> 8192, 16 rows
-// 54.4 / 64.1 (41).
-#include <algorithm>
-
+// Measured (device time, us, cold weights, against the tcgen05 kernels): bf16 2560 -> 6912, one group, 1 row 8.1 / 18.5, 16
+// rows 10.6 / 17.7 (HBM: 5.4); four groups, 8 rows 24.0 / 43.2 (all of them busy: 21.6); eight groups 2048 -> 8192, 16 rows
+// 53 / 64 (41).
+// How many of the ten loads are in flight is the compiler's choice of registers.  Four blocks to an SM leave it 64 and are the
+// best of what was measured: with 40, its own choice, it takes them in turns (1 row 10.3, 16 rows 13.3, four groups 25.2, eight
+// 63); three blocks of 80: 8.4, 9.4, 28, 57; two of 96: 11.0, 13.0, 32, 63.
 #include "block_scale.cuh"
 #include "few_rows.cuh"
 #include "ragged.cuh"
@@ -20,17 +21,21 @@ namespace comfy_b200 {
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewCols = 16;                   // output columns per block
+constexpr int kFewBlocks = 4;                  // of the unscaled kernel, to an SM
 
 // No more groups than rows have any: a grid has that many of them, few_slots.  Blocks (., slot) take group `slot` where
 // that is every group, else the slot-th group that has rows; false: there is none for them.  The same in every lane of a warp.
-// (Blocks for every group, busy or not: bf16 1024 -> 2048, 8 rows in 8 of 768 groups 208 us against 23, of 64 groups 20
-// against 11; 2560 -> 6912, 2 rows in 2 of 4 groups 16.9 against 13.5.)
+// (With blocks for every group, busy or not: bf16 1024 -> 2048, 8 rows in 8 of 768 groups 208 us, now 20; of 64 groups 20, now
+// 10; block-scaled 2560 -> 6912, 2 rows in 2 of 4 groups 14.8, now 13.5.)
 __host__ __device__ __forceinline__ int few_slots(const FewParams& p) { return p.groups < p.rows ? p.groups : p.rows; }
 
+// kSeek: groups > rows.  (A variant of its own: with both ways in one kernel 8 block-scaled rows in four groups, 2560 -> 6912,
+// took 23.6 us against 22.2.)
+template <bool kSeek>
 __device__ __forceinline__ bool few_group(const FewParams& p, int slot, int& group, int& begin, int& count) {
   const int lane = threadIdx.x & 31;
   count = 0;
-  if (p.groups <= p.rows) {
+  if constexpr (!kSeek) {
     group = slot;
     if (!p.offsets) {
       begin = 0;
@@ -144,12 +149,12 @@ __device__ __forceinline__ void few_zero(const FewParams& p) {
         *reinterpret_cast<uint4*>(p.out + static_cast<long long>(row) * p.ld_out + b) = make_uint4(0, 0, 0, 0);
 }
 
-template <typename T, int kTiles>
-__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p) {
+template <typename T, int kTiles, bool kSeek>
+__global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_rows_kernel(const FewParams p) {
   __shared__ float part[kFewWarps][kFewCols][8 * kTiles + 1];
   if (blockIdx.y == few_slots(p)) { few_zero(p); return; }
   int grp, begin, count;
-  if (!few_group(p, blockIdx.y, grp, begin, count)) return;
+  if (!few_group<kSeek>(p, blockIdx.y, grp, begin, count)) return;
   const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
   const int n0 = blockIdx.x * kFewCols;
   const uint8_t* w0 = p.w + grp * p.w_group + static_cast<long long>(n0 + g) * p.ld_w;
@@ -187,17 +192,17 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p
 // Block-scaled.  kQuantise: one or two rows are quantised here, by every block again (by the rule of block_scale.cuh; each
 // warp the blocks that it multiplies), while its weights are on their way: no workspace, one launch.  That costs 1.2 us a
 // row at 2560 -> 6912, a launch of the quantiser 1.7 us and the host 3 us, so from three rows on, up to eight, they come
-// quantised.  Measured as above: one group, 1 row 8.5 / 12.7, 8 rows 8.5 / 12.7 (HBM: 2.7); four groups, 8 rows 19.8 / 30.3;
+// quantised.  Measured as above: one group, 1 row 8.3 / 12.7, 8 rows 8.3 / 12.7 (HBM: 2.7); four groups, 8 rows 22.2 / 30.3;
 // 1024 -> 1024, 8 rows 4.9 / 8.5.  (16 rows, two tiles: 12.1 / 12.4, four groups 28.1 / 30.4, eight 50 / 40: left to tcgen05.)
 constexpr int kFewBlk = COMFY_MOE_SCALE_BLOCK;
 
-template <typename T, bool kQuantise>
+template <typename T, bool kQuantise, bool kSeek>
 __global__ void __launch_bounds__(kFewThreads) few_rows_block_kernel(const FewParams p) {
   extern __shared__ __align__(16) uint8_t xq[];            // kQuantise: [blocks of the contraction][rows][128]
   __shared__ float part[kFewWarps][kFewCols][9];
   if (blockIdx.y == few_slots(p)) { few_zero(p); return; }
   int grp, begin, count;
-  if (!few_group(p, blockIdx.y, grp, begin, count)) return;
+  if (!few_group<kSeek>(p, blockIdx.y, grp, begin, count)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * kFewCols;
   const uint8_t* w0 = p.w + grp * p.w_group + static_cast<long long>(n0 + g) * p.ld_w;
@@ -302,25 +307,31 @@ static int launch_few(const FewParams& p, size_t smem, size_t most, cudaStream_t
   return check_launch();
 }
 
-int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
-  if (p.rows <= 8)
-    return fp16 ? launch_few<few_rows_kernel<__half, 1>>(p, 0, 0, stream)
-                : launch_few<few_rows_kernel<__nv_bfloat16, 1>>(p, 0, 0, stream);
-  return fp16 ? launch_few<few_rows_kernel<__half, 2>>(p, 0, 0, stream)
-              : launch_few<few_rows_kernel<__nv_bfloat16, 2>>(p, 0, 0, stream);
+template <typename T, bool kSeek>
+static int launch_rows_typed(const FewParams& p, cudaStream_t stream) {
+  return p.rows <= 8 ? launch_few<few_rows_kernel<T, 1, kSeek>>(p, 0, 0, stream)
+                     : launch_few<few_rows_kernel<T, 2, kSeek>>(p, 0, 0, stream);
 }
 
-template <typename T>
+int launch_few_rows(const FewParams& p, bool fp16, cudaStream_t stream) {
+  if (p.groups > p.rows)
+    return fp16 ? launch_rows_typed<__half, true>(p, stream) : launch_rows_typed<__nv_bfloat16, true>(p, stream);
+  return fp16 ? launch_rows_typed<__half, false>(p, stream) : launch_rows_typed<__nv_bfloat16, false>(p, stream);
+}
+
+template <typename T, bool kSeek>
 static int launch_block_typed(const FewParams& p, cudaStream_t stream) {
   if (p.xs == nullptr)
-    return launch_few<few_rows_block_kernel<T, true>>(
+    return launch_few<few_rows_block_kernel<T, true, kSeek>>(
         p, static_cast<size_t>((p.k + kFewBlk - 1) / kFewBlk) * kFewRowsQuantise * kFewBlk,
         static_cast<size_t>(kFewQuantiseMaxK) * kFewRowsQuantise, stream);
-  return launch_few<few_rows_block_kernel<T, false>>(p, 0, 0, stream);
+  return launch_few<few_rows_block_kernel<T, false, kSeek>>(p, 0, 0, stream);
 }
 
 int launch_few_rows_block(const FewParams& p, bool fp16, cudaStream_t stream) {
-  return fp16 ? launch_block_typed<__half>(p, stream) : launch_block_typed<__nv_bfloat16>(p, stream);
+  if (p.groups > p.rows)
+    return fp16 ? launch_block_typed<__half, true>(p, stream) : launch_block_typed<__nv_bfloat16, true>(p, stream);
+  return fp16 ? launch_block_typed<__half, false>(p, stream) : launch_block_typed<__nv_bfloat16, false>(p, stream);
 }
 
 }  // namespace comfy_b200
