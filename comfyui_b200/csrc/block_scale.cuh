@@ -14,8 +14,10 @@
 // border.  So s moves by one unit towards t if t counts and s is even, as borders are: onto no border and over none.
 // (8192 x 2560: 22.4 us; ((x * 7 / 16) / m) * 1024, whose product and quotient both round, took 19.4 and missed by a step
 // next to borders.)
-// The floor 2^-100 keeps the scales and their products out of the subnormal range; a block of zeros has zeros.  The maximum is
-// taken on the bit patterns, so a NaN or an infinity wins it and reaches every result the block takes part in: its scale
+// The floor 2^-100 keeps a scale normal (2^-109 or more); a block of zeros has zeros.  The product of two scales is taken in
+// fp32: it is subnormal, and loses digits, where the two blocks' maxima multiply to less than 2^-108 (results below 2^-101),
+// and infinite where they multiply to more than 2^145.  The maximum is taken on the bit patterns, so a NaN or an infinity
+// wins it and reaches every result the block takes part in: its scale
 // is then NaN or infinite.
 #pragma once
 #include <type_traits>

@@ -11,7 +11,7 @@
 // 53 / 64 (41).
 // How many of the ten loads are in flight is the compiler's choice of registers.  Four blocks to an SM leave it 64 and are the
 // best of what was measured: with 40, its own choice, it takes them in turns (1 row 10.3, 16 rows 13.3, four groups 25.2, eight
-// 63); three blocks of 80: 8.4, 9.4, 28, 57; two of 96: 11.0, 13.0, 32, 63.
+// 63); five blocks of 48: 8.7, 12.6, 26, 59; three of 80: 8.4, 9.4, 28, 57; two of 96: 11.0, 13.0, 32, 63.
 #include "block_scale.cuh"
 #include "few_rows.cuh"
 #include "ragged.cuh"

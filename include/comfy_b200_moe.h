@@ -401,8 +401,8 @@ int comfy_moe_grouped_matmul_wgrad(const void* dy, int64_t ld_dy, const void* x,
  *                                    elements without transpose_w) and multiplies:
  *                                    out[r, :] = x[r, :] . w[g]^T (+ bias);  transpose_w: out[r, :] = x[r, :] . w[g].
  * Groups of rows, zero_unused, status: as for comfy_moe_grouped_matmul; offsets NULL with n_groups = 1 means all rows.
- * Block products are summed in fp32 and folded, times both scales, into fp32 sums; out (and bias, contiguous) have x's
- * dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes.  Rows and
+ * Block products are summed in fp32 and folded, times the fp32 product of both scales (normal where the two blocks' maxima
+ * multiply to between 2^-108 and 2^145), into fp32 sums; out (and bias, contiguous) have x's dtype.  in_features is a multiple of 16, out_features of 8 (of 16 with transpose_w); rows start on 16 bytes.  Rows and
  * features as above; what is quantised has at most COMFY_MOE_MAX_SCALE_BLOCKS blocks along a row (weights: and along a column,
  * and as many groups). */
 #define COMFY_MOE_SCALE_BLOCK 128
@@ -573,9 +573,10 @@ int comfy_moe_ffn_block(const ComfyMoeLayer* h_layer, const ComfyMoeWorkspace* h
                         int tokens_per_batch, float eps, void* out, void* stream);
 
 /* The device status word.  Kernels move it from 0 to a code when something went wrong on the device (1-3: a bounded
- * wait of the grouped GEMM's producer / MMA / epilogue role ran out; 5: one of the attention kernel's; 7: a peer's flag did not arrive in time; 8: routed
- * rows did not fit a peer receive buffer and were dropped; 9: the routing check found an inconsistency) and never overwrite a code that is already there; no entry
- * point clears it on the way in.  A caller may therefore share one word among all layers of a model and look at it at
+ * wait of the grouped GEMM's producer / MMA / epilogue role ran out; 5: one of the attention kernel's; 7: a peer's flag did
+ * not arrive in time; 8: routed rows did not fit a peer receive buffer and were dropped; 9: the routing check found an
+ * inconsistency; 10-12: a bounded wait of the producer / MMA / epilogue role of a product over ragged rows) and never
+ * overwrite a code that is already there; no entry point clears it on the way in.  A caller may therefore share one word among all layers of a model and look at it at
  * a natural synchronisation point (end of a model forward).
  * comfy_moe_read_status synchronises `stream`, copies status[0] to *h_status and returns COMFY_MOE_OK for 0,
  * COMFY_MOE_ETOOLARGE for code 8, COMFY_MOE_EINVAL for code 9 (comfy_moe_validate_routing found an inconsistency) and
