@@ -87,3 +87,36 @@ def test_the_gradient_of_a_bias_alone(cuda_device):
     for y, b in ((M.block_linear(x, w, ws, leaf), leaf), (lin(x), lin.bias)):
         assert torch.equal(y, want)
         assert torch.equal(torch.autograd.grad(y, b, dy)[0], dy.float().sum(0).bfloat16())
+
+
+@pytest.mark.parametrize("reentrant", [False, True], ids=["hooks", "reentrant"])
+def test_under_checkpointing(cuda_device, reentrant):
+    """Recomputed operands, slices of a wider projection among them, give the gradients of the plain run bit for bit."""
+    from torch.utils.checkpoint import checkpoint
+
+    from comfyui_b200 import moe_ops as M
+
+    dev, k, n = cuda_device, 144, 80
+    gen = torch.Generator(device=dev).manual_seed(6)
+    off = torch.tensor([0, 70, 70, 201], dtype=torch.int32, device=dev)
+    x = torch.randn((201, k), generator=gen, device=dev).bfloat16().requires_grad_(True)
+    w = torch.randn((3, 2 * n, k), generator=gen, device=dev).bfloat16().requires_grad_(True)
+    v = torch.randn((3, k, n), generator=gen, device=dev).bfloat16().requires_grad_(True)
+    wq, ws = M.quantize_weight_blocks_e4m3(torch.randn((64, k), generator=gen, device=dev))
+    bias = torch.randn((64,), generator=gen, device=dev).bfloat16().requires_grad_(True)
+    dy = torch.randn((201, 64), generator=gen, device=dev).bfloat16()
+
+    def block(x, w, v):
+        h = M.grouped_matmul(x, w, off)
+        h = M.grouped_matmul(h[:, :n] * torch.sigmoid(h[:, n:]) + 0 * h[:, n:], v, off) + M.grouped_matmul(h[:, n:], v, off)
+        return M.block_linear(h, wq, ws, bias)
+
+    leaves = (x, w, v, bias)
+    grads = []
+    for run in (block, lambda *a: checkpoint(block, *a, use_reentrant=reentrant)):
+        for t in leaves:
+            t.grad = None
+        run(x, w, v).backward(dy)
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*grads))
+    M.read_status(M.device_status(dev))
